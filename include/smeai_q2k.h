@@ -82,8 +82,9 @@ void smeai_debug_fail_next_allocs(int n);
 
 /* Reads and clears the current device's error word.  Kernels never trap or
  * spin forever: a wait that exceeds its time bound sets bit 0 (timeout) here
- * and the kernel returns early, leaving its outputs incomplete.  Returns 0,
- * or a negative status if the word cannot be read. */
+ * and the kernel returns early, leaving its outputs incomplete; a length,
+ * slot, position or page outside its buffers (smeai_paged.h) sets bit 1 and is
+ * skipped.  Returns 0, or a negative status if the word cannot be read. */
 int smeai_take_device_error(unsigned *code);
 
 /* Repack n_rows x k of block_q2_K (row-major, host or device memory) into the
@@ -107,6 +108,16 @@ int smeai_rms_q8k_quantize(const float *x_dev, int64_t ld_x, int64_t n_cols, int
  * device; NULL = none), each product rounded once, then Q8_K. */
 int smeai_rms_q8k_quantize_w(const float *x_dev, int64_t ld_x, int64_t n_cols, int64_t k, const float *weight_dev,
                              float eps, void *y_q8k_dev, void *stream);
+
+/* The same of x + resid, the residual stream between two linears: the sum
+ * (rounded once to fp32) goes to sum, its RMSNorm with the weight to Q8_K, so
+ * the quants equal smeai_rms_q8k_quantize_w's on that sum bit for bit.  For
+ * linears without a residual epilogue (Q3_K, Q6_K) and for the norm that
+ * follows one.  sum may be x or resid themselves (same pointer and stride);
+ * otherwise it must not overlap them.  k is a multiple of 256 up to 65536. */
+int smeai_add_rms_q8k_quantize(const float *x_dev, int64_t ld_x, const float *resid_dev, int64_t ld_resid,
+                               int64_t n_cols, int64_t k, const float *weight_dev, float eps, float *sum_dev,
+                               int64_t ld_sum, void *y_q8k_dev, void *stream);
 
 /* y[c*ldy + r] = sum_k W[r,k] * X[c,k]  for r < n_rows, c < n_cols: the
  * result of ggml's mul_mat for a Q2_K src0 and Q8_K-quantized src1 (dst

@@ -251,6 +251,21 @@ int smeai_rms_q8k_quantize_w(const float* x_dev, int64_t ld_x, int64_t n_cols, i
   return rms_q8k_quantize(x_dev, ld_x, n_cols, k, eps, y_q8k_dev, as_stream(stream), weight_dev);
 }
 
+int smeai_add_rms_q8k_quantize(const float* x_dev, int64_t ld_x, const float* resid_dev, int64_t ld_resid,
+                               int64_t n_cols, int64_t k, const float* weight_dev, float eps, float* sum_dev,
+                               int64_t ld_sum, void* y_q8k_dev, void* stream) {
+  if (!x_dev || !resid_dev || !sum_dev || !y_q8k_dev) {
+    set_last_error("smeai_add_rms_q8k_quantize: NULL pointer");
+    return kBadArgument;
+  }
+  if ((sum_dev == x_dev && ld_sum != ld_x) || (sum_dev == resid_dev && ld_sum != ld_resid)) {
+    set_last_error("smeai_add_rms_q8k_quantize: a sum in place of an input has that input's row stride");
+    return kBadArgument;
+  }
+  return add_rms_q8k_quantize(x_dev, ld_x, resid_dev, ld_resid, n_cols, k, eps, weight_dev, sum_dev, ld_sum,
+                              y_q8k_dev, as_stream(stream));
+}
+
 int smeai_q2k_mul_mat(const void* w_dev, int64_t n_rows, int64_t k, const void* x_q8k_dev, int64_t n_cols,
                       float* y_dev, size_t ldy, void* stream) {
   const Handle* h = as_fmt(w_dev, kFmtQ2K, "smeai_q2k_mul_mat");

@@ -126,6 +126,9 @@ __device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 
+// Codes of the device error word (see raise_device_error).
+enum DeviceError : unsigned { kDevErrTimeout = 1u, kDevErrBadIndex = 2u };
+
 // ---- mbarrier + bulk-copy (TMA) primitives ---------------------------------
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -180,8 +183,8 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, unsigned parity
     if (global_timer_ns() - t0 > timeout_ns) return false;
   }
 }
-// The same, also giving up as soon as the device error word is set: a
-// producer whose consumers left early (a wait of theirs gave up) stops
+// The same, also giving up as soon as the device error word says a wait timed
+// out: a producer whose consumers left early (a wait of theirs gave up) stops
 // instead of waiting out its own limit for slots nobody will free.
 __device__ __forceinline__ bool mbar_wait_or_error(uint64_t* bar, unsigned parity, uint64_t timeout_ns,
                                                    const unsigned* err) {
@@ -190,7 +193,7 @@ __device__ __forceinline__ bool mbar_wait_or_error(uint64_t* bar, unsigned parit
   for (;;) {
     for (int i = 0; i < 64; ++i)
       if (mbar_try_wait(bar, parity)) return true;
-    if (*reinterpret_cast<const volatile unsigned*>(err)) return false;
+    if (*reinterpret_cast<const volatile unsigned*>(err) & kDevErrTimeout) return false;
     if (global_timer_ns() - t0 > timeout_ns) return false;
   }
 }
@@ -209,11 +212,11 @@ __device__ __forceinline__ void bulk_copy_g2s(void* dst, const void* src, unsign
       : "memory");
 }
 
-// Device-side error word: a kernel whose bounded wait expires ORs a code
-// into it and returns instead of hanging or trapping; the host reads and
-// clears it with device_error_take().  Kernels receive its address
+// Device-side error word: a kernel whose bounded wait expires, or that finds a
+// length, slot or page outside its buffers, ORs a code into it and returns (or
+// skips the access) instead of hanging, trapping or reading out of bounds; the
+// host reads and clears it with device_error_take().  Kernels receive its address
 // (device_error_ptr(), one word per device) as a parameter.
-enum DeviceError : unsigned { kDevErrTimeout = 1u };
 __device__ __forceinline__ void raise_device_error(unsigned* err, unsigned code) { atomicOr(err, code); }
 unsigned* device_error_ptr();
 int device_error_take(unsigned* code);

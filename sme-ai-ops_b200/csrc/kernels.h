@@ -14,6 +14,10 @@ int q8k_quantize(const float* x, int64_t ld_x, int64_t n_rows, int64_t k, void* 
 int rms_q8k_quantize(const float* x, int64_t ld_x, int64_t n_rows, int64_t k, float eps, void* y,
                      cudaStream_t stream, const float* norm_w = nullptr);
 
+// h = x + resid (one rounding), then rms_q8k_quantize of h; h may be x or resid.
+int add_rms_q8k_quantize(const float* x, int64_t ld_x, const float* resid, int64_t ld_r, int64_t n_rows, int64_t k,
+                         float eps, const float* norm_w, float* h, int64_t ld_h, void* y, cudaStream_t stream);
+
 // ---- Q2_K weight quantizer / decoder (q2k_quant.cu) ----
 int q2k_quantize(const float* x, int64_t k_total, void* y, cudaStream_t stream);
 int q2k_dequantize(const void* w, int64_t k_total, float* y, cudaStream_t stream);

@@ -1,0 +1,567 @@
+// paged_attn.cu -- attention of new tokens over a paged key/value cache for
+// requests that bring few rows (a decoding step, drafted tokens, short
+// chunks), and the joining of partial results.
+//
+//   o_r = sum_j p_rj v_j / sum_j p_rj,   p_rj = 2^(c s_rj - m_r),
+//   s_rj = q_r . k_j,  c = scale log2(e),  m_r = max over the keys seen so far of c s_rj
+//
+// in one pass over the keys: when m_r grows by d, the sum and the context
+// gathered so far are multiplied by 2^-d.
+#include "paged_attn.cuh"
+
+namespace smeai {
+
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kKeys = 64;            // keys a block
+constexpr float kNegInf = -INFINITY;
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Shared-memory layout: [stages][K, V][kKeys rows][DP] 16-bit, the 16-byte
+// chunks of a row XORed with the row's index mod 8, so that ldmatrix's eight
+// rows fall on different banks; then the merge buffer.
+template <int DP>
+struct Shape {
+  static constexpr int kRowBytes = DP * 2;
+  static constexpr int kTileBytes = kKeys * kRowBytes;
+  static constexpr int kStages = DP == 64 ? 6 : 3;      // 96 KB in flight (192 KB at DP 256)
+  static constexpr int kPerSm = DP == 256 ? 1 : 2;      // CTAs an SM
+};
+template <int DP, bool kRowSplit>
+constexpr size_t smem_bytes() {
+  using S = Shape<DP>;
+  return (size_t)S::kStages * 2 * S::kTileBytes + (kRowSplit ? 64 * DP * 2 : 16 * DP * 4);
+}
+
+template <int DP>
+__device__ __forceinline__ uint32_t chunk_addr(uint32_t base, int row, int chunk) {
+  return base + row * Shape<DP>::kRowBytes + ((chunk ^ (row & 7)) << 4);
+}
+
+// kRowSplit false: tiles of 16 rows (a decode step's query heads of one key
+//   head).  All rows meet every key, and each warp takes 16 of a block's 64
+//   keys, with its own ring of keys in shared memory: warps never wait for one
+//   another before the tile's end, where their maxima, sums and contexts are
+//   merged.  Per 16 keys and 128 elements a warp issues 32 mma for 8 KB of
+//   cache; HBM's share of an SM (44 GB/s) leaves five times the issue slots
+//   that this takes, so the kernel is bound by the cache's bytes.
+// kRowSplit true: tiles of 64 rows, 16 a warp, every warp through all keys.
+//
+// Two CTAs an SM with 96 KB of keys and values in flight each cover HBM's
+// latency (44 GB/s x ~1 us = 44 KB an SM) through the ends of tiles.
+// Each lane looks up the page of one key a block ahead and hands the address
+// to the lanes that copy the row, so the table's latency hides behind a block.
+template <typename T, int DP, bool kRowSplit>
+__global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_kernel(const AttnParams p) {
+  using S = Shape<DP>;
+  constexpr int TR = kRowSplit ? 64 : 16;
+  constexpr int NK = kRowSplit ? 64 : 16;        // keys a warp computes with per block
+  constexpr int kChunks = DP / 8;                // 16-byte chunks a row
+  constexpr bool kQRegs = DP <= 128;             // query fragments live in registers
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ AttnShare share;
+  __shared__ float merge_m[kWarps][16], merge_l[kWarps][16];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t ring = smem_addr(smem);
+  float* merge = reinterpret_cast<float*>(smem + (size_t)S::kStages * 2 * S::kTileBytes);
+  const uint32_t q_smem = smem_addr(merge);      // row-split, DP 256: the query tile instead
+
+  pdl_wait();
+  attn_share<TR, kKeys, kThreads>(p, &share);
+  const int64_t u0 = share.u0, u1 = share.u1;
+  if (threadIdx.x == 0) p.head[blockIdx.x] = make_int4(-1, 0, 0, kPartNone);
+  if (u1 <= u0) return;
+
+  // ---- loading: `ld` walks ahead of the computation
+  AttnPos ld;
+  attn_open<TR, kKeys>(p, share, ld);
+  AttnPos w = ld;
+  int64_t to_load = u1 - u0;
+  const int page_mask = (1 << p.kv.page_log2) - 1;
+  int page = -1;                                  // page of this lane's key in block `ld`
+  auto look_up = [&]() {
+    const int key = ld.kb * kKeys + warp * 16 + (lane & 15);
+    page = key < ld.r.kv ? p.table[(int64_t)ld.b * p.ld_table + (key >> p.kv.page_log2)] : -1;
+    if (key < ld.r.kv && (page < 0 || page >= p.kv.n_pages)) {
+      raise_device_error(p.err, kDevErrBadIndex);
+      page = -1;
+    }
+  };
+  auto load_block = [&](int stage) {
+    if (to_load > 0) {
+      const int key = ld.kb * kKeys + warp * 16 + (lane & 15);
+      // byte offset of this lane's key row, or -1: nothing there, zeros instead
+      const int64_t off = page < 0 ? -1
+                                   : page * p.kv.page_bytes + (key & page_mask) * p.kv.token_bytes +
+                                         ld.h * p.kv.head_bytes;
+      const uint32_t kt = ring + (stage * 2) * S::kTileBytes, vt = kt + S::kTileBytes;
+      constexpr int kPer = 16 * kChunks / 32;     // chunks a lane copies of K, and of V
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int c = i * 32 + lane, row = c / kChunks, col = c % kChunks;
+        const int64_t o = __shfl_sync(0xffffffffu, off, row);
+        const int n = o >= 0 && col * 8 < p.kv.dim ? 16 : 0;
+        const int64_t at = n ? o + col * 16 : 0;
+        const int r = warp * 16 + row;
+        cp_async16(chunk_addr<DP>(kt, r, col), p.kv.k + at, n);
+        cp_async16(chunk_addr<DP>(vt, r, col), p.kv.v + at, n);
+      }
+      if (--to_load > 0) {
+        if (++ld.kb == ld.nkb) attn_next_tile<TR, kKeys>(p, ld);
+        look_up();
+      }
+    }
+    cp_async_commit();
+  };
+  look_up();
+  for (int s = 0; s < S::kStages - 1; ++s) load_block(s);
+
+  // ---- computing
+  const int g = lane >> 2, t4 = lane & 3;
+  uint32_t qf[kQRegs ? DP / 16 : 1][4];
+  float o[DP / 8][4];
+  float m[2], l[2];
+  int lim[2], lim_all = 0;
+  int tile_kb0 = w.kb;
+  // rows of this lane: packed rows row0 and row0 + 8
+  auto open_tile = [&]() {
+    tile_kb0 = w.kb;
+    const int row0 = w.rt * TR + (kRowSplit ? warp * 16 : 0) + g;
+    lim_all = min(w.r.kv, attn_limit(p, w.r, w.rt * TR));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = row0 + 8 * i;
+      const bool live = row < w.r.rows;
+      lim[i] = live ? min(w.r.kv, attn_limit(p, w.r, row)) : 0;
+      m[i] = kNegInf;
+      l[i] = 0.f;
+    }
+#pragma unroll
+    for (int d = 0; d < DP / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
+    auto q_row = [&](int row) -> const char* {
+      const int tok = row / p.group, hd = w.h * p.group + row % p.group;
+      return p.q + (int64_t)(w.r.q0 + tok) * p.ld_q + (int64_t)hd * p.kv.dim * 2;
+    };
+    if (kQRegs) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = row0 + 8 * i;
+        const bool live = row < w.r.rows;
+        const char* src = q_row(live ? row : 0);
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) {
+          const int d = ks * 16 + 2 * t4;
+          qf[kQRegs ? ks : 0][i] = live && d < p.kv.dim ? *reinterpret_cast<const uint32_t*>(src + d * 2) : 0u;
+          qf[kQRegs ? ks : 0][i + 2] =
+              live && d + 8 < p.kv.dim ? *reinterpret_cast<const uint32_t*>(src + d * 2 + 16) : 0u;
+        }
+      }
+    } else {
+      // the query tile in shared memory, in the layout of the keys
+      __syncthreads();
+      for (int c = threadIdx.x; c < TR * kChunks; c += kThreads) {
+        const int r = c / kChunks, col = c % kChunks, row = w.rt * TR + r;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (row < w.r.rows && col * 8 < p.kv.dim) v = *reinterpret_cast<const uint4*>(q_row(row) + col * 16);
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(merge) + (chunk_addr<DP>(0, r, col))) = v;
+      }
+      __syncthreads();
+    }
+  };
+  open_tile();
+
+  for (int64_t u = u0; u < u1; ++u) {
+    const int stage = (int)((u - u0) % S::kStages);
+    cp_async_wait<S::kStages - 2>();
+    if (kRowSplit) __syncthreads();
+    else __syncwarp();
+    load_block((int)((u - u0 + S::kStages - 1) % S::kStages));
+
+    const uint32_t kt = ring + (stage * 2) * S::kTileBytes, vt = kt + S::kTileBytes;
+    const int krow0 = kRowSplit ? 0 : warp * 16;    // first of this warp's keys in the block
+    float s[NK / 8][4];
+#pragma unroll
+    for (int n = 0; n < NK / 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) {
+      uint32_t a[4];
+      if (kQRegs) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = qf[kQRegs ? ks : 0][i];
+      } else {
+        const int r = (kRowSplit ? warp * 16 : 0) + (lane & 7) + ((lane >> 3) & 1) * 8;
+        ldsm4(chunk_addr<DP>(q_smem, r, ks * 2 + (lane >> 4)), a);
+      }
+#pragma unroll
+      for (int n2 = 0; n2 < NK / 16; ++n2) {
+        uint32_t b[4];
+        const int r = krow0 + n2 * 16 + (lane & 7) + ((lane >> 4) & 1) * 8;
+        ldsm4(chunk_addr<DP>(kt, r, ks * 2 + ((lane >> 3) & 1)), b);
+        mma16816<T>(s[2 * n2], a, b[0], b[1]);
+        mma16816<T>(s[2 * n2 + 1], a, b[2], b[3]);
+      }
+    }
+    const int key0 = w.kb * kKeys + krow0;
+    const bool masked = key0 + NK > lim_all;
+    float mx[2] = {kNegInf, kNegInf};
+#pragma unroll
+    for (int n = 0; n < NK / 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (masked && key0 + n * 8 + 2 * t4 + (i & 1) >= lim[i >> 1]) s[n][i] = kNegInf;
+        mx[i >> 1] = fmaxf(mx[i >> 1], s[n][i]);
+      }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+      mx[i] = fmaxf(m[i], mx[i] * p.scale_log2);
+    }
+    if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float f = mx[i] > m[i] ? exp2_fast(m[i] - mx[i]) : 1.f;   // m = -inf: 0
+        m[i] = mx[i];
+        l[i] *= f;
+#pragma unroll
+        for (int d = 0; d < DP / 8; ++d) {
+          o[d][2 * i] *= f;
+          o[d][2 * i + 1] *= f;
+        }
+      }
+    }
+    const float sub[2] = {m[0] == kNegInf ? 0.f : Num<T>::kBias - m[0], m[1] == kNegInf ? 0.f : Num<T>::kBias - m[1]};
+#pragma unroll
+    for (int n = 0; n < NK / 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[n][i] = exp2_fast(fmaf(s[n][i], p.scale_log2, sub[i >> 1]));
+        l[i >> 1] += s[n][i];
+      }
+#pragma unroll
+    for (int k2 = 0; k2 < NK / 16; ++k2) {
+      const uint32_t a[4] = {Num<T>::pack(s[2 * k2][0], s[2 * k2][1]), Num<T>::pack(s[2 * k2][2], s[2 * k2][3]),
+                             Num<T>::pack(s[2 * k2 + 1][0], s[2 * k2 + 1][1]),
+                             Num<T>::pack(s[2 * k2 + 1][2], s[2 * k2 + 1][3])};
+#pragma unroll
+      for (int d2 = 0; d2 < DP / 16; ++d2) {
+        uint32_t b[4];
+        const int r = krow0 + k2 * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
+        ldsm4_t(chunk_addr<DP>(vt, r, d2 * 2 + (lane >> 4)), b);
+        mma16816<T>(o[2 * d2], a, b[0], b[1]);
+        mma16816<T>(o[2 * d2 + 1], a, b[2], b[3]);
+      }
+    }
+
+    // ---- end of the tile, or of this CTA's share of it
+    const bool last = w.kb + 1 == w.nkb;
+    if (last || u + 1 == u1) {
+      const bool whole = last && tile_kb0 == 0;
+      // slot 0: a tile entered in the middle; slot 1: a tile left unfinished
+      const int64_t slot = 2 * (int64_t)blockIdx.x + (tile_kb0 == 0 ? 1 : 0);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+      }
+      auto out_row = [&](int row) -> char* {
+        const int tok = row / p.group, hd = w.h * p.group + row % p.group;
+        return p.out + (int64_t)(w.r.q0 + tok) * p.ld_out + (int64_t)hd * p.kv.dim * 2;
+      };
+      if (kRowSplit) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int r = warp * 16 + g + 8 * i, row = w.rt * TR + r;
+          if (row >= w.r.rows) continue;
+          if (whole) {
+            const float inv = l[i] > 0.f ? 1.f / l[i] : (l[i] == 0.f ? 0.f : l[i]);
+            char* dst = out_row(row);
+#pragma unroll
+            for (int d = 0; d < DP / 8; ++d)
+              if (d * 8 < p.kv.dim)
+                *reinterpret_cast<uint32_t*>(dst + (d * 8 + 2 * t4) * 2) =
+                    Num<T>::pack(o[d][2 * i] * inv, o[d][2 * i + 1] * inv);
+          } else {
+            float* dst = p.part_o + (slot * TR + r) * DP;
+#pragma unroll
+            for (int d = 0; d < DP / 8; ++d)
+              *reinterpret_cast<float2*>(dst + d * 8 + 2 * t4) = make_float2(o[d][2 * i], o[d][2 * i + 1]);
+            if (t4 == 0) p.part_ml[slot * TR + r] = make_float2(m[i], l[i]);
+          }
+        }
+      } else {
+        // merge the warps: their common maximum, then the contexts added up
+        // in warp order
+        if (t4 == 0) {
+          merge_m[warp][g] = m[0];
+          merge_m[warp][g + 8] = m[1];
+        }
+        __syncthreads();
+        float top[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          top[i] = merge_m[0][g + 8 * i];
+#pragma unroll
+          for (int ww = 1; ww < kWarps; ++ww) top[i] = fmaxf(top[i], merge_m[ww][g + 8 * i]);
+          const float f = m[i] == kNegInf ? 0.f : exp2_fast(m[i] - top[i]);
+          l[i] = l[i] * f;
+#pragma unroll
+          for (int d = 0; d < DP / 8; ++d) {
+            o[d][2 * i] *= f;
+            o[d][2 * i + 1] *= f;
+          }
+        }
+        if (t4 == 0) {
+          merge_l[warp][g] = l[0];
+          merge_l[warp][g + 8] = l[1];
+        }
+        for (int ww = 0; ww < kWarps; ++ww) {
+          if (warp == ww) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int d = 0; d < DP / 8; ++d) {
+                // columns XORed with the row, so that the eight rows of a store take different banks
+                float2* dst = reinterpret_cast<float2*>(merge + (g + 8 * i) * DP + ((d * 8 + 2 * t4) ^ (g * 8)));
+                float2 v = make_float2(o[d][2 * i], o[d][2 * i + 1]);
+                if (ww) {
+                  const float2 old = *dst;
+                  v.x = old.x + v.x;
+                  v.y = old.y + v.y;
+                }
+                *dst = v;
+              }
+          }
+          __syncthreads();
+        }
+        for (int c = threadIdx.x; c < 16 * (DP / 8); c += kThreads) {
+          const int r = c / (DP / 8), d8 = c % (DP / 8), row = w.rt * TR + r;
+          if (row >= w.r.rows) continue;
+          const float4* src = reinterpret_cast<const float4*>(merge + r * DP + ((d8 * 8) ^ ((r & 7) * 8)));
+          const float4 a = src[0], b = src[1];
+          const float sum = merge_l[0][r] + merge_l[1][r] + merge_l[2][r] + merge_l[3][r];
+          if (whole) {
+            const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+            if (d8 * 8 < p.kv.dim)
+              *reinterpret_cast<uint4*>(out_row(row) + d8 * 16) =
+                  make_uint4(Num<T>::pack(a.x * inv, a.y * inv), Num<T>::pack(a.z * inv, a.w * inv),
+                             Num<T>::pack(b.x * inv, b.y * inv), Num<T>::pack(b.z * inv, b.w * inv));
+          } else {
+            float4* dst = reinterpret_cast<float4*>(p.part_o + (slot * TR + r) * DP + d8 * 8);
+            dst[0] = a;
+            dst[1] = b;
+            if (d8 == 0) {
+              const float top_m = fmaxf(fmaxf(merge_m[0][r], merge_m[1][r]), fmaxf(merge_m[2][r], merge_m[3][r]));
+              p.part_ml[slot * TR + r] = make_float2(top_m, sum);
+            }
+          }
+        }
+        __syncthreads();
+      }
+      if (!whole && threadIdx.x == 0) {
+        int4* hd = &p.head[blockIdx.x];
+        if (tile_kb0 == 0) {
+          hd->x = w.b;
+          hd->y = w.rt;
+          hd->z = w.h;
+        } else {
+          hd->w = last ? kPartEnds : kPartGoesOn;
+        }
+      }
+      if (u + 1 < u1) {
+        attn_next_tile<TR, kKeys>(p, w);
+        open_tile();
+      }
+    } else {
+      ++w.kb;
+    }
+  }
+  cp_async_wait<0>();
+  pdl_trigger();
+}
+
+// Joins the pieces of each tile that some CTA left unfinished: the CTA's slot
+// 1, then slot 0 of the CTAs after it up to the one where the tile ends.  One
+// CTA a (tile, row slice); a warp takes every eighth piece of a row, all lanes
+// the row's columns, and the warps' sums meet in shared memory in warp order.
+template <typename T, int TR, int DP>
+__global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnParams p, int ctas) {
+  constexpr int kCols = DP >= 128 ? 4 : 2;            // consecutive columns a lane
+  constexpr int kSpans = DP / (32 * kCols);           // 1, or 2 at DP 256
+  __shared__ float acc[8][DP];
+  __shared__ float wsum[8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x;
+  pdl_wait();
+  const int4 hd = p.head[c];
+  if (hd.x < 0) return;
+  // pieces: the first CTA after c whose slot 0 ends the tile
+  int n = 0;
+  for (int i = c + 1; n == 0 && i < ctas; i += 32) {
+    const int st = i + lane < ctas ? p.head[i + lane].w : kPartEnds;   // the last CTA ends the line
+    const unsigned ends = __ballot_sync(0xffffffffu, st == kPartEnds);
+    if (ends) n = i + __ffs(ends) - c;
+  }
+  if (n == 0) return;
+  if (c + n > ctas) n = ctas - c;
+  auto slot = [&](int i) -> int64_t { return i == 0 ? 2 * (int64_t)c + 1 : 2 * (int64_t)(c + i); };
+  const AttnReq r = attn_req(p, hd.x);
+  for (int row_t = blockIdx.y; row_t < TR; row_t += gridDim.y) {
+    const int row = hd.y * TR + row_t;
+    if (row >= r.rows) return;
+    float top = kNegInf;
+    for (int i = lane; i < n; i += 32) top = fmaxf(top, p.part_ml[slot(i) * TR + row_t].x);
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    float a[kSpans * kCols] = {}, sum = 0.f;
+#pragma unroll 4
+    for (int i = warp; i < n; i += 8) {
+      const float2 ml = p.part_ml[slot(i) * TR + row_t];
+      const float f = ml.x == kNegInf ? 0.f : exp2_fast(ml.x - top);
+      sum = fmaf(ml.y, f, sum);
+      const float* src = p.part_o + (slot(i) * TR + row_t) * DP + lane * kCols;
+#pragma unroll
+      for (int s = 0; s < kSpans; ++s) {
+        float v[4];
+        if (kCols == 4) {
+          const float4 x = *reinterpret_cast<const float4*>(src + s * 128);
+          v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+        } else {
+          const float2 x = *reinterpret_cast<const float2*>(src);
+          v[0] = x.x; v[1] = x.y;
+        }
+#pragma unroll
+        for (int k = 0; k < kCols; ++k) a[s * kCols + k] = fmaf(v[k], f, a[s * kCols + k]);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < kSpans; ++s)
+#pragma unroll
+      for (int k = 0; k < kCols; ++k) acc[warp][s * 128 + lane * kCols + k] = a[s * kCols + k];
+    if (lane == 0) wsum[warp] = sum;
+    __syncthreads();
+    float total = 0.f;
+#pragma unroll
+    for (int ww = 0; ww < 8; ++ww) total += wsum[ww];
+    const float inv = total > 0.f ? 1.f / total : (total == 0.f ? 0.f : total);
+    const int tok = row / p.group, head = hd.z * p.group + row % p.group;
+    uint16_t* dst = reinterpret_cast<uint16_t*>(p.out + (int64_t)(r.q0 + tok) * p.ld_out) + (int64_t)head * p.kv.dim;
+    for (int d = threadIdx.x; d < p.kv.dim; d += 256) {
+      float v = 0.f;
+#pragma unroll
+      for (int ww = 0; ww < 8; ++ww) v += acc[ww][d];
+      dst[d] = Num<T>::one(v * inv);
+    }
+    __syncthreads();
+  }
+}
+
+template <typename T, int DP, bool kRowSplit>
+int run_class(AttnParams p, const PagedAttention& a, int sms, cudaStream_t stream) {
+  constexpr int TR = kRowSplit ? 64 : 16;
+  const int ctas = sms * Shape<DP>::kPerSm;
+  attn_carve<TR, DP>(p, a.workspace, ctas);
+  constexpr size_t smem = smem_bytes<DP, kRowSplit>();
+  auto kernel = paged_attn_kernel<T, DP, kRowSplit>;
+  SMEAI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  SMEAI_CUDA_TRY(launch(kernel, dim3((unsigned)ctas), dim3(kThreads), smem, stream, p));
+  // a tile of up to 2 * kSnap blocks is never split
+  if (a.max_kv > 2 * kSnap * kKeys) SMEAI_CUDA_TRY((attn_join<T, TR, DP>(p, ctas, stream)));
+  return kOk;
+}
+
+template <typename T, int DP>
+int run_dim(const AttnParams& p, const PagedAttention& a, int sms, cudaStream_t stream) {
+  const int64_t most = a.max_new * p.group;      // packed rows of the largest request
+  if (most <= 16) return run_class<T, DP, false>(p, a, sms, stream);
+  return run_class<T, DP, true>(p, a, sms, stream);
+}
+
+int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+
+}  // namespace
+
+template <typename T, int TR, int DP>
+cudaError_t attn_join(const AttnParams& p, int ctas, cudaStream_t stream) {
+  return launch(paged_attn_join_kernel<T, TR, DP>, dim3((unsigned)ctas, 4u), dim3(256), 0, stream, p, ctas);
+}
+
+size_t paged_attention_workspace(const PagedAttention& a) {
+  int sms = 0;
+  if (sm_count(&sms)) return 0;
+  const bool few = a.max_new * (a.n_heads / a.kv.n_kv) <= 16;
+  switch (padded_dim(a.kv.dim)) {
+    case 64: return few ? attn_part_bytes<16, 64>(2 * sms) : attn_part_bytes<64, 64>(2 * sms);
+    case 128: return few ? attn_part_bytes<16, 128>(2 * sms) : attn_part_bytes<64, 128>(2 * sms);
+    default: return few ? attn_part_bytes<16, 256>(sms) : attn_part_bytes<64, 256>(sms);
+  }
+}
+
+int paged_attention(const PagedAttention& a, cudaStream_t stream) {
+  AttnParams p;
+  p.kv = a.kv;
+  p.q = static_cast<const char*>(a.q);
+  p.out = static_cast<char*>(a.out);
+  p.ld_q = a.ld_q * 2;
+  p.ld_out = a.ld_out * 2;
+  p.q_start = a.q_start;
+  p.kv_len = a.kv_len;
+  p.table = a.table;
+  p.ld_table = a.ld_table;
+  p.n_req = a.n_req;
+  p.max_kv = a.max_kv;
+  p.n_tokens = (int)a.n_tokens;
+  p.group = a.n_heads / a.kv.n_kv;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.causal = a.causal ? 1 : 0;
+  p.rows_lo = 0;
+  p.rows_hi = 0x7fffffff;
+  p.err = device_error_ptr();
+  int sms = 0;
+  const int st = sm_count(&sms);
+  if (st) return st;
+  if (!p.err) {
+    set_last_error("paged_attention: no device error word");
+    return kCudaError;
+  }
+  const int dp = padded_dim(a.kv.dim);
+  if (a.kv.bf16)
+    return dp == 64    ? run_dim<__nv_bfloat16, 64>(p, a, sms, stream)
+           : dp == 128 ? run_dim<__nv_bfloat16, 128>(p, a, sms, stream)
+                       : run_dim<__nv_bfloat16, 256>(p, a, sms, stream);
+  return dp == 64    ? run_dim<__half, 64>(p, a, sms, stream)
+         : dp == 128 ? run_dim<__half, 128>(p, a, sms, stream)
+                     : run_dim<__half, 256>(p, a, sms, stream);
+}
+
+}  // namespace smeai

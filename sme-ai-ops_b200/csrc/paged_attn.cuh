@@ -1,0 +1,256 @@
+// paged_attn.cuh -- what the paged attention kernels share: parameters, the
+// split of a step's work over CTAs, and the partial results of rows whose keys
+// several CTAs share.
+//
+// Work.  The rows of a request that read one key head are its new tokens times
+// the query heads of that key head's group, packed as (token, head in group)
+// and cut into tiles of TR rows.  A tile is (request, row tile, key head); its
+// keys come in blocks of KB.  All key blocks of all tiles of a launch, in a
+// fixed order, are one line of units, and every CTA takes an equal piece of
+// that line -- whatever the requests' lengths, no CTA has more than its share.
+// A piece that ends inside a tile leaves that tile's rows as a partial result
+// (running maximum, sum, unnormalized context; all fp32), which a second
+// kernel joins in key order, so results do not depend on timing.  Pieces are
+// snapped to a tile's edge when one is within kSnap units: short tiles are
+// never split and need no joining.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+#include "paged.h"
+
+namespace smeai {
+
+constexpr int kSnap = 3;
+
+struct AttnParams {
+  KvView kv;
+  const char* q;
+  char* out;
+  int64_t ld_q, ld_out;   // bytes
+  const int32_t *q_start, *kv_len, *table;
+  int64_t ld_table;
+  int n_req, max_kv, n_tokens;
+  int group;              // query heads per key head
+  float scale_log2;       // scale * log2(e)
+  int causal;
+  int rows_lo, rows_hi;   // requests with rows_lo < rows <= rows_hi are this launch's
+  float* part_o;          // [2 * CTAs][TR][DP]
+  float2* part_ml;        // [2 * CTAs][TR] running maximum (log2 units), sum
+  int4* head;             // [CTAs] {tile left unfinished at the end: request or -1, row tile, key head; state of slot 0}
+  unsigned* err;
+};
+
+// State of a CTA's partial slot 0, the tile it entered in the middle.
+enum : int { kPartNone = 0, kPartGoesOn = 1, kPartEnds = 2 };
+
+struct AttnReq {
+  int q0, n_new, kv, rows;   // first row, new tokens, keys, packed rows (0: not this launch's)
+};
+
+__device__ __forceinline__ AttnReq attn_req(const AttnParams& p, int b) {
+  AttnReq r;
+  const int a = p.q_start[b], e = p.q_start[b + 1], kv = p.kv_len[b];
+  r.q0 = min(max(a, 0), p.n_tokens);
+  r.n_new = min(max(e, r.q0), p.n_tokens) - r.q0;
+  r.kv = min(max(kv, 0), p.max_kv);
+  if (a != r.q0 || e != r.q0 + r.n_new || kv != r.kv) raise_device_error(p.err, kDevErrBadIndex);
+  r.rows = r.n_new * p.group;
+  if (r.rows <= p.rows_lo || r.rows > p.rows_hi) r.rows = 0;
+  return r;
+}
+
+// Keys that packed row `row` sees: j < the result.
+__device__ __forceinline__ int attn_limit(const AttnParams& p, const AttnReq& r, int row) {
+  return p.causal ? max(0, r.kv - r.n_new + 1 + row / p.group) : r.kv;
+}
+
+// Key blocks of row tile rt (at least one: a tile whose rows see nothing still
+// has its zeros to write).
+template <int TR, int KB>
+__device__ __forceinline__ int attn_blocks(const AttnParams& p, const AttnReq& r, int rt) {
+  const int last = min((rt + 1) * TR, r.rows) - 1;
+  return max(1, (min(r.kv, attn_limit(p, r, last)) + KB - 1) / KB);
+}
+
+template <int TR, int KB>
+__device__ __forceinline__ int64_t attn_units(const AttnParams& p, const AttnReq& r) {
+  int64_t u = 0;
+  const int n_rt = (r.rows + TR - 1) / TR;
+  for (int rt = 0; rt < n_rt; ++rt) u += attn_blocks<TR, KB>(p, r, rt);
+  return u * p.kv.n_kv;
+}
+
+// A place on the line: tile (b, rt, h), key block kb of its nkb.
+struct AttnPos {
+  int b, rt, h, kb, nkb;
+  AttnReq r;
+};
+
+template <int TR, int KB>
+__device__ __forceinline__ void attn_next_tile(const AttnParams& p, AttnPos& w) {
+  w.kb = 0;
+  if (++w.h < p.kv.n_kv) return;
+  w.h = 0;
+  ++w.rt;
+  if (w.rt * TR >= w.r.rows) {
+    w.rt = 0;
+    do {
+      if (++w.b >= p.n_req) return;
+      w.r = attn_req(p, w.b);
+    } while (w.r.rows == 0);
+  }
+  w.nkb = attn_blocks<TR, KB>(p, w.r, w.rt);
+}
+
+struct AttnShare {
+  int64_t u0, u1;            // this CTA's units
+  int b, rt, h, kb;          // place of u0
+};
+
+// This CTA's piece of the line.  All threads of the block call it; the place
+// is in shared memory on return.  Each thread sums the units of its own run of
+// requests; the one whose run holds an end of the piece walks to it.
+template <int TR, int KB, int NT>
+__device__ void attn_share(const AttnParams& p, AttnShare* s) {
+  __shared__ int64_t warp_sum[NT / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int per = (p.n_req + NT - 1) / NT;
+  const int b0 = min((int)threadIdx.x * per, p.n_req), b1 = min(b0 + per, p.n_req);
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) mine += attn_units<TR, KB>(p, attn_req(p, b));
+  int64_t incl = mine;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int64_t t = __shfl_up_sync(0xffffffffu, incl, off);
+    if (lane >= off) incl += t;
+  }
+  if (lane == 31) warp_sum[warp] = incl;
+  __syncthreads();
+  int64_t before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < NT / 32; ++w) {
+    if (w < warp) before += warp_sum[w];
+    total += warp_sum[w];
+  }
+  const int64_t lo = before + incl - mine;   // units ahead of this thread's run
+  const int64_t per_cta = (total + gridDim.x - 1) / gridDim.x;
+  const int64_t cut0 = min(total, per_cta * blockIdx.x), cut1 = min(total, cut0 + per_cta);
+  if (threadIdx.x == 0) {
+    if (cut0 >= total) s->u0 = total;
+    if (cut1 >= total) s->u1 = total;
+  }
+  // walk to each cut that lies in this run: the tile around it, and the edge it snaps to
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    const int64_t cut = which ? cut1 : cut0;
+    if (cut < lo || cut >= lo + mine) continue;
+    int64_t at = lo;
+    for (int b = b0; b < b1; ++b) {
+      const AttnReq r = attn_req(p, b);
+      const int n_rt = (r.rows + TR - 1) / TR;
+      for (int rt = 0; rt < n_rt; ++rt) {
+        const int nkb = attn_blocks<TR, KB>(p, r, rt);
+        if (cut >= at + (int64_t)nkb * p.kv.n_kv) {
+          at += (int64_t)nkb * p.kv.n_kv;
+          continue;
+        }
+        int h = (int)((cut - at) / nkb), kb = (int)((cut - at) % nkb);
+        int64_t u = cut;
+        if (kb <= kSnap && kb <= nkb - kb) {
+          u -= kb;
+          kb = 0;
+        } else if (nkb - kb <= kSnap) {
+          u += nkb - kb;
+          kb = nkb;        // the start of the next tile
+        }
+        if (which) s->u1 = u;
+        else {
+          s->u0 = u;
+          s->b = b;
+          s->rt = rt;
+          s->h = h;
+          s->kb = kb;
+        }
+        b = b1;
+        break;
+      }
+    }
+  }
+  __syncthreads();
+}
+
+template <int TR, int KB>
+__device__ __forceinline__ void attn_open(const AttnParams& p, const AttnShare& s, AttnPos& w) {
+  w.b = s.b;
+  w.rt = s.rt;
+  w.h = s.h;
+  w.r = attn_req(p, s.b);
+  w.nkb = attn_blocks<TR, KB>(p, w.r, s.rt);
+  w.kb = s.kb;
+  if (s.kb == w.nkb) attn_next_tile<TR, KB>(p, w);
+}
+
+// ---- 16-bit types ---------------------------------------------------------------
+// kBias: softmax weights are kept as 2^(kBias + s - m).  Half has 14 exponent
+// steps below 1; the bias moves the weights up so that ones as small as
+// 2^-24 of the largest keep their 11 bits, and 2^(kBias) and its 2^-8 lazily
+// updated maximum stay below 65504.  bfloat16 has fp32's range and needs none.
+template <typename T>
+struct Num;
+template <>
+struct Num<__half> {
+  static constexpr float kBias = 7.f;
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ uint16_t one(float v) { return __half_as_ushort(__float2half_rn(v)); }
+};
+template <>
+struct Num<__nv_bfloat16> {
+  static constexpr float kBias = 0.f;
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ uint16_t one(float v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
+};
+
+// 2^x, the hardware's approximation (2 ulp; 2^-inf = 0).
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Partial slots and headers of a launch with `ctas` CTAs.
+template <int TR, int DP>
+constexpr size_t attn_part_bytes(int ctas) {
+  return (size_t)2 * ctas * TR * (DP * sizeof(float) + sizeof(float2)) + (size_t)ctas * sizeof(int4);
+}
+template <int TR, int DP>
+void attn_carve(AttnParams& p, void* ws, int ctas) {
+  char* c = static_cast<char*>(ws);
+  p.part_o = reinterpret_cast<float*>(c);
+  c += (size_t)2 * ctas * TR * DP * sizeof(float);
+  p.part_ml = reinterpret_cast<float2*>(c);
+  c += (size_t)2 * ctas * TR * sizeof(float2);
+  p.head = reinterpret_cast<int4*>(c);
+}
+
+// Joins the partial results (paged_attn.cu).
+template <typename T, int TR, int DP>
+cudaError_t attn_join(const AttnParams& p, int ctas, cudaStream_t stream);
+
+}  // namespace smeai

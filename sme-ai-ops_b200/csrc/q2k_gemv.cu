@@ -68,7 +68,7 @@ __device__ bool peer_wait(const unsigned* sig, const unsigned* epoch, unsigned c
   const unsigned target = (ld_acquire_sys(epoch) + 1u) * count;
   const uint64_t t0 = now_ns();
   while ((int)(ld_acquire_sys(sig) - target) < 0) {
-    if (*reinterpret_cast<const volatile unsigned*>(err)) return false;
+    if (*reinterpret_cast<const volatile unsigned*>(err) & kDevErrTimeout) return false;
     if (now_ns() - t0 > timeout_ns) return false;
     __nanosleep(64);
   }

@@ -162,6 +162,16 @@ __device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
   }
 }
 
+__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
+  if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = v[i];
+  }
+}
+
 // load8 through L2 only (ld.global.cg): for data other CTAs of the running
 // grid wrote, which this SM's L1 may hold stale.
 __device__ __forceinline__ void load8_cg(const float* p, float (&v)[8]) {

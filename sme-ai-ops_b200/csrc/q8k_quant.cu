@@ -62,6 +62,77 @@ __global__ void rms_q8k_quantize_kernel(const float* __restrict__ x, int64_t ld_
   }
 }
 
+// Residual addition + RMSNorm + quantization, one CTA per row: h = x + resid
+// is formed once and kept in registers (kKeep 256-value blocks a warp) between
+// the two passes that the norm needs, so a row costs one read of x and of
+// resid, one write of h and one of the blocks: 13.1 bytes a value.  Blocks
+// past kKeep a warp are read back from h by the lanes that wrote it.  No
+// __restrict__ on h: it may be x or resid.
+template <int kKeep>
+__global__ void __launch_bounds__(512) add_rms_q8k_quantize_kernel(const float* x, int64_t ld_x, const float* resid,
+                                                                   int64_t ld_r, int nb, float eps,
+                                                                   const float* __restrict__ norm_w, float* h,
+                                                                   int64_t ld_h, uint8_t* __restrict__ y) {
+  extern __shared__ float sm_gsum[];  // 8 group sums per block
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
+  const int64_t row = blockIdx.x;
+  const float *xr = x + row * ld_x, *rr = resid + row * ld_r;
+  float* hr = h + row * ld_h;
+  float v[kKeep][8], a[8];
+#pragma unroll
+  for (int i = 0; i < kKeep; ++i) {
+    const int b = warp + i * nwarps;
+    if (b < nb) load8(xr + b * QK_K + lane * 8, v[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < kKeep; ++i) {
+    const int b = warp + i * nwarps;
+    if (b < nb) {
+      load8(rr + b * QK_K + lane * 8, a);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = __fadd_rn(v[i][j], a[j]);
+      store8(hr + b * QK_K + lane * 8, v[i]);
+      const float s = group_sumsq_load8(v[i]);
+      if ((lane & 3) == 0) sm_gsum[b * 8 + (lane >> 2)] = s;
+    }
+  }
+  for (int b = warp + kKeep * nwarps; b < nb; b += nwarps) {
+    float t[8];
+    load8(xr + b * QK_K + lane * 8, t);
+    load8(rr + b * QK_K + lane * 8, a);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[j] = __fadd_rn(t[j], a[j]);
+    store8(hr + b * QK_K + lane * 8, t);
+    const float s = group_sumsq_load8(t);
+    if ((lane & 3) == 0) sm_gsum[b * 8 + (lane >> 2)] = s;
+  }
+  __syncthreads();
+  // every warp folds the group sums itself: the same order, one barrier less
+  const float inv = rms_inv_from_sum(rms_fold_groups(sm_gsum, nb * 8), nb * QK_K, eps);
+  auto finish = [&](float (&t)[8], int b) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[j] = __fmul_rn(t[j], inv);
+    if (norm_w) {
+      load8(norm_w + b * QK_K + lane * 8, a);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) t[j] = __fmul_rn(t[j], a[j]);
+    }
+    q8k_store_global(q8k_quantize_lane(t), y + (row * nb + b) * Q8K_BLOCK_BYTES);
+  };
+#pragma unroll
+  for (int i = 0; i < kKeep; ++i) {
+    const int b = warp + i * nwarps;
+    if (b < nb) finish(v[i], b);
+  }
+  for (int b = warp + kKeep * nwarps; b < nb; b += nwarps) {
+    float t[8];
+    load8(hr + b * QK_K + lane * 8, t);
+    finish(t, b);
+  }
+}
+
 int q8k_quantize(const float* x, int64_t ld_x, int64_t n_rows, int64_t k, void* y, cudaStream_t stream) {
   if (k <= 0 || k % QK_K != 0 || n_rows <= 0 || ld_x < k) {
     set_last_error("q8k_quantize: k must be a positive multiple of 256 (k=%lld rows=%lld ld=%lld)",
@@ -88,6 +159,23 @@ int rms_q8k_quantize(const float* x, int64_t ld_x, int64_t n_rows, int64_t k, fl
   const int threads = nb >= 16 ? 512 : (nb >= 8 ? 256 : 128);
   SMEAI_CUDA_TRY(launch(rms_q8k_quantize_kernel, dim3((unsigned)n_rows), dim3(threads), (size_t)(8 * nb + 1) * 4,
                         stream, x, ld_x, nb, eps, norm_w, static_cast<uint8_t*>(y)));
+  return kOk;
+}
+
+int add_rms_q8k_quantize(const float* x, int64_t ld_x, const float* resid, int64_t ld_r, int64_t n_rows, int64_t k,
+                         float eps, const float* norm_w, float* h, int64_t ld_h, void* y, cudaStream_t stream) {
+  if (k <= 0 || k % QK_K != 0 || k > 65536 || n_rows <= 0 || n_rows > 0x7fffffff || ld_x < k || ld_r < k ||
+      ld_h < k) {
+    set_last_error("add_rms_q8k_quantize: k must be a multiple of 256 from 256 to 65536, the row strides at least k "
+                   "(k=%lld rows=%lld)", (long long)k, (long long)n_rows);
+    return kBadArgument;
+  }
+  const int nb = (int)(k / QK_K);
+  const size_t smem = (size_t)8 * nb * 4;
+  uint8_t* out = static_cast<uint8_t*>(y);
+  const int warps = nb < 16 ? nb : 16;
+  SMEAI_CUDA_TRY(launch(add_rms_q8k_quantize_kernel<2>, dim3((unsigned)n_rows), dim3(32 * warps), smem, stream, x,
+                        ld_x, resid, ld_r, nb, eps, norm_w, h, ld_h, out));
   return kOk;
 }
 

@@ -1,7 +1,7 @@
 """Python view of libsmeai_b200.so (the sm_100a Q2_K / packed-Linear library).
 
-Everything here calls the C-ABI declared in include/sme_ai_ops.h and
-include/smeai_q2k.h through ctypes; torch is used only for device memory and
+Everything here calls the C-ABI declared in include/sme_ai_ops.h,
+include/smeai_q2k.h and include/smeai_paged.h through ctypes; torch is used only for device memory and
 streams.  There is no fallback: if the shared library is missing or cannot
 be loaded, ``lib()`` raises.
 """
@@ -78,10 +78,20 @@ class PeerExchange(ctypes.Structure):
                 ("wait_sig", ctypes.c_void_p), ("wait_count", ctypes.c_uint), ("epoch", ctypes.c_void_p)]
 
 
+KV_F16, KV_BF16 = 1, 30      # element types of a paged cache (ggml's numbers)
+
+
+class KVCache(ctypes.Structure):
+    """smeai_kv_cache: a paged key/value cache."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("type", ctypes.c_int), ("page_size", ctypes.c_int),
+                ("n_kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int), ("n_pages", ctypes.c_int64),
+                ("page_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64), ("token_stride", ctypes.c_int64)]
+
+
 def _declare(L: ctypes.CDLL) -> None:
     P, U64, I64, I, F, SZ = (ctypes.c_void_p, ctypes.c_uint64, ctypes.c_int64, ctypes.c_int,
                              ctypes.c_float, ctypes.c_size_t)
-    WS, PW = ctypes.POINTER(Workspace), ctypes.POINTER(PackedWeight)
+    WS, PW, KV = ctypes.POINTER(Workspace), ctypes.POINTER(PackedWeight), ctypes.POINTER(KVCache)
     sig = {
         # smeai_q2k.h
         "quantize_row_q8_K": (None, [P, P, I64]),
@@ -136,6 +146,7 @@ def _declare(L: ctypes.CDLL) -> None:
         "smeai_q8k_quantize": (I, [P, I64, I64, I64, P, P]),
         "smeai_rms_q8k_quantize": (I, [P, I64, I64, I64, F, P, P]),
         "smeai_rms_q8k_quantize_w": (I, [P, I64, I64, I64, P, F, P, P]),
+        "smeai_add_rms_q8k_quantize": (I, [P, I64, P, I64, I64, I64, P, F, P, I64, P, P]),
         "smeai_q2k_mul_mat": (I, [P, I64, I64, P, I64, P, SZ, P]),
         "smeai_q2k_mul_mat_ex": (I, [P, P, I64, P, SZ, I, P, SZ, P]),
         "smeai_q2k_mul_mat_tc": (I, [P, P, I64, P, SZ, P]),
@@ -161,6 +172,11 @@ def _declare(L: ctypes.CDLL) -> None:
         "smeai_q2k_program_free": (None, [P]),
         "smeai_q2k_quantize_device": (I, [P, I64, P, P]),
         "smeai_q2k_dequantize_device": (I, [P, I64, P, P]),
+        # smeai_paged.h
+        "smeai_paged_plan": (I, [P, P, I64, I, P, I64, P, P, P, I64, I64, P, P, P, P, I64, P]),
+        "smeai_paged_append": (I, [KV, P, I64, P, I64, P, I64, I, P, I64, I64, P, P, P, I64, I, P]),
+        "smeai_paged_attention_workspace": (SZ, [KV, I, I64, I64, I64, I64]),
+        "smeai_paged_attention": (I, [KV, P, I64, I, I64, P, P, I64, P, I64, I64, I64, F, I, P, I64, P, SZ, P]),
         # sme_ai_ops.h
         "sme_ai_has_sme": (I, []),
         "sme_ai_has_sme2": (I, []),

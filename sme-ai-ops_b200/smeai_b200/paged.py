@@ -1,0 +1,179 @@
+"""The paged key/value cache over torch device memory (thin wrappers of smeai_paged.h).
+
+A step of a serving loop, per layer where it says so:
+
+    plan.build(cached_len, new_len, free_pages, n_used)             # once a step
+    q = append(kv, k, v, plan.slots, q=q, positions=plan.positions, rope=rope)      # per layer
+    context = attention(q, kv, plan.block_table, plan.q_start, plan.kv_len, max_new)
+
+All calls queue work on the current stream and neither wait nor keep anything;
+with the outputs given, all of them can be captured in a CUDA graph.  A length,
+slot, position or page outside its buffer is reported by take_device_error().
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import KV_BF16, KV_F16, KVCache, check, lib
+from .q2k import on_device
+
+_TYPES = {torch.float16: KV_F16, torch.bfloat16: KV_BF16}
+
+
+def rope_table(n_positions: int, head_dim: int, base: float = 10000.0, device=None) -> torch.Tensor:
+    """[n_positions, head_dim] fp32: the cosines of a position's head_dim/2
+    angles, then their sines; angles formed in 64 bits."""
+    i = torch.arange(0, head_dim, 2, dtype=torch.float64, device=device)
+    angle = torch.arange(n_positions, dtype=torch.float64, device=device)[:, None] * base ** (-i / head_dim)
+    return torch.cat([angle.cos(), angle.sin()], 1).float().contiguous()
+
+
+class PagedKV:
+    """Pages of keys and values: k, v [n_pages, n_kv_heads, page_size, head_dim],
+    fp16 or bf16 (a cache stored page by token by head is passed as its
+    transposed view)."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor):
+        assert k.dim() == 4 and k.shape == v.shape and k.stride() == v.stride(), "k and v of one shape and layout"
+        assert k.is_cuda and k.device == v.device and k.dtype == v.dtype and k.dtype in _TYPES
+        assert k.stride(3) == 1 or k.shape[3] == 1, "a head's elements lie next to one another"
+        self.k, self.v = k, v
+        self.device, self.dtype = k.device, k.dtype
+        self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
+        self.struct = KVCache(k.data_ptr(), v.data_ptr(), _TYPES[k.dtype], self.page_size, self.n_kv_heads, self.head_dim,
+                              self.n_pages, k.stride(0), k.stride(1), k.stride(2))
+        self.ref = ctypes.byref(self.struct)
+
+    @classmethod
+    def empty(cls, n_pages: int, n_kv_heads: int, page_size: int, head_dim: int, dtype=torch.float16, device=None) -> "PagedKV":
+        device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
+        shape = (n_pages, n_kv_heads, page_size, head_dim)
+        return cls(torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device))
+
+
+class PagedPlan:
+    """Buffers of a step's bookkeeping over a block table [n_req, max_blocks]
+    (int32, kept by the caller from step to step): q_start [n_req + 1], kv_len
+    [n_req], slots (int64) and positions [n_tokens]."""
+
+    def __init__(self, block_table: torch.Tensor, page_size: int, n_tokens: int):
+        assert block_table.dim() == 2 and block_table.dtype == torch.int32 and block_table.is_cuda
+        assert block_table.stride(1) == 1 or block_table.shape[1] == 1
+        self.block_table, self.page_size, self.n_tokens = block_table, page_size, n_tokens
+        self.n_req, self.max_blocks = block_table.shape
+        dev = block_table.device
+        self.device = dev
+        self.q_start = torch.zeros(self.n_req + 1, dtype=torch.int32, device=dev)
+        self.kv_len = torch.zeros(self.n_req, dtype=torch.int32, device=dev)
+        self.slots = torch.full((n_tokens,), -1, dtype=torch.int64, device=dev)
+        self.positions = torch.zeros(n_tokens, dtype=torch.int32, device=dev)
+        self._out = (block_table.data_ptr(), max(self.max_blocks, block_table.stride(0)), self.max_blocks,
+                     self.q_start.data_ptr(), self.kv_len.data_ptr(), self.slots.data_ptr(), self.positions.data_ptr(),
+                     n_tokens)
+
+    def build(self, cached_len: torch.Tensor, new_len: torch.Tensor, free_pages: torch.Tensor, n_used: torch.Tensor,
+              used_out: torch.Tensor | None = None) -> "PagedPlan":
+        """Fills the buffers for requests that hold cached_len tokens and bring
+        new_len more; new pages come from free_pages, from index n_used[0] on,
+        which advances (in place, or into used_out)."""
+        if used_out is None:
+            used_out = n_used
+        for t, n in ((cached_len, self.n_req), (new_len, self.n_req), (free_pages, None), (n_used, 1), (used_out, 1)):
+            assert t.dtype == torch.int32 and t.device == self.device and t.is_contiguous()
+            assert n is None or t.numel() == n
+        with on_device(self.device) as stream:
+            check(lib().smeai_paged_plan(cached_len.data_ptr(), new_len.data_ptr(), self.n_req, self.page_size,
+                                         free_pages.data_ptr(), free_pages.numel(), n_used.data_ptr(), used_out.data_ptr(),
+                                         *self._out, stream), "paged_plan")
+        return self
+
+
+def _rows(x: torch.Tensor, heads: int, dim: int, dtype, dev) -> int:
+    """The row stride of [n_tokens, heads, dim] whose rows are contiguous."""
+    assert x.dim() == 3 and x.shape[1] == heads and x.shape[2] == dim and x.dtype == dtype and x.device == dev
+    n, row = x.shape[0], heads * dim
+    st = x.stride()
+    assert (st[2] == 1 or dim == 1) and (st[1] == dim or heads == 1), "a token's heads lie next to one another"
+    return st[0] if n > 1 else max(row, st[0])
+
+
+def append(kv: PagedKV, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, q: torch.Tensor | None = None,
+           q_out: torch.Tensor | None = None, positions: torch.Tensor | None = None, rope: torch.Tensor | None = None,
+           halves: bool = False) -> torch.Tensor | None:
+    """Writes k, v (fp32 [n_tokens, n_kv_heads, head_dim], rows of any stride)
+    into the tokens' slots (int64, -1: left out), rotated by rope (rope_table;
+    element pairs, or halves) at positions (int32) when given, and returns q
+    (fp32 [n_tokens, n_heads, head_dim]) rotated the same way, in the cache's type."""
+    dev, dim, n = kv.device, kv.head_dim, k.shape[0]
+    ld_k, ld_v = _rows(k, kv.n_kv_heads, dim, torch.float32, dev), _rows(v, kv.n_kv_heads, dim, torch.float32, dev)
+    assert v.shape[0] == n and slots.dtype == torch.int64 and slots.device == dev and slots.numel() == n and slots.is_contiguous()
+    heads = ld_q = ld_qo = n_rope = 0
+    if q is not None:
+        heads = q.shape[1]
+        ld_q = _rows(q, heads, dim, torch.float32, dev)
+        if q_out is None:
+            q_out = torch.empty((n, heads, dim), dtype=kv.dtype, device=dev)
+        ld_qo = _rows(q_out, heads, dim, kv.dtype, dev)
+        assert q.shape[0] == q_out.shape[0] == n
+    else:
+        assert q_out is None
+    if rope is not None:
+        assert rope.dtype == torch.float32 and rope.device == dev and rope.dim() == 2 and rope.shape[1] == dim and rope.is_contiguous()
+        assert positions is not None and positions.dtype == torch.int32 and positions.device == dev
+        assert positions.numel() == n and positions.is_contiguous()
+        n_rope = rope.shape[0]
+    if n == 0:
+        return q_out
+    with on_device(dev) as stream:
+        check(lib().smeai_paged_append(kv.ref, k.data_ptr(), ld_k, v.data_ptr(), ld_v, q.data_ptr() if heads else None, ld_q,
+                                       heads, q_out.data_ptr() if heads else None, ld_qo, n, slots.data_ptr(),
+                                       positions.data_ptr() if n_rope else None, rope.data_ptr() if n_rope else None, n_rope,
+                                       halves, stream), "paged_append")
+    return q_out
+
+
+def attention(q: torch.Tensor, kv: PagedKV, block_table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor,
+              max_new: int, scale: float | None = None, causal: bool = True, out: torch.Tensor | None = None,
+              workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Context rows of q [n_tokens, n_heads, head_dim] (the cache's type; rows
+    of any stride) over the requests' pages; scale defaults to head_dim ** -0.5.
+    Rows outside q_start[0] .. q_start[-1] are not written (without `out` they
+    hold anything).  max_new: the largest number of new tokens of a request.
+    workspace: uint8 tensor of attention_workspace() bytes, one per call in
+    flight; by default it is allocated for this call."""
+    dev, dim = kv.device, kv.head_dim
+    n, heads = q.shape[0], q.shape[1]
+    ld_q = _rows(q, heads, dim, kv.dtype, dev)
+    if out is None:
+        out = torch.empty((n, heads, dim), dtype=kv.dtype, device=dev)
+    ld_out = _rows(out, heads, dim, kv.dtype, dev)
+    n_req, max_blocks = block_table.shape
+    assert out.shape[0] == n and block_table.dtype == q_start.dtype == kv_len.dtype == torch.int32
+    assert block_table.device == q_start.device == kv_len.device == dev and (block_table.stride(1) == 1 or max_blocks <= 1)
+    assert q_start.numel() == n_req + 1 and kv_len.numel() == n_req and q_start.is_contiguous() and kv_len.is_contiguous()
+    L = lib()
+    if n == 0:
+        return out
+    with on_device(dev) as stream:
+        if workspace is None:
+            workspace = torch.empty(L.smeai_paged_attention_workspace(kv.ref, heads, n, n_req, max_blocks, max_new),
+                                    dtype=torch.uint8, device=dev)
+        check(L.smeai_paged_attention(kv.ref, q.data_ptr(), ld_q, heads, n, q_start.data_ptr(), kv_len.data_ptr(), n_req,
+                                      block_table.data_ptr(), max(max_blocks, block_table.stride(0)), max_blocks, max_new,
+                                      dim ** -0.5 if scale is None else scale, causal, out.data_ptr(), ld_out,
+                                      workspace.data_ptr(), workspace.numel(), stream), "paged_attention")
+    return out
+
+
+def attention_workspace(kv: PagedKV, n_heads: int, n_tokens: int, n_req: int, max_blocks: int, max_new: int) -> int:
+    """Bytes of attention()'s workspace for calls of at most these sizes."""
+    with on_device(kv.device):
+        n = lib().smeai_paged_attention_workspace(kv.ref, n_heads, n_tokens, n_req, max_blocks, max_new)
+    if n == 0:
+        check(-1, "paged_attention_workspace")
+    return n
+
+
+__all__ = ["PagedKV", "PagedPlan", "append", "attention", "attention_workspace", "rope_table"]

@@ -18,6 +18,31 @@ def cur_stream() -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+class on_device:
+    """The stream of a device's current work, with that device current inside
+    the block (a call on another device's tensors launches there)."""
+    __slots__ = ("want", "had")
+
+    def __init__(self, dev: torch.device):
+        self.want = dev.index
+
+    def __enter__(self):
+        self.had = torch.cuda.current_device()
+        if self.want is not None and self.had != self.want:
+            torch.cuda.set_device(self.want)
+        return torch.cuda.current_stream().cuda_stream
+
+    def __exit__(self, *exc):
+        if self.want is not None and self.had != self.want:
+            torch.cuda.set_device(self.had)
+        return False
+
+
+def _ld(x: torch.Tensor) -> int:
+    """Row stride of a 2-d tensor; a single row's stride says nothing."""
+    return x.stride(0) if x.shape[0] > 1 else max(x.shape[1], x.stride(0))
+
+
 def quantize_q8k(x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
     """fp32 [n, k] (cuda) -> ggml block_q8_K rows, uint8 [n, k/256*292]."""
     x2 = x.reshape(-1, x.shape[-1])
@@ -45,6 +70,33 @@ def rms_quantize_q8k(x: torch.Tensor, eps: float, out: torch.Tensor | None = Non
         check(lib().smeai_rms_q8k_quantize_w(_ptr(x2), x2.stride(0), n, k, _ptr(norm_w), ctypes.c_float(eps),
                                               _ptr(out), cur_stream()), "rms_q8k_quantize_w")
     return out
+
+
+def add_rms_quantize_q8k(x: torch.Tensor, resid: torch.Tensor, eps: float, out: torch.Tensor | None = None,
+                         sum_out: torch.Tensor | None = None, norm_w: torch.Tensor | None = None):
+    """h = x + resid, then rms_quantize_q8k(h, eps, norm_w=norm_w) in the same
+    kernel; returns (h, blocks).  x, resid and sum_out: fp32 [n, k] (cuda),
+    rows of any stride; sum_out may be x or resid themselves."""
+    n, k = x.shape
+    dev = x.device
+    if sum_out is None:
+        sum_out = torch.empty((n, k), dtype=torch.float32, device=dev)
+    if out is None:
+        out = torch.empty((n, k // QK_K * Q8K_BLOCK_BYTES), dtype=torch.uint8, device=dev)
+    assert x.is_cuda and x.dtype == resid.dtype == sum_out.dtype == torch.float32
+    assert resid.shape == sum_out.shape == x.shape and resid.device == sum_out.device == out.device == dev
+    assert k == 1 or x.stride(1) == resid.stride(1) == sum_out.stride(1) == 1
+    assert out.dtype == torch.uint8 and out.is_contiguous() and out.numel() == n * (k // QK_K) * Q8K_BLOCK_BYTES
+    if norm_w is not None:
+        assert norm_w.dtype == torch.float32 and norm_w.device == dev and norm_w.numel() == k and norm_w.is_contiguous()
+    if n == 0:
+        return sum_out, out
+    with on_device(dev) as stream:
+        check(lib().smeai_add_rms_q8k_quantize(x.data_ptr(), _ld(x), resid.data_ptr(), _ld(resid), n, k,
+                                               None if norm_w is None else norm_w.data_ptr(), eps,
+                                               sum_out.data_ptr(), _ld(sum_out), out.data_ptr(), stream),
+              "add_rms_q8k_quantize")
+    return sum_out, out
 
 
 def quantize_q2k(x: torch.Tensor) -> torch.Tensor:
@@ -190,7 +242,7 @@ class Q2KMatrix:
             pass
 
 
-__all__ = ["quantize_q8k", "rms_quantize_q8k", "quantize_q2k", "dequantize_q2k", "Q2KMatrix", "Q3KMatrix",
+__all__ = ["quantize_q8k", "rms_quantize_q8k", "add_rms_quantize_q8k", "quantize_q2k", "dequantize_q2k", "Q2KMatrix", "Q3KMatrix",
            "dequantize_q3k", "Q6KMatrix", "dequantize_q6k", "as_bytes",
            "EPI_STORE", "EPI_RESIDUAL", "EPI_SILU_MUL"]
 
