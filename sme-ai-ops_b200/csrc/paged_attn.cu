@@ -411,78 +411,107 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_kernel
   pdl_trigger();
 }
 
-// Joins the pieces of each tile that some CTA left unfinished: the CTA's slot
-// 1, then slot 0 of the CTAs after it up to the one where the tile ends.  One
-// CTA a (tile, row slice); a warp takes every eighth piece of a row, all lanes
-// the row's columns, and the warps' sums meet in shared memory in warp order.
+// The pieces of the tile that CTA c left unfinished: c's slot 1, then slot 0 of
+// the CTAs after it up to the one where the tile ends.
+__device__ __forceinline__ int join_pieces(const AttnParams& p, int c, int ctas) {
+  const int lane = threadIdx.x & 31;
+  for (int i = c + 1;; i += 32) {
+    const int st = i + lane < ctas ? p.head[i + lane].w : kPartEnds;   // the last CTA ends the line
+    const unsigned ends = __ballot_sync(0xffffffffu, st == kPartEnds);
+    if (ends) return min(i + __ffs(ends) - c, ctas - c);
+  }
+}
+__device__ __forceinline__ int64_t join_slot(int c, int i) {
+  return i == 0 ? 2 * (int64_t)c + 1 : 2 * (int64_t)(c + i);
+}
+template <int TR>
+__device__ __forceinline__ float join_top(const AttnParams& p, int c, int n, int row_t) {
+  float top = kNegInf;
+  for (int i = threadIdx.x & 31; i < n; i += 32) top = fmaxf(top, p.part_ml[join_slot(c, i) * TR + row_t].x);
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+  return top;
+}
+// a[], sum += pieces i0, i0 + step, ..; lane's columns: kCols consecutive ones a span of 32 * kCols
+template <int TR, int DP, int kCols>
+__device__ __forceinline__ void join_add(const AttnParams& p, int c, int n, int row_t, int i0, int step, float top,
+                                         float* a, float& sum) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll 4
+  for (int i = i0; i < n; i += step) {
+    const float2 ml = p.part_ml[join_slot(c, i) * TR + row_t];
+    const float* src = p.part_o + (join_slot(c, i) * TR + row_t) * DP + lane * kCols;
+    float v[DP / 32];
+#pragma unroll
+    for (int s = 0; s < DP / (32 * kCols); ++s) {
+      if (kCols == 4) *reinterpret_cast<float4*>(v + 4 * s) = *reinterpret_cast<const float4*>(src + s * 128);
+      else *reinterpret_cast<float2*>(v + 2 * s) = *reinterpret_cast<const float2*>(src + s * 64);
+    }
+    if (ml.y == 0.f) continue;      // saw no key; its context may not have been written
+    const float f = exp2_fast(ml.x - top);
+    sum = fmaf(ml.y, f, sum);
+#pragma unroll
+    for (int k = 0; k < DP / 32; ++k) a[k] = fmaf(v[k], f, a[k]);
+  }
+}
+
+// Joins the pieces of tiles that CTAs left unfinished, in key order.
+// kSplit (tiles of 16 rows, up to hundreds of pieces): a warp takes every
+// eighth piece of a row, and the warps' sums meet in shared memory in warp
+// order.  Otherwise a warp takes a row: tiles of 64 and 256 rows have few
+// pieces and many rows.
 template <typename T, int TR, int DP>
 __global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnParams p, int ctas) {
-  constexpr int kCols = DP >= 128 ? 4 : 2;            // consecutive columns a lane
-  constexpr int kSpans = DP / (32 * kCols);           // 1, or 2 at DP 256
-  __shared__ float acc[8][DP];
+  constexpr int kCols = DP >= 128 ? 4 : 2;
+  constexpr bool kSplit = TR == 16;
+  __shared__ float acc[kSplit ? 8 : 1][DP];
   __shared__ float wsum[8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x;
   pdl_wait();
   const int4 hd = p.head[c];
   if (hd.x < 0) return;
-  // pieces: the first CTA after c whose slot 0 ends the tile
-  int n = 0;
-  for (int i = c + 1; n == 0 && i < ctas; i += 32) {
-    const int st = i + lane < ctas ? p.head[i + lane].w : kPartEnds;   // the last CTA ends the line
-    const unsigned ends = __ballot_sync(0xffffffffu, st == kPartEnds);
-    if (ends) n = i + __ffs(ends) - c;
-  }
-  if (n == 0) return;
-  if (c + n > ctas) n = ctas - c;
-  auto slot = [&](int i) -> int64_t { return i == 0 ? 2 * (int64_t)c + 1 : 2 * (int64_t)(c + i); };
+  const int n = join_pieces(p, c, ctas);
   const AttnReq r = attn_req(p, hd.x);
-  for (int row_t = blockIdx.y; row_t < TR; row_t += gridDim.y) {
-    const int row = hd.y * TR + row_t;
-    if (row >= r.rows) return;
-    float top = kNegInf;
-    for (int i = lane; i < n; i += 32) top = fmaxf(top, p.part_ml[slot(i) * TR + row_t].x);
+  const int rows = min(TR, r.rows - hd.y * TR);
+  auto dst_row = [&](int row) {
+    const int tok = row / p.group, head = hd.z * p.group + row % p.group;
+    return p.out + (int64_t)(r.q0 + tok) * p.ld_out + (int64_t)head * p.kv.dim * 2;
+  };
+  if (kSplit) {
+    for (int row_t = blockIdx.y; row_t < rows; row_t += gridDim.y) {
+      const float top = join_top<TR>(p, c, n, row_t);
+      float a[DP / 32] = {}, sum = 0.f;
+      join_add<TR, DP, kCols>(p, c, n, row_t, warp, 8, top, a, sum);
 #pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-    float a[kSpans * kCols] = {}, sum = 0.f;
-#pragma unroll 4
-    for (int i = warp; i < n; i += 8) {
-      const float2 ml = p.part_ml[slot(i) * TR + row_t];
-      const float f = ml.x == kNegInf ? 0.f : exp2_fast(ml.x - top);
-      sum = fmaf(ml.y, f, sum);
-      const float* src = p.part_o + (slot(i) * TR + row_t) * DP + lane * kCols;
+      for (int k = 0; k < DP / 32; ++k) acc[kSplit ? warp : 0][(k / kCols) * 32 * kCols + lane * kCols + k % kCols] = a[k];
+      if (lane == 0) wsum[warp] = sum;
+      __syncthreads();
+      float total = 0.f;
 #pragma unroll
-      for (int s = 0; s < kSpans; ++s) {
-        float v[4];
-        if (kCols == 4) {
-          const float4 x = *reinterpret_cast<const float4*>(src + s * 128);
-          v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-        } else {
-          const float2 x = *reinterpret_cast<const float2*>(src);
-          v[0] = x.x; v[1] = x.y;
-        }
+      for (int ww = 0; ww < 8; ++ww) total += wsum[ww];
+      const float inv = total > 0.f ? 1.f / total : (total == 0.f ? 0.f : total);
+      uint16_t* dst = reinterpret_cast<uint16_t*>(dst_row(hd.y * TR + row_t));
+      for (int d = threadIdx.x; d < p.kv.dim; d += 256) {
+        float v = 0.f;
 #pragma unroll
-        for (int k = 0; k < kCols; ++k) a[s * kCols + k] = fmaf(v[k], f, a[s * kCols + k]);
+        for (int ww = 0; ww < 8; ++ww) v += acc[kSplit ? ww : 0][d];
+        dst[d] = Num<T>::one(v * inv);
+      }
+      __syncthreads();
+    }
+  } else {
+    for (int row_t = blockIdx.y * 8 + warp; row_t < rows; row_t += gridDim.y * 8) {
+      const float top = join_top<TR>(p, c, n, row_t);
+      float a[DP / 32] = {}, sum = 0.f;
+      join_add<TR, DP, kCols>(p, c, n, row_t, 0, 1, top, a, sum);
+      const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+      char* dst = dst_row(hd.y * TR + row_t);
+#pragma unroll
+      for (int k = 0; k < DP / 32; k += 2) {
+        const int d = (k / kCols) * 32 * kCols + lane * kCols + k % kCols;
+        if (d < p.kv.dim) *reinterpret_cast<uint32_t*>(dst + d * 2) = Num<T>::pack(a[k] * inv, a[k + 1] * inv);
       }
     }
-#pragma unroll
-    for (int s = 0; s < kSpans; ++s)
-#pragma unroll
-      for (int k = 0; k < kCols; ++k) acc[warp][s * 128 + lane * kCols + k] = a[s * kCols + k];
-    if (lane == 0) wsum[warp] = sum;
-    __syncthreads();
-    float total = 0.f;
-#pragma unroll
-    for (int ww = 0; ww < 8; ++ww) total += wsum[ww];
-    const float inv = total > 0.f ? 1.f / total : (total == 0.f ? 0.f : total);
-    const int tok = row / p.group, head = hd.z * p.group + row % p.group;
-    uint16_t* dst = reinterpret_cast<uint16_t*>(p.out + (int64_t)(r.q0 + tok) * p.ld_out) + (int64_t)head * p.kv.dim;
-    for (int d = threadIdx.x; d < p.kv.dim; d += 256) {
-      float v = 0.f;
-#pragma unroll
-      for (int ww = 0; ww < 8; ++ww) v += acc[ww][d];
-      dst[d] = Num<T>::one(v * inv);
-    }
-    __syncthreads();
   }
 }
 
@@ -500,31 +529,77 @@ int run_class(AttnParams p, const PagedAttention& a, int sms, cudaStream_t strea
   return kOk;
 }
 
-template <typename T, int DP>
-int run_dim(const AttnParams& p, const PagedAttention& a, int sms, cudaStream_t stream) {
-  const int64_t most = a.max_new * p.group;      // packed rows of the largest request
-  if (most <= 16) return run_class<T, DP, false>(p, a, sms, stream);
-  return run_class<T, DP, true>(p, a, sms, stream);
+// Which kernels a call needs, from what the host knows: the largest request's
+// packed rows and the total.
+//   up to 16 rows   the 16-row tiles: keys split over the warps
+//   up to 64        the 64-row tiles
+//   more            the tensor-core kernel, and the 16-row tiles beside it for
+//                   requests of up to 16 rows (a step that mixes prompts and
+//                   decoding) unless the total says that there are none;
+//                   head_dim above 128: the 64-row tiles for all
+struct Classes {
+  bool few, mid, many;
+};
+Classes classes(const PagedAttention& a) {
+  const int64_t group = a.n_heads / a.kv.n_kv, most = a.max_new * group;
+  Classes c = {false, false, false};
+  if (most <= 16) c.few = true;
+  else if (most <= 64 || a.kv.dim > 128) c.mid = true;
+  else {
+    c.many = true;
+    // with one request of r <= 16 / group rows the others, of max_new at most, could not make up n_tokens
+    c.few = a.n_tokens <= (a.n_req - 1) * a.max_new + 16 / group;
+  }
+  return c;
 }
 
 int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+
+template <typename T, int DP>
+int run_dim(const AttnParams& p, const PagedAttention& a, int sms, cudaStream_t stream) {
+  const Classes c = classes(a);
+  if (c.few) {
+    AttnParams q = p;
+    if (c.many) q.rows_hi = 16;
+    const int st = run_class<T, DP, false>(q, a, sms, stream);
+    if (st) return st;
+  }
+  if (c.mid) return run_class<T, DP, true>(p, a, sms, stream);
+  if (c.many && DP <= 128) {
+    AttnParams q = p;
+    if (c.few) q.rows_lo = 16;
+    return paged_attn_tc(q, DP, a.workspace, a.max_kv, sms, stream);
+  }
+  return kOk;
+}
 
 }  // namespace
 
 template <typename T, int TR, int DP>
 cudaError_t attn_join(const AttnParams& p, int ctas, cudaStream_t stream) {
-  return launch(paged_attn_join_kernel<T, TR, DP>, dim3((unsigned)ctas, 4u), dim3(256), 0, stream, p, ctas);
+  const unsigned slices = TR == 16 ? 4u : TR / 16;
+  return launch(paged_attn_join_kernel<T, TR, DP>, dim3((unsigned)ctas, slices), dim3(256), 0, stream, p, ctas);
 }
+template cudaError_t attn_join<__half, 256, 64>(const AttnParams&, int, cudaStream_t);
+template cudaError_t attn_join<__half, 256, 128>(const AttnParams&, int, cudaStream_t);
+template cudaError_t attn_join<__nv_bfloat16, 256, 64>(const AttnParams&, int, cudaStream_t);
+template cudaError_t attn_join<__nv_bfloat16, 256, 128>(const AttnParams&, int, cudaStream_t);
 
 size_t paged_attention_workspace(const PagedAttention& a) {
   int sms = 0;
   if (sm_count(&sms)) return 0;
-  const bool few = a.max_new * (a.n_heads / a.kv.n_kv) <= 16;
-  switch (padded_dim(a.kv.dim)) {
-    case 64: return few ? attn_part_bytes<16, 64>(2 * sms) : attn_part_bytes<64, 64>(2 * sms);
-    case 128: return few ? attn_part_bytes<16, 128>(2 * sms) : attn_part_bytes<64, 128>(2 * sms);
-    default: return few ? attn_part_bytes<16, 256>(sms) : attn_part_bytes<64, 256>(sms);
+  const Classes c = classes(a);
+  const int dp = padded_dim(a.kv.dim);
+  size_t few = 0, mid = 0;
+  switch (dp) {
+    case 64: few = attn_part_bytes<16, 64>(2 * sms), mid = attn_part_bytes<64, 64>(2 * sms); break;
+    case 128: few = attn_part_bytes<16, 128>(2 * sms), mid = attn_part_bytes<64, 128>(2 * sms); break;
+    default: few = attn_part_bytes<16, 256>(sms), mid = attn_part_bytes<64, 256>(sms);
   }
+  size_t need = c.few ? few : 0;
+  if (c.mid && mid > need) need = mid;
+  const size_t many = c.many ? paged_attn_tc_workspace(dp, sms) : 0;
+  return many > need ? many : need;
 }
 
 int paged_attention(const PagedAttention& a, cudaStream_t stream) {

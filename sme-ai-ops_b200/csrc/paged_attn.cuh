@@ -249,6 +249,11 @@ void attn_carve(AttnParams& p, void* ws, int ctas) {
   p.head = reinterpret_cast<int4*>(c);
 }
 
+// The tensor-core kernel of requests with many rows, head_dim up to 128
+// (paged_attn_tc.cu): one CTA an SM.
+size_t paged_attn_tc_workspace(int padded_dim, int sms);
+int paged_attn_tc(const AttnParams& p, int padded_dim, void* workspace, int max_kv, int sms, cudaStream_t stream);
+
 // Joins the partial results (paged_attn.cu).
 template <typename T, int TR, int DP>
 cudaError_t attn_join(const AttnParams& p, int ctas, cudaStream_t stream);

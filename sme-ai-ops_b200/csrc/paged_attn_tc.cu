@@ -1,0 +1,574 @@
+// paged_attn_tc.cu -- attention of new tokens over a paged key/value cache for
+// requests that bring many rows (a prompt, a chunk of one), on the sm_100a
+// tensor cores.
+//
+// The mathematics is that of paged_attn.cu, on tiles of 256 packed rows (two
+// halves of 128, the MMA's M) and blocks of 128 keys:
+//   S_t = Q_t K^T      tcgen05.mma, both operands in shared memory, fp32 in TMEM
+//   P_t = 2^(c S_t - m) in registers: a thread owns a row, so its maximum and
+//                      sum need no exchange; P replaces S in TMEM as 16-bit pairs
+//   O_t += P_t V       tcgen05.mma with P read from TMEM, O fp32 in TMEM
+// The running maximum is only raised when it grows by more than 2^8 (P then
+// stays below 2^8, or 2^15 with half's bias), so O, which has to be rescaled
+// when it is, is touched rarely; the thread that owns the row does it.
+//
+// Warp roles (16 warps, one CTA an SM):
+//   warps 0-3, 4-7   softmax of half 0 and half 1 (192 registers a thread)
+//   warps 8-11       load: queries, keys and values with 16-byte cp.async into
+//                    the 128-byte-swizzled layout the MMA reads; rows may lie
+//                    anywhere, so any page size and stride costs the same
+//   warp 12          allocates TMEM; one lane issues the MMAs
+// While one half's softmax runs, the tensor core works for the other: in issue
+// order PV_0(j), QK_0(j+1), PV_1(j), QK_1(j+1).  At 128 elements a block
+// takes 4 x 128^3 multiply-adds for the tensor core (2048 cycles at its rate)
+// and 2 x 128 x 128 exponentials (2048 cycles at 16 a cycle): the two are
+// nearly in balance, and both halves' softmax has to hide behind the MMAs.
+//
+// Every wait is bounded by wall time; on expiry the kernel records
+// kDevErrTimeout, all roles stop, copies and MMAs in flight are drained, TMEM
+// is freed and the kernel returns.  No multicast.
+#include "paged_attn.cuh"
+#include "tcgen05.cuh"
+
+namespace smeai {
+
+namespace {
+
+constexpr int kTR = 256;             // packed rows a tile
+constexpr int kKB = 128;             // keys a block
+constexpr int kThreads = 512;
+constexpr int kLoadWarp0 = 8, kMmaWarp = 12;
+constexpr int kAtom = 128 * 128;     // 128 rows x 128 bytes
+constexpr int kTmemCols = 512;       // S0 S1 (128 columns each), O0 O1 (up to 128 each)
+constexpr int kLag = 2;              // copied items not yet announced
+constexpr float kRaise = 8.f;        // growth of the maximum (log2) that rescales O
+constexpr float kNegInf = -INFINITY;
+
+template <int DP>
+struct Tc {
+  static constexpr int kCb = DP / 64;              // 64-element column blocks
+  static constexpr int kItem = kCb * kAtom;        // bytes of 128 rows
+  static constexpr int kSlots = DP == 128 ? 4 : 8; // ring of key and value blocks: 128 KB
+  static constexpr int kQBytes = 2 * kItem;
+  static constexpr size_t kSmem = 1024 + (size_t)kQBytes + (size_t)kSlots * kItem + 256;
+};
+
+struct TcSmem {
+  uint8_t* q;
+  uint8_t* ring;
+  uint64_t *full, *empty;            // per slot: 4 load warps; one commit
+  uint64_t* q_empty;                 // commit: the tile's last QK has read the queries
+  uint64_t *s_full, *p_full, *o_full;  // per half: commit; 4 warps; commit
+  uint64_t* drain;
+  uint32_t* tmem;
+  int* abort;
+};
+
+template <int DP>
+__device__ __forceinline__ TcSmem carve(uint8_t* base) {
+  TcSmem m;
+  uint8_t* p = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(base) + 1023) & ~(uintptr_t)1023);
+  m.q = p;
+  m.ring = p + Tc<DP>::kQBytes;
+  uint64_t* b = reinterpret_cast<uint64_t*>(m.ring + (size_t)Tc<DP>::kSlots * Tc<DP>::kItem);
+  m.full = b;
+  m.empty = b + 8;
+  m.q_empty = b + 16;
+  m.s_full = b + 17;
+  m.p_full = b + 19;
+  m.o_full = b + 21;
+  m.drain = b + 23;
+  m.tmem = reinterpret_cast<uint32_t*>(b + 24);
+  m.abort = reinterpret_cast<int*>(b + 25);
+  return m;
+}
+
+// Bounded wait that also gives up once another role has.
+__device__ __forceinline__ bool wait_or_abort(const TcSmem& m, uint64_t* bar, unsigned parity, unsigned* err,
+                                              uint64_t limit_ns) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = global_timer_ns();
+  for (;;) {
+    for (int i = 0; i < 32; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (*reinterpret_cast<volatile int*>(m.abort)) return false;
+    if (global_timer_ns() - t0 > limit_ns) {
+      *reinterpret_cast<volatile int*>(m.abort) = 1;
+      raise_device_error(err, kDevErrTimeout);
+      return false;
+    }
+  }
+}
+__device__ __forceinline__ bool wait_warp(const TcSmem& m, uint64_t* bar, unsigned parity, unsigned* err,
+                                          uint64_t limit_ns) {
+  return __all_sync(0xffffffffu, wait_or_abort(m, bar, parity, err, limit_ns));
+}
+
+// D[tmem] (+)= A[tmem] * B[smem desc]^T, 16-bit inputs, fp32 accumulate.
+__device__ __forceinline__ void tc_mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                              uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}"
+      :
+      : "r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
+        "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+        "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const float* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+      "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]),
+      "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]), "f"(v[16]), "f"(v[17]), "f"(v[18]),
+      "f"(v[19]), "f"(v[20]), "f"(v[21]), "f"(v[22]), "f"(v[23]), "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]),
+      "f"(v[28]), "f"(v[29]), "f"(v[30]), "f"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          addr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// Keeps uses of a load's registers behind the wait before it.
+__device__ __forceinline__ void pin32(float* v) {
+  asm volatile(""
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                 "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]),
+                 "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]),
+                 "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]),
+                 "+f"(v[30]), "+f"(v[31]));
+}
+
+// Instruction descriptor: M = 128, fp32 accumulator, fp16 (0) or bf16 (1)
+// operands; bit 16: operand B has its N dimension contiguous (the values, [key][element]).
+__host__ __device__ constexpr uint32_t idesc(bool bf16, int n, bool b_n_major) {
+  return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_n_major ? 1u : 0u) << 16) |
+         ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+
+template <typename T>
+struct IsBf16 {
+  static constexpr bool value = false;
+};
+template <>
+struct IsBf16<__nv_bfloat16> {
+  static constexpr bool value = true;
+};
+
+// One CTA's stretch of a tile: key blocks kb0 .. kb0 + n of it; half t works on
+// the first cnt[t] of them (causal: the lower rows see fewer keys).
+struct Stretch {
+  int kb0, n, cnt[2];
+  bool last;   // reaches the tile's end
+};
+__device__ __forceinline__ Stretch stretch(const AttnParams& p, const AttnPos& w, int64_t left) {
+  Stretch s;
+  s.kb0 = w.kb;
+  const int to_end = w.nkb - w.kb;
+  s.n = left < to_end ? (int)left : to_end;
+  s.last = s.n == to_end;
+  const bool two = w.rt * kTR + 128 < w.r.rows;
+  s.cnt[0] = s.n;
+  s.cnt[1] = two ? s.n : 0;
+  if (two) s.cnt[0] = max(0, min(s.n, attn_blocks<128, kKB>(p, w.r, 2 * w.rt) - w.kb));
+  return s;
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnParams p, uint64_t limit_ns) {
+  using C = Tc<DP>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ AttnShare share;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const TcSmem m = carve<DP>(smem_raw);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 8; ++i) {
+      mbar_init(&m.full[i], 4);
+      mbar_init(&m.empty[i], 1);
+    }
+    mbar_init(m.q_empty, 1);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&m.s_full[t], 1);
+      mbar_init(&m.p_full[t], 4);
+      mbar_init(&m.o_full[t], 1);
+    }
+    mbar_init(m.drain, 1);
+    *m.abort = 0;
+    mbar_fence_init();
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(m.tmem)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_wait();
+  attn_share<kTR, kKB, kThreads>(p, &share);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *m.tmem;
+  const int64_t units = share.u1 - share.u0;
+  if (threadIdx.x == 0) p.head[blockIdx.x] = make_int4(-1, 0, 0, kPartNone);
+
+  if (units <= 0) {
+    // nothing to do
+  } else if (warp >= kLoadWarp0 && warp < kLoadWarp0 + 4) {
+    // ---------------- load
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    const int lw = warp - kLoadWarp0;
+    AttnPos w;
+    attn_open<kTR, kKB>(p, share, w);
+    const int page_mask = (1 << p.kv.page_log2) - 1;
+    int64_t left = units;
+    int it = 0, told = 0;          // items copied, items announced
+    int tiles = 0;
+    bool ok = true;
+    // announce the items whose copies have landed (all but the newest `keep`)
+    auto tell = [&](int keep) {
+      fence_async_smem();
+      __syncwarp();
+      for (; told < it - keep; ++told)
+        if (lane == 0) mbar_arrive(&m.full[told % C::kSlots]);
+    };
+    // a free slot for item `it`; what is in flight is announced before a long wait
+    auto acquire = [&]() {
+      if (it < C::kSlots) return true;
+      uint64_t* bar = &m.empty[it % C::kSlots];
+      const unsigned parity = (unsigned)((it / C::kSlots - 1) & 1);
+      if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+      cp_async_wait<0>();
+      tell(0);
+      return wait_warp(m, bar, parity, p.err, limit_ns);
+    };
+    constexpr int kChunks = DP / 8;
+    constexpr int kPer = 32 * kChunks / 32;      // chunks a lane copies of an item
+    auto copy_rows = [&](uint8_t* dst, const char* src, int64_t off, int row0) {
+#pragma unroll 4
+      for (int i = 0; i < kPer; ++i) {
+        const int c = i * 32 + lane, row = c / kChunks, col = c % kChunks;
+        const int64_t o = __shfl_sync(0xffffffffu, off, row);
+        const int n = o >= 0 && col * 8 < p.kv.dim ? 16 : 0;
+        const int r = row0 + row;
+        cp_async16(smem_addr(dst) + (col >> 3) * kAtom + r * 128 + (((col & 7) ^ (r & 7)) << 4),
+                   src + (n ? o + col * 16 : 0), n);
+      }
+    };
+    while (left > 0 && ok) {
+      const Stretch s = stretch(p, w, left);
+      const int32_t* table = p.table + (int64_t)w.b * p.ld_table;
+      auto look_up = [&](int kb) {   // byte offset of this lane's key row; -1: zeros
+        const int key = kb * kKB + lw * 32 + lane;
+        if (key >= w.r.kv) return (int64_t)-1;
+        const int page = table[key >> p.kv.page_log2];
+        if (page < 0 || page >= p.kv.n_pages) {
+          raise_device_error(p.err, kDevErrBadIndex);
+          return (int64_t)-1;
+        }
+        return page * p.kv.page_bytes + (key & page_mask) * p.kv.token_bytes + w.h * p.kv.head_bytes;
+      };
+      int64_t off = look_up(s.kb0);
+      for (int b = 0; b < s.n && ok; ++b) {
+        const int64_t next = b + 1 < s.n ? look_up(s.kb0 + b + 1) : -1;
+        if (!(ok = acquire())) break;
+        if (b == 0) {
+          // the tile's queries, announced with its first keys; their place is free
+          // once the previous tile's last keys, copied but perhaps not yet
+          // announced, have been read
+          if (tiles > 0) {
+            const unsigned parity = (unsigned)((tiles - 1) & 1);
+            if (!__all_sync(0xffffffffu, mbar_try_wait(m.q_empty, parity))) {
+              cp_async_wait<0>();
+              tell(0);
+              if (!(ok = wait_warp(m, m.q_empty, parity, p.err, limit_ns))) break;
+            }
+          }
+#pragma unroll
+          for (int q4 = 0; q4 < 2; ++q4) {
+            const int r = lw * 64 + q4 * 32 + lane, row = w.rt * kTR + r;
+            int64_t qoff = -1;
+            if (row < w.r.rows) {
+              const int tok = row / p.group, hd = w.h * p.group + row % p.group;
+              qoff = (int64_t)(w.r.q0 + tok) * p.ld_q + (int64_t)hd * p.kv.dim * 2;
+            }
+            copy_rows(m.q + (lw >> 1) * C::kItem, p.q, qoff, (lw & 1) * 64 + q4 * 32);
+          }
+        }
+        copy_rows(m.ring + (size_t)(it % C::kSlots) * C::kItem, p.kv.k, off, lw * 32);
+        cp_async_commit();
+        ++it;
+        cp_async_wait<kLag>();
+        tell(kLag);
+        if (!(ok = acquire())) break;
+        copy_rows(m.ring + (size_t)(it % C::kSlots) * C::kItem, p.kv.v, off, lw * 32);
+        cp_async_commit();
+        ++it;
+        cp_async_wait<kLag>();
+        tell(kLag);
+        off = next;
+      }
+      left -= s.n;
+      ++tiles;
+      if (left > 0) attn_next_tile<kTR, kKB>(p, w);
+    }
+    cp_async_wait<0>();
+    tell(0);
+  } else if (warp >= kMmaWarp) {
+    // ---------------- issue the MMAs
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp == kMmaWarp && lane == 0) {
+      constexpr uint32_t kQk = idesc(IsBf16<T>::value, kKB, false), kPv = idesc(IsBf16<T>::value, DP, true);
+      AttnPos w;
+      attn_open<kTR, kKB>(p, share, w);
+      int64_t left = units;
+      int it = 0;
+      unsigned pc[2] = {0, 0};
+      bool ok = true;
+      auto qk = [&](int t, int item) {
+        const uint8_t* kb = m.ring + (size_t)(item % C::kSlots) * C::kItem;
+        const uint64_t a0 = smem_desc(m.q + t * C::kItem, 16, 1024, kLayoutSw128);
+        const uint64_t b0 = smem_desc(kb, 16, 1024, kLayoutSw128);
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) {
+          const uint64_t step = (uint64_t)(((ks >> 2) * kAtom + (ks & 3) * 32) >> 4);
+          tc_mma_f16(tmem + t * 128, a0 + step, b0 + step, kQk, ks > 0);
+        }
+      };
+      auto pv = [&](int t, int item, bool first) {
+        const uint8_t* vb = m.ring + (size_t)(item % C::kSlots) * C::kItem;
+        const uint64_t b0 = smem_desc(vb, kAtom, 1024, kLayoutSw128);
+#pragma unroll
+        for (int ks = 0; ks < kKB / 16; ++ks)
+          tc_mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + ks * 8, b0 + (uint64_t)((ks * 2048) >> 4), kPv,
+                        !(first && ks == 0));
+      };
+      auto full = [&](int item) {
+        return wait_or_abort(m, &m.full[item % C::kSlots], (unsigned)((item / C::kSlots) & 1), p.err, limit_ns);
+      };
+      while (left > 0 && ok) {
+        const Stretch s = stretch(p, w, left);
+        if (!(ok = full(it))) break;
+        tc_fence_after();
+        for (int t = 0; t < 2; ++t)
+          if (s.cnt[t] > 0) {
+            qk(t, it);
+            tc_commit(&m.s_full[t]);
+          }
+        tc_commit(&m.empty[it % C::kSlots]);
+        if (s.n == 1) tc_commit(m.q_empty);
+        for (int b = 0; b < s.n && ok; ++b) {
+          const int iv = it + 2 * b + 1, ik = iv + 1;
+          const bool more = b + 1 < s.n;
+          if (!(ok = full(iv) && (!more || full(ik)))) break;
+          for (int t = 0; t < 2; ++t) {
+            if (b >= s.cnt[t]) continue;
+            if (!(ok = wait_or_abort(m, &m.p_full[t], pc[t] & 1, p.err, limit_ns))) break;
+            ++pc[t];
+            tc_fence_after();
+            pv(t, iv, b == 0);
+            if (b + 1 < s.cnt[t]) {
+              qk(t, ik);
+              tc_commit(&m.s_full[t]);
+            } else {
+              tc_commit(&m.o_full[t]);
+            }
+          }
+          if (!ok) break;
+          tc_commit(&m.empty[iv % C::kSlots]);
+          if (more) tc_commit(&m.empty[ik % C::kSlots]);
+          if (b + 2 == s.n) tc_commit(m.q_empty);
+        }
+        it += 2 * s.n;
+        left -= s.n;
+        if (left > 0) attn_next_tile<kTR, kKB>(p, w);
+      }
+      // everything issued has finished before TMEM is freed
+      tc_commit(m.drain);
+      mbar_wait_bounded(m.drain, 0, limit_ns);
+    }
+    __syncwarp();
+  } else {
+    // ---------------- softmax of half t, one row a thread
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    const int t = warp >> 2, r = (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_col = tmem + lanes + t * 128, o_col = tmem + lanes + 256 + t * 128;
+    AttnPos w;
+    attn_open<kTR, kKB>(p, share, w);
+    int64_t left = units;
+    unsigned sc = 0, oc = 0;
+    bool ok = true;
+    while (left > 0 && ok) {
+      const Stretch s = stretch(p, w, left);
+      const int row = w.rt * kTR + t * 128 + r;
+      const bool live = row < w.r.rows;
+      const int lim = live ? min(w.r.kv, attn_limit(p, w.r, row)) : 0;
+      const int lim_all = min(w.r.kv, attn_limit(p, w.r, w.rt * kTR + t * 128));
+      float mx = kNegInf, l = 0.f;
+      const int cnt = s.cnt[t];
+      for (int b = 0; b < cnt; ++b) {
+        if (!(ok = wait_warp(m, &m.s_full[t], sc & 1, p.err, limit_ns))) break;
+        ++sc;
+        tc_fence_after();
+        float v[128];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tmem_ld32(s_col + i * 32, v + i * 32);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pin32(v + i * 32);
+        const int key0 = (s.kb0 + b) * kKB;
+        if (key0 + kKB > lim_all) {
+#pragma unroll
+          for (int i = 0; i < 128; ++i)
+            if (key0 + i >= lim) v[i] = kNegInf;
+        }
+        float top[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+        for (int i = 4; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], v[i]);
+        const float mn = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
+        const bool raise = mn > mx + kRaise || (mx == kNegInf && mn > mx);
+        if (__any_sync(0xffffffffu, raise)) {
+          const float f = raise ? exp2_fast(mx - mn) : 1.f;
+          if (raise) mx = mn;
+          l *= f;
+          if (b > 0) {
+#pragma unroll 1
+            for (int i = 0; i < DP / 32; ++i) {
+              float o[32];
+              tmem_ld32(o_col + i * 32, o);
+              tmem_ld_wait();
+              pin32(o);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) o[k] *= f;
+              tmem_st32(o_col + i * 32, o);
+            }
+          }
+        }
+        const float sub = mx == kNegInf ? 0.f : Num<T>::kBias - mx;
+        const uint64_t c2 = pack_f32x2(p.scale_log2, p.scale_log2), sub2 = pack_f32x2(sub, sub);
+        uint64_t sum2[2] = {0ull, 0ull};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t w16[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            const uint64_t x = fma_f32x2(pack_f32x2(v[i * 32 + 2 * k], v[i * 32 + 2 * k + 1]), c2, sub2);
+            const float e0 = exp2_fast(__uint_as_float((uint32_t)x)), e1 = exp2_fast(__uint_as_float((uint32_t)(x >> 32)));
+            sum2[k & 1] = add_f32x2(sum2[k & 1], pack_f32x2(e0, e1));
+            w16[k] = Num<T>::pack(e0, e1);
+          }
+          tmem_st16(s_col + i * 16, w16);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&m.p_full[t]);
+        sum2[0] = add_f32x2(sum2[0], sum2[1]);
+        l += __uint_as_float((uint32_t)sum2[0]) + __uint_as_float((uint32_t)(sum2[0] >> 32));
+      }
+      if (!ok) break;
+      if (cnt > 0) {
+        if (!(ok = wait_warp(m, &m.o_full[t], oc & 1, p.err, limit_ns))) break;
+        ++oc;
+        tc_fence_after();
+      }
+      const bool whole = s.last && s.kb0 == 0;
+      const int64_t slot = 2 * (int64_t)blockIdx.x + (s.kb0 == 0 ? 1 : 0);
+      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+      const int tok = row / p.group, hd = w.h * p.group + row % p.group;
+      char* dst = p.out + (int64_t)(w.r.q0 + tok) * p.ld_out + (int64_t)hd * p.kv.dim * 2;
+      float* part = p.part_o + (slot * kTR + t * 128 + r) * DP;
+      if (cnt > 0) {
+#pragma unroll 1
+        for (int i = 0; i < DP / 32; ++i) {
+          float o[32];
+          tmem_ld32(o_col + i * 32, o);
+          tmem_ld_wait();
+          pin32(o);
+          if (live && whole) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (i * 32 + k * 8 < p.kv.dim)
+                *reinterpret_cast<uint4*>(dst + (i * 32 + k * 8) * 2) =
+                    make_uint4(Num<T>::pack(o[8 * k] * inv, o[8 * k + 1] * inv),
+                               Num<T>::pack(o[8 * k + 2] * inv, o[8 * k + 3] * inv),
+                               Num<T>::pack(o[8 * k + 4] * inv, o[8 * k + 5] * inv),
+                               Num<T>::pack(o[8 * k + 6] * inv, o[8 * k + 7] * inv));
+          } else if (live) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              *reinterpret_cast<float4*>(part + i * 32 + 4 * k) =
+                  make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+          }
+          __syncwarp();
+        }
+        // the next tile's first PV, which overwrites O, waits for this warp's next arrival on p_full
+        tc_fence_before();
+      }
+      // a half without blocks in this stretch leaves an empty sum: its context is not read
+      if (!whole && live) p.part_ml[slot * kTR + t * 128 + r] = make_float2(mx, l);
+      if (!whole && threadIdx.x == 0) {
+        int4* h = &p.head[blockIdx.x];
+        if (s.kb0 == 0) {
+          h->x = w.b;
+          h->y = w.rt;
+          h->z = w.h;
+        } else {
+          h->w = s.last ? kPartEnds : kPartGoesOn;
+        }
+      }
+      left -= s.n;
+      if (left > 0) attn_next_tile<kTR, kKB>(p, w);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_trigger();
+  if (warp == kMmaWarp)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+}
+
+template <typename T, int DP>
+int run_tc(AttnParams p, void* workspace, int max_kv, int sms, cudaStream_t stream) {
+  attn_carve<kTR, DP>(p, workspace, sms);
+  auto kernel = paged_attn_tc_kernel<T, DP>;
+  SMEAI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Tc<DP>::kSmem));
+  SMEAI_CUDA_TRY(launch(kernel, dim3((unsigned)sms), dim3(kThreads), Tc<DP>::kSmem, stream, p, wait_timeout_ns()));
+  if (max_kv > 2 * kSnap * kKB) SMEAI_CUDA_TRY((attn_join<T, kTR, DP>(p, sms, stream)));
+  return kOk;
+}
+
+}  // namespace
+
+size_t paged_attn_tc_workspace(int padded_dim, int sms) {
+  return padded_dim == 64 ? attn_part_bytes<kTR, 64>(sms) : attn_part_bytes<kTR, 128>(sms);
+}
+
+int paged_attn_tc(const AttnParams& p, int padded_dim, void* workspace, int max_kv, int sms, cudaStream_t stream) {
+  if (p.kv.bf16)
+    return padded_dim == 64 ? run_tc<__nv_bfloat16, 64>(p, workspace, max_kv, sms, stream)
+                            : run_tc<__nv_bfloat16, 128>(p, workspace, max_kv, sms, stream);
+  return padded_dim == 64 ? run_tc<__half, 64>(p, workspace, max_kv, sms, stream)
+                          : run_tc<__half, 128>(p, workspace, max_kv, sms, stream);
+}
+
+}  // namespace smeai

@@ -274,6 +274,19 @@ def test_attention_chunks(cuda, dtype, causal, H, K, D, page):
     p.check(p.run(causal=causal), causal=causal)
 
 
+MANY = [(300, 300), (257, 1000), (128, 2500), (129, 129), (256, 256), (1, 70), (400, 380), (90, 0), (16, 500), (513, 900)]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("H,K,D,page", [(1, 1, 64, 16), (1, 1, 128, 16), (4, 2, 128, 1), (3, 1, 80, 32), (8, 1, 64, 128)])
+def test_attention_many_rows(cuda, dtype, causal, H, K, D, page):
+    """Tiles of 256 rows, the last one or its lower half partly filled; keys that
+    end inside a block; rows that see nothing (fewer keys than new tokens)."""
+    p = Problem(cuda, MANY, H, K, D, page, dtype, seed=12)
+    p.check(p.run(causal=causal), causal=causal)
+
+
 @pytest.mark.parametrize("H,K,D,n,m", [(4, 1, 128, 1, 20000), (1, 1, 64, 1, 50001), (32, 8, 128, 3, 3001), (2, 1, 256, 1, 9000),
                                        (8, 8, 128, 300, 2500), (2, 1, 64, 1000, 1000), (1, 1, 128, 2, 30000)])
 def test_attention_split_over_ctas(cuda, H, K, D, n, m):
