@@ -40,7 +40,6 @@ constexpr int kThreads = 512;
 constexpr int kLoadWarp0 = 8, kMmaWarp = 12;
 constexpr int kAtom = 128 * 128;     // 128 rows x 128 bytes
 constexpr int kTmemCols = 512;       // S0 S1 (128 columns each), O0 O1 (up to 128 each)
-constexpr int kLag = 2;              // copied items not yet announced
 constexpr float kRaise = 8.f;        // growth of the maximum (log2) that rescales O
 constexpr float kNegInf = -INFINITY;
 
@@ -48,7 +47,7 @@ template <int DP>
 struct Tc {
   static constexpr int kCb = DP / 64;              // 64-element column blocks
   static constexpr int kItem = kCb * kAtom;        // bytes of 128 rows
-  static constexpr int kSlots = DP == 128 ? 4 : 8; // ring of key and value blocks: 128 KB
+  static constexpr int kSlots = DP == 128 ? 5 : 8; // ring of key and value blocks: 160 or 128 KB
   static constexpr int kQBytes = 2 * kItem;
   static constexpr size_t kSmem = 1024 + (size_t)kQBytes + (size_t)kSlots * kItem + 256;
 };
@@ -56,7 +55,7 @@ struct Tc {
 struct TcSmem {
   uint8_t* q;
   uint8_t* ring;
-  uint64_t *full, *empty;            // per slot: 4 load warps; one commit
+  uint64_t *full, *empty;            // per slot: the 128 load threads' copies; one commit
   uint64_t* q_empty;                 // commit: the tile's last QK has read the queries
   uint64_t *s_full, *p_full, *o_full;  // per half: commit; 4 warps; commit
   uint64_t* drain;
@@ -146,6 +145,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* v) {
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// Arrives on `bar` when this thread's cp.async copies so far have landed (the
+// barrier's count includes this arrival).
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
 // Keeps uses of a load's registers behind the wait before it.
 __device__ __forceinline__ void pin32(float* v) {
   asm volatile(""
@@ -201,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 8; ++i) {
-      mbar_init(&m.full[i], 4);
+      mbar_init(&m.full[i], 128);
       mbar_init(&m.empty[i], 1);
     }
     mbar_init(m.q_empty, 1);
@@ -239,25 +243,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
     attn_open<kTR, kKB>(p, share, w);
     const int page_mask = (1 << p.kv.page_log2) - 1;
     int64_t left = units;
-    int it = 0, told = 0;          // items copied, items announced
+    int it = 0;                    // items copied
     int tiles = 0;
     bool ok = true;
-    // announce the items whose copies have landed (all but the newest `keep`)
-    auto tell = [&](int keep) {
-      fence_async_smem();
-      __syncwarp();
-      for (; told < it - keep; ++told)
-        if (lane == 0) mbar_arrive(&m.full[told % C::kSlots]);
-    };
-    // a free slot for item `it`; what is in flight is announced before a long wait
     auto acquire = [&]() {
-      if (it < C::kSlots) return true;
-      uint64_t* bar = &m.empty[it % C::kSlots];
-      const unsigned parity = (unsigned)((it / C::kSlots - 1) & 1);
-      if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-      cp_async_wait<0>();
-      tell(0);
-      return wait_warp(m, bar, parity, p.err, limit_ns);
+      return it < C::kSlots ||
+             wait_warp(m, &m.empty[it % C::kSlots], (unsigned)((it / C::kSlots - 1) & 1), p.err, limit_ns);
     };
     constexpr int kChunks = DP / 8;
     constexpr int kPer = 32 * kChunks / 32;      // chunks a lane copies of an item
@@ -290,17 +281,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
         const int64_t next = b + 1 < s.n ? look_up(s.kb0 + b + 1) : -1;
         if (!(ok = acquire())) break;
         if (b == 0) {
-          // the tile's queries, announced with its first keys; their place is free
-          // once the previous tile's last keys, copied but perhaps not yet
-          // announced, have been read
-          if (tiles > 0) {
-            const unsigned parity = (unsigned)((tiles - 1) & 1);
-            if (!__all_sync(0xffffffffu, mbar_try_wait(m.q_empty, parity))) {
-              cp_async_wait<0>();
-              tell(0);
-              if (!(ok = wait_warp(m, m.q_empty, parity, p.err, limit_ns))) break;
-            }
-          }
+          // the tile's queries land with its first keys
+          if (tiles > 0 && !(ok = wait_warp(m, m.q_empty, (unsigned)((tiles - 1) & 1), p.err, limit_ns))) break;
 #pragma unroll
           for (int q4 = 0; q4 < 2; ++q4) {
             const int r = lw * 64 + q4 * 32 + lane, row = w.rt * kTR + r;
@@ -313,24 +295,20 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
           }
         }
         copy_rows(m.ring + (size_t)(it % C::kSlots) * C::kItem, p.kv.k, off, lw * 32);
-        cp_async_commit();
+        cp_async_arrive(&m.full[it % C::kSlots]);
         ++it;
-        cp_async_wait<kLag>();
-        tell(kLag);
         if (!(ok = acquire())) break;
         copy_rows(m.ring + (size_t)(it % C::kSlots) * C::kItem, p.kv.v, off, lw * 32);
-        cp_async_commit();
+        cp_async_arrive(&m.full[it % C::kSlots]);
         ++it;
-        cp_async_wait<kLag>();
-        tell(kLag);
         off = next;
       }
       left -= s.n;
       ++tiles;
       if (left > 0) attn_next_tile<kTR, kKB>(p, w);
     }
+    cp_async_commit();
     cp_async_wait<0>();
-    tell(0);
   } else if (warp >= kMmaWarp) {
     // ---------------- issue the MMAs
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
@@ -366,6 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
       while (left > 0 && ok) {
         const Stretch s = stretch(p, w, left);
         if (!(ok = full(it))) break;
+        fence_async_smem();      // the copies are ordinary writes; the MMA reads through the async proxy
         tc_fence_after();
         for (int t = 0; t < 2; ++t)
           if (s.cnt[t] > 0) {
@@ -378,6 +357,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
           const int iv = it + 2 * b + 1, ik = iv + 1;
           const bool more = b + 1 < s.n;
           if (!(ok = full(iv) && (!more || full(ik)))) break;
+          fence_async_smem();
           for (int t = 0; t < 2; ++t) {
             if (b >= s.cnt[t]) continue;
             if (!(ok = wait_or_abort(m, &m.p_full[t], pc[t] & 1, p.err, limit_ns))) break;
