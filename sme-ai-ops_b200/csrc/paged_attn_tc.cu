@@ -103,6 +103,13 @@ __device__ __forceinline__ bool wait_warp(const TcSmem& m, uint64_t* bar, unsign
   return __all_sync(0xffffffffu, wait_or_abort(m, bar, parity, err, limit_ns));
 }
 
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+  return e != 0;
+}
+
 // D[tmem] (+)= A[tmem] * B[smem desc]^T, 16-bit inputs, fp32 accumulate.
 __device__ __forceinline__ void tc_mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
                                               uint32_t accumulate) {
@@ -311,77 +318,99 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
     cp_async_wait<0>();
   } else if (warp >= kMmaWarp) {
     // ---------------- issue the MMAs
+    // The whole warp walks and waits, so that descriptors stay in uniform
+    // registers; one elected lane issues.
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    if (warp == kMmaWarp && lane == 0) {
+    if (warp == kMmaWarp) {
       constexpr uint32_t kQk = idesc(IsBf16<T>::value, kKB, false), kPv = idesc(IsBf16<T>::value, DP, true);
       AttnPos w;
       attn_open<kTR, kKB>(p, share, w);
       int64_t left = units;
-      int it = 0;
-      unsigned pc[2] = {0, 0};
+      int slot = 0;                // of the next item
+      unsigned round = 0;          // parity of the ring's current round
+      unsigned pc0 = 0, pc1 = 0;   // softmax results taken, per half
       bool ok = true;
-      auto qk = [&](int t, int item) {
-        const uint8_t* kb = m.ring + (size_t)(item % C::kSlots) * C::kItem;
-        const uint64_t a0 = smem_desc(m.q + t * C::kItem, 16, 1024, kLayoutSw128);
-        const uint64_t b0 = smem_desc(kb, 16, 1024, kLayoutSw128);
+      const uint64_t q_desc = smem_desc(m.q, 16, 1024, kLayoutSw128);
+      const uint64_t k_desc = smem_desc(m.ring, 16, 1024, kLayoutSw128);
+      const uint64_t v_desc = smem_desc(m.ring, kAtom, 1024, kLayoutSw128);
+      auto qk = [&](int t, int at) {
+        if (elect_one()) {
+          const uint64_t a0 = q_desc + (uint64_t)t * (C::kItem >> 4), b0 = k_desc + (uint64_t)at * (C::kItem >> 4);
 #pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) {
-          const uint64_t step = (uint64_t)(((ks >> 2) * kAtom + (ks & 3) * 32) >> 4);
-          tc_mma_f16(tmem + t * 128, a0 + step, b0 + step, kQk, ks > 0);
+          for (int ks = 0; ks < DP / 16; ++ks) {
+            const uint64_t step = (uint64_t)(((ks >> 2) * kAtom + (ks & 3) * 32) >> 4);
+            tc_mma_f16(tmem + t * 128, a0 + step, b0 + step, kQk, ks > 0);
+          }
+          tc_commit(&m.s_full[t]);
         }
+        __syncwarp();
       };
-      auto pv = [&](int t, int item, bool first) {
-        const uint8_t* vb = m.ring + (size_t)(item % C::kSlots) * C::kItem;
-        const uint64_t b0 = smem_desc(vb, kAtom, 1024, kLayoutSw128);
+      auto pv = [&](int t, int at, bool first) {
+        if (elect_one()) {
+          const uint64_t b0 = v_desc + (uint64_t)at * (C::kItem >> 4);
 #pragma unroll
-        for (int ks = 0; ks < kKB / 16; ++ks)
-          tc_mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + ks * 8, b0 + (uint64_t)((ks * 2048) >> 4), kPv,
-                        !(first && ks == 0));
+          for (int ks = 0; ks < kKB / 16; ++ks)
+            tc_mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + ks * 8, b0 + (uint64_t)((ks * 2048) >> 4), kPv,
+                          !(first && ks == 0));
+        }
+        __syncwarp();
       };
-      auto full = [&](int item) {
-        return wait_or_abort(m, &m.full[item % C::kSlots], (unsigned)((item / C::kSlots) & 1), p.err, limit_ns);
+      auto commit = [&](uint64_t* bar) {
+        if (elect_one()) tc_commit(bar);
+        __syncwarp();
       };
-      while (left > 0 && ok) {
+      // the next item of the ring, landed; -1 when the wait gave up
+      auto take = [&]() {
+        const int at = slot;
+        ok = wait_warp(m, &m.full[at], round, p.err, limit_ns);
+        if (++slot == C::kSlots) {
+          slot = 0;
+          round ^= 1;
+        }
+        return at;
+      };
+      while (left > 0) {
         const Stretch s = stretch(p, w, left);
-        if (!(ok = full(it))) break;
+        const int k0 = take();
+        if (!ok) break;
         fence_async_smem();      // the copies are ordinary writes; the MMA reads through the async proxy
         tc_fence_after();
-        for (int t = 0; t < 2; ++t)
-          if (s.cnt[t] > 0) {
-            qk(t, it);
-            tc_commit(&m.s_full[t]);
-          }
-        tc_commit(&m.empty[it % C::kSlots]);
-        if (s.n == 1) tc_commit(m.q_empty);
-        for (int b = 0; b < s.n && ok; ++b) {
-          const int iv = it + 2 * b + 1, ik = iv + 1;
+        if (s.cnt[0] > 0) qk(0, k0);
+        if (s.cnt[1] > 0) qk(1, k0);
+        commit(&m.empty[k0]);
+        if (s.n == 1) commit(m.q_empty);
+        for (int b = 0; b < s.n; ++b) {
+          const int iv = take();
+          if (!ok) break;
           const bool more = b + 1 < s.n;
-          if (!(ok = full(iv) && (!more || full(ik)))) break;
+          int ik = 0;
+          if (more) {
+            ik = take();
+            if (!ok) break;
+          }
           fence_async_smem();
+#pragma unroll
           for (int t = 0; t < 2; ++t) {
             if (b >= s.cnt[t]) continue;
-            if (!(ok = wait_or_abort(m, &m.p_full[t], pc[t] & 1, p.err, limit_ns))) break;
-            ++pc[t];
+            unsigned& pc = t ? pc1 : pc0;
+            if (!(ok = wait_warp(m, &m.p_full[t], pc & 1, p.err, limit_ns))) break;
+            ++pc;
             tc_fence_after();
             pv(t, iv, b == 0);
-            if (b + 1 < s.cnt[t]) {
-              qk(t, ik);
-              tc_commit(&m.s_full[t]);
-            } else {
-              tc_commit(&m.o_full[t]);
-            }
+            if (b + 1 < s.cnt[t]) qk(t, ik);
+            else commit(&m.o_full[t]);
           }
           if (!ok) break;
-          tc_commit(&m.empty[iv % C::kSlots]);
-          if (more) tc_commit(&m.empty[ik % C::kSlots]);
-          if (b + 2 == s.n) tc_commit(m.q_empty);
+          commit(&m.empty[iv]);
+          if (more) commit(&m.empty[ik]);
+          if (b + 2 == s.n) commit(m.q_empty);
         }
-        it += 2 * s.n;
+        if (!ok) break;
         left -= s.n;
         if (left > 0) attn_next_tile<kTR, kKB>(p, w);
       }
       // everything issued has finished before TMEM is freed
-      tc_commit(m.drain);
+      commit(m.drain);
       mbar_wait_bounded(m.drain, 0, limit_ns);
     }
     __syncwarp();
