@@ -257,18 +257,29 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
       return it < C::kSlots ||
              wait_warp(m, &m.empty[it % C::kSlots], (unsigned)((it / C::kSlots - 1) & 1), p.err, limit_ns);
     };
-    constexpr int kChunks = DP / 8;
-    constexpr int kPer = 32 * kChunks / 32;      // chunks a lane copies of an item
-    auto copy_rows = [&](uint8_t* dst, const char* src, int64_t off, int row0) {
-#pragma unroll 4
-      for (int i = 0; i < kPer; ++i) {
-        const int c = i * 32 + lane, row = c / kChunks, col = c % kChunks;
-        const int64_t o = __shfl_sync(0xffffffffu, off, row);
-        const int n = o >= 0 && col * 8 < p.kv.dim ? 16 : 0;
-        const int r = row0 + row;
-        cp_async16(smem_addr(dst) + (col >> 3) * kAtom + r * 128 + (((col & 7) ^ (r & 7)) << 4),
-                   src + (n ? o + col * 16 : 0), n);
-      }
+    // A warp copies 32 rows, 4 at a time: 8 lanes take 128 contiguous bytes of
+    // a row.  Row i * 4 + sub of the 32 lands in atom row row0 + that row, its
+    // 16-byte chunks XORed with the row mod 8 -- which is sub, or sub + 4 for odd i.
+    const int sub = lane >> 3, col = lane & 7;
+    const uint32_t even = (uint32_t)(sub * 128 + ((col ^ sub) << 4)), odd = (uint32_t)(sub * 128 + ((col ^ (sub + 4)) << 4));
+    int bytes[C::kCb];                             // 0 past the head's elements
+#pragma unroll
+    for (int cb = 0; cb < C::kCb; ++cb) bytes[cb] = cb * 64 + col * 8 < p.kv.dim ? 16 : 0;
+    // the lanes' own row offsets (-1: zeros) -> those of the rows this lane helps to copy
+    auto spread = [&](int64_t off, int64_t (&o)[8]) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = __shfl_sync(0xffffffffu, off, i * 4 + sub);
+    };
+    auto copy_rows = [&](uint8_t* dst, const char* src, const int64_t (&o)[8], int row0) {
+      const uint32_t d = smem_addr(dst) + row0 * 128;
+      const char* from = src + col * 16;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int cb = 0; cb < C::kCb; ++cb) {
+          const int n = o[i] >= 0 ? bytes[cb] : 0;
+          cp_async16(d + i * 512 + cb * kAtom + (i & 1 ? odd : even), n ? from + o[i] + cb * 128 : src, n);
+        }
     };
     while (left > 0 && ok) {
       const Stretch s = stretch(p, w, left);
@@ -298,14 +309,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
               const int tok = row / p.group, hd = w.h * p.group + row % p.group;
               qoff = (int64_t)(w.r.q0 + tok) * p.ld_q + (int64_t)hd * p.kv.dim * 2;
             }
-            copy_rows(m.q + (lw >> 1) * C::kItem, p.q, qoff, (lw & 1) * 64 + q4 * 32);
+            int64_t qo[8];
+            spread(qoff, qo);
+            copy_rows(m.q + (lw >> 1) * C::kItem, p.q, qo, (lw & 1) * 64 + q4 * 32);
           }
         }
-        copy_rows(m.ring + (size_t)(it % C::kSlots) * C::kItem, p.kv.k, off, lw * 32);
+        int64_t o[8];
+        spread(off, o);
+        copy_rows(m.ring + (size_t)(it % C::kSlots) * C::kItem, p.kv.k, o, lw * 32);
         cp_async_arrive(&m.full[it % C::kSlots]);
         ++it;
         if (!(ok = acquire())) break;
-        copy_rows(m.ring + (size_t)(it % C::kSlots) * C::kItem, p.kv.v, off, lw * 32);
+        copy_rows(m.ring + (size_t)(it % C::kSlots) * C::kItem, p.kv.v, o, lw * 32);
         cp_async_arrive(&m.full[it % C::kSlots]);
         ++it;
         off = next;
@@ -449,10 +464,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
           for (int i = 0; i < 128; ++i)
             if (key0 + i >= lim) v[i] = kNegInf;
         }
-        float top[4] = {v[0], v[1], v[2], v[3]};
+        float top[8];
 #pragma unroll
-        for (int i = 4; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], v[i]);
-        const float mn = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
+        for (int i = 0; i < 8; ++i) top[i] = v[i];
+#pragma unroll
+        for (int i = 8; i < 120; i += 16)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) top[k] = fmaxf(fmaxf(top[k], v[i + k]), v[i + 8 + k]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) top[k] = fmaxf(top[k], v[120 + k]);
+        const float mn = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])),
+                               fmaxf(fmaxf(top[4], top[5]), fmaxf(top[6], top[7]))) * p.scale_log2;
         const bool raise = mn > mx + kRaise || (mx == kNegInf && mn > mx);
         if (__any_sync(0xffffffffu, raise)) {
           const float f = raise ? exp2_fast(mx - mn) : 1.f;
