@@ -12,12 +12,15 @@
 // stays below 2^8, or 2^15 with half's bias), so O, which has to be rescaled
 // when it is, is touched rarely; the thread that owns the row does it.
 //
-// Warp roles (16 warps, one CTA an SM):
-//   warps 0-3, 4-7   softmax of half 0 and half 1 (192 registers a thread)
-//   warps 8-11       load: queries, keys and values with 16-byte cp.async into
-//                    the 128-byte-swizzled layout the MMA reads; rows may lie
-//                    anywhere, so any page size and stride costs the same
-//   warp 12          allocates TMEM; one lane issues the MMAs
+// Warp roles (12 warps, one CTA an SM):
+//   warps 0-3, 4-7   softmax of half 0 and half 1 (208 registers a thread)
+//   warps 8-9        load: keys and values a page (or 64 rows of one) at a time
+//                    by TMA into the 128-byte-swizzled layout the MMA reads;
+//                    queries, values of a block that the request ends in (whose
+//                    other rows must be zeros, not what the page held before),
+//                    and everything when pages are smaller than 8 tokens with
+//                    16-byte cp.async
+//   warp 10          allocates TMEM; one lane issues the MMAs
 // While one half's softmax runs, the tensor core works for the other: in issue
 // order PV_0(j), QK_0(j+1), PV_1(j), QK_1(j+1).  At 128 elements a block
 // takes 4 x 128^3 multiply-adds for the tensor core (2048 cycles at its rate)
@@ -27,6 +30,11 @@
 // Every wait is bounded by wall time; on expiry the kernel records
 // kDevErrTimeout, all roles stop, copies and MMAs in flight are drained, TMEM
 // is freed and the kernel returns.  No multicast.
+#include <cuda.h>
+#include <string.h>
+
+#include <atomic>
+
 #include "paged_attn.cuh"
 #include "tcgen05.cuh"
 
@@ -36,8 +44,10 @@ namespace {
 
 constexpr int kTR = 256;             // packed rows a tile
 constexpr int kKB = 128;             // keys a block
-constexpr int kThreads = 512;
-constexpr int kLoadWarp0 = 8, kMmaWarp = 12;
+constexpr int kThreads = 384;
+constexpr int kLoadWarp0 = 8, kLoadWarps = 2, kMmaWarp = 10;
+constexpr int kTmaMinPage = 8;       // tokens
+// 384 threads x 168 registers at launch = 256 x 208 + 128 x 88
 constexpr int kAtom = 128 * 128;     // 128 rows x 128 bytes
 constexpr int kTmemCols = 512;       // S0 S1 (128 columns each), O0 O1 (up to 128 each)
 constexpr float kRaise = 8.f;        // growth of the maximum (log2) that rescales O
@@ -55,7 +65,7 @@ struct Tc {
 struct TcSmem {
   uint8_t* q;
   uint8_t* ring;
-  uint64_t *full, *empty;            // per slot: the 128 load threads' copies; one commit
+  uint64_t *full, *empty;            // per slot: both load warps (their threads, without TMA); one commit
   uint64_t* q_empty;                 // commit: the tile's last QK has read the queries
   uint64_t *s_full, *p_full, *o_full;  // per half: commit; 4 warps; commit
   uint64_t* drain;
@@ -202,8 +212,28 @@ __device__ __forceinline__ Stretch stretch(const AttnParams& p, const AttnPos& w
   return s;
 }
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnParams p, uint64_t limit_ns) {
+// A TMA load of box rows x 64 elements at (element, token, head, page).
+__device__ __forceinline__ void tma_load_box(uint32_t dst, const CUtensorMap* map, int x, int token, int head, int page,
+                                             uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(token), "r"(head), "r"(page), "r"(smem_addr(bar))
+      : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, unsigned bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
+}
+
+// The cache as the TMA sees it; box_log2: log2 of the rows of a box.
+struct TcMaps {
+  CUtensorMap k, v;
+  int box_log2;
+};
+
+template <typename T, int DP, bool kTma>
+__global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnParams p, const __grid_constant__ TcMaps maps,
+                                                                    uint64_t limit_ns) {
   using C = Tc<DP>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ AttnShare share;
@@ -212,7 +242,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 8; ++i) {
-      mbar_init(&m.full[i], 128);
+      mbar_init(&m.full[i], kTma ? kLoadWarps : 32 * kLoadWarps);
       mbar_init(&m.empty[i], 1);
     }
     mbar_init(m.q_empty, 1);
@@ -242,100 +272,159 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
 
   if (units <= 0) {
     // nothing to do
-  } else if (warp >= kLoadWarp0 && warp < kLoadWarp0 + 4) {
-    // ---------------- load
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+  } else if (warp >= kLoadWarp0 && warp < kLoadWarp0 + kLoadWarps) {
+    // ---------------- load: this warp's 64 rows of every item
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     const int lw = warp - kLoadWarp0;
     AttnPos w;
     attn_open<kTR, kKB>(p, share, w);
     const int page_mask = (1 << p.kv.page_log2) - 1;
     int64_t left = units;
-    int it = 0;                    // items copied
-    int tiles = 0;
+    int slot = 0;                  // of the next item
+    unsigned round = 1;            // parity of the wait for its being free
+    int64_t items = 0;             // announced
     bool ok = true;
-    auto acquire = [&]() {
-      return it < C::kSlots ||
-             wait_warp(m, &m.empty[it % C::kSlots], (unsigned)((it / C::kSlots - 1) & 1), p.err, limit_ns);
-    };
-    // A warp copies 32 rows, 4 at a time: 8 lanes take 128 contiguous bytes of
-    // a row.  Row i * 4 + sub of the 32 lands in atom row row0 + that row, its
-    // 16-byte chunks XORed with the row mod 8 -- which is sub, or sub + 4 for odd i.
+    unsigned q_round = 1;          // parity of the wait for the queries' place
+    // cp.async: 4 rows at a time, 8 lanes take 128 contiguous bytes of a row.
+    // Row i * 4 + sub of 32 lands in atom row row0 + that row, its 16-byte
+    // chunks XORed with the row mod 8 -- which is sub, or sub + 4 for odd i.
     const int sub = lane >> 3, col = lane & 7;
     const uint32_t even = (uint32_t)(sub * 128 + ((col ^ sub) << 4)), odd = (uint32_t)(sub * 128 + ((col ^ (sub + 4)) << 4));
     int bytes[C::kCb];                             // 0 past the head's elements
 #pragma unroll
     for (int cb = 0; cb < C::kCb; ++cb) bytes[cb] = cb * 64 + col * 8 < p.kv.dim ? 16 : 0;
-    // the lanes' own row offsets (-1: zeros) -> those of the rows this lane helps to copy
-    auto spread = [&](int64_t off, int64_t (&o)[8]) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = __shfl_sync(0xffffffffu, off, i * 4 + sub);
-    };
-    auto copy_rows = [&](uint8_t* dst, const char* src, const int64_t (&o)[8], int row0) {
+    // off: byte offset of row row0 + lane, -1: zeros
+    auto copy_rows = [&](uint8_t* dst, const char* src, int64_t off, int row0) {
       const uint32_t d = smem_addr(dst) + row0 * 128;
       const char* from = src + col * 16;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < 8; ++i) {
+        const int64_t o = __shfl_sync(0xffffffffu, off, i * 4 + sub);
 #pragma unroll
         for (int cb = 0; cb < C::kCb; ++cb) {
-          const int n = o[i] >= 0 ? bytes[cb] : 0;
-          cp_async16(d + i * 512 + cb * kAtom + (i & 1 ? odd : even), n ? from + o[i] + cb * 128 : src, n);
+          const int n = o >= 0 ? bytes[cb] : 0;
+          cp_async16(d + i * 512 + cb * kAtom + (i & 1 ? odd : even), n ? from + o + cb * 128 : src, n);
         }
+      }
     };
+    auto acquire = [&]() {   // the first round over the ring finds it free
+      return wait_warp(m, &m.empty[slot], round, p.err, limit_ns);
+    };
+    auto next_slot = [&]() {
+      ++items;
+      if (++slot == C::kSlots) {
+        slot = 0;
+        round ^= 1;
+      }
+    };
+    // copies of this warp so far have landed: announce them
+    auto landed = [&]() {
+      cp_async_commit();
+      cp_async_wait<0>();
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&m.full[slot]);
+    };
+    const int box_rows = 1 << maps.box_log2, boxes = 64 >> maps.box_log2;
+    const int my_box = lane / C::kCb, my_cb = lane % C::kCb;
     while (left > 0 && ok) {
       const Stretch s = stretch(p, w, left);
       const int32_t* table = p.table + (int64_t)w.b * p.ld_table;
-      auto look_up = [&](int kb) {   // byte offset of this lane's key row; -1: zeros
-        const int key = kb * kKB + lw * 32 + lane;
-        if (key >= w.r.kv) return (int64_t)-1;
+      auto page_of = [&](int key) {   // -1: no such key, or a bad page
+        if (key >= w.r.kv) return -1;
         const int page = table[key >> p.kv.page_log2];
-        if (page < 0 || page >= p.kv.n_pages) {
-          raise_device_error(p.err, kDevErrBadIndex);
-          return (int64_t)-1;
-        }
-        return page * p.kv.page_bytes + (key & page_mask) * p.kv.token_bytes + w.h * p.kv.head_bytes;
+        if (page >= 0 && page < p.kv.n_pages) return page;
+        raise_device_error(p.err, kDevErrBadIndex);
+        return -1;
       };
-      int64_t off = look_up(s.kb0);
+      auto row_off = [&](int key) {
+        const int page = page_of(key);
+        return page < 0 ? (int64_t)-1
+                        : page * p.kv.page_bytes + (key & page_mask) * p.kv.token_bytes + w.h * p.kv.head_bytes;
+      };
+      auto copy_item = [&](const char* src, int key0) {
+        uint8_t* dst = m.ring + (size_t)slot * C::kItem;
+        copy_rows(dst, src, row_off(key0 + lane), lw * 64);
+        copy_rows(dst, src, row_off(key0 + 32 + lane), lw * 64 + 32);
+      };
+      // this lane's box of a TMA item: its first key's page, -1 when it has none
+      const bool has_box = kTma && my_box < boxes;
+      int page = has_box ? page_of(s.kb0 * kKB + lw * 64 + my_box * box_rows) : -1;
+      auto load_item = [&](const CUtensorMap* map, int key0) {
+        const unsigned n = __popc(__ballot_sync(0xffffffffu, page >= 0));
+        if (lane == 0) mbar_expect_tx(&m.full[slot], n * box_rows * 128);
+        __syncwarp();
+        if (page >= 0) {
+          const int row = my_box * box_rows;
+          tma_load_box(smem_addr(m.ring) + slot * C::kItem + my_cb * kAtom + (lw * 64 + row) * 128, map, my_cb * 64,
+                       (key0 + row) & page_mask, w.h, page, &m.full[slot]);
+        }
+      };
       for (int b = 0; b < s.n && ok; ++b) {
-        const int64_t next = b + 1 < s.n ? look_up(s.kb0 + b + 1) : -1;
+        const int key0 = (s.kb0 + b) * kKB + lw * 64;
+        // the next block's pages are looked up before this block's waits
+        const int next_page = has_box && b + 1 < s.n ? page_of(key0 + kKB + my_box * box_rows) : -1;
         if (!(ok = acquire())) break;
+        if (kTma) load_item(&maps.k, key0);
         if (b == 0) {
-          // the tile's queries land with its first keys
-          if (tiles > 0 && !(ok = wait_warp(m, m.q_empty, (unsigned)((tiles - 1) & 1), p.err, limit_ns))) break;
+          // the tile's queries land with its first keys, once the last tile's are read
+          if (!(ok = wait_warp(m, m.q_empty, q_round, p.err, limit_ns))) {
+            if (lane == 0) mbar_arrive(&m.full[slot]);
+            ++items;
+            break;
+          }
+          q_round ^= 1;
 #pragma unroll
-          for (int q4 = 0; q4 < 2; ++q4) {
-            const int r = lw * 64 + q4 * 32 + lane, row = w.rt * kTR + r;
-            int64_t qoff = -1;
+          for (int q4 = 0; q4 < 4; ++q4) {
+            const int row = w.rt * kTR + lw * 128 + q4 * 32 + lane;
+            int64_t off = -1;
             if (row < w.r.rows) {
               const int tok = row / p.group, hd = w.h * p.group + row % p.group;
-              qoff = (int64_t)(w.r.q0 + tok) * p.ld_q + (int64_t)hd * p.kv.dim * 2;
+              off = (int64_t)(w.r.q0 + tok) * p.ld_q + (int64_t)hd * p.kv.dim * 2;
             }
-            int64_t qo[8];
-            spread(qoff, qo);
-            copy_rows(m.q + (lw >> 1) * C::kItem, p.q, qo, (lw & 1) * 64 + q4 * 32);
+            copy_rows(m.q + lw * C::kItem, p.q, off, q4 * 32);
           }
         }
-        int64_t o[8];
-        spread(off, o);
-        copy_rows(m.ring + (size_t)(it % C::kSlots) * C::kItem, p.kv.k, o, lw * 32);
-        cp_async_arrive(&m.full[it % C::kSlots]);
-        ++it;
+        if (!kTma) {
+          copy_item(p.kv.k, key0);
+          cp_async_arrive(&m.full[slot]);
+        } else if (b == 0) {
+          landed();
+        } else if (lane == 0) {
+          mbar_arrive(&m.full[slot]);
+        }
+        next_slot();
         if (!(ok = acquire())) break;
-        copy_rows(m.ring + (size_t)(it % C::kSlots) * C::kItem, p.kv.v, o, lw * 32);
-        cp_async_arrive(&m.full[it % C::kSlots]);
-        ++it;
-        off = next;
+        if (!kTma) {
+          copy_item(p.kv.v, key0);
+          cp_async_arrive(&m.full[slot]);
+        } else if ((s.kb0 + b + 1) * kKB > w.r.kv) {
+          copy_item(p.kv.v, key0);
+          landed();
+        } else {
+          load_item(&maps.v, key0);
+          if (lane == 0) mbar_arrive(&m.full[slot]);
+        }
+        next_slot();
+        page = next_page;
       }
       left -= s.n;
-      ++tiles;
       if (left > 0) attn_next_tile<kTR, kKB>(p, w);
     }
     cp_async_commit();
     cp_async_wait<0>();
+    if (kTma && !ok) {
+      // gave up: TMA loads in flight still write this CTA's shared memory; their
+      // bytes complete the phases they were announced on (a phase that the
+      // other load warp never joined costs the whole millisecond)
+      for (int64_t i = items > C::kSlots ? items - C::kSlots : 0; i < items; ++i)
+        mbar_wait_bounded(&m.full[i % C::kSlots], (unsigned)((i / C::kSlots) & 1), 1000000);
+    }
   } else if (warp >= kMmaWarp) {
     // ---------------- issue the MMAs
     // The whole warp walks and waits, so that descriptors stay in uniform
     // registers; one elected lane issues.
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp == kMmaWarp) {
       constexpr uint32_t kQk = idesc(IsBf16<T>::value, kKB, false), kPv = idesc(IsBf16<T>::value, DP, true);
       AttnPos w;
@@ -431,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
     __syncwarp();
   } else {
     // ---------------- softmax of half t, one row a thread
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int t = warp >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_col = tmem + lanes + t * 128, o_col = tmem + lanes + 256 + t * 128;
@@ -578,12 +667,61 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
 
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled() {
+  static std::atomic<void*> cached{nullptr};
+  void* fn = cached.load();
+  if (!fn) {
+    cudaDriverEntryPointQueryResult res;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &res) != cudaSuccess ||
+        res != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
+      return nullptr;
+    }
+    cached.store(fn);
+  }
+  return reinterpret_cast<EncodeTiled>(fn);
+}
+
+// Boxes of 64 elements x up to 64 tokens of one head and page.  Elements past
+// head_dim read as zeros.  Strides of dimensions of one element are never
+// used, but have to be valid.
+bool cache_map(const KvView& kv, const void* base, int box_rows, CUtensorMap* map) {
+  const EncodeTiled encode = encode_tiled();
+  if (!encode) return false;
+  const cuuint64_t page = (cuuint64_t)1 << kv.page_log2;
+  const cuuint64_t dims[4] = {(cuuint64_t)kv.dim, page, (cuuint64_t)kv.n_kv, (cuuint64_t)kv.n_pages};
+  const cuuint64_t fill = (cuuint64_t)kv.token_bytes;
+  const cuuint64_t strides[3] = {fill, kv.n_kv > 1 ? (cuuint64_t)kv.head_bytes : fill,
+                                 kv.n_pages > 1 ? (cuuint64_t)kv.page_bytes : fill};
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, step[4] = {1, 1, 1, 1};
+  return encode(map, kv.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int DP, bool kTma>
+int run_kernel(const AttnParams& p, const TcMaps& maps, int sms, cudaStream_t stream) {
+  auto kernel = paged_attn_tc_kernel<T, DP, kTma>;
+  SMEAI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Tc<DP>::kSmem));
+  SMEAI_CUDA_TRY(launch(kernel, dim3((unsigned)sms), dim3(kThreads), Tc<DP>::kSmem, stream, p, maps, wait_timeout_ns()));
+  return kOk;
+}
+
 template <typename T, int DP>
 int run_tc(AttnParams p, void* workspace, int max_kv, int sms, cudaStream_t stream) {
   attn_carve<kTR, DP>(p, workspace, sms);
-  auto kernel = paged_attn_tc_kernel<T, DP>;
-  SMEAI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Tc<DP>::kSmem));
-  SMEAI_CUDA_TRY(launch(kernel, dim3((unsigned)sms), dim3(kThreads), Tc<DP>::kSmem, stream, p, wait_timeout_ns()));
+  TcMaps maps;
+  memset(&maps, 0, sizeof(maps));
+  maps.box_log2 = p.kv.page_log2 < 6 ? p.kv.page_log2 : 6;
+  const bool tma = (1 << p.kv.page_log2) >= kTmaMinPage && cache_map(p.kv, p.kv.k, 1 << maps.box_log2, &maps.k) &&
+                   cache_map(p.kv, p.kv.v, 1 << maps.box_log2, &maps.v);
+  const int st = tma ? run_kernel<T, DP, true>(p, maps, sms, stream) : run_kernel<T, DP, false>(p, maps, sms, stream);
+  if (st) return st;
   if (max_kv > 2 * kSnap * kKB) SMEAI_CUDA_TRY((attn_join<T, kTR, DP>(p, sms, stream)));
   return kOk;
 }
