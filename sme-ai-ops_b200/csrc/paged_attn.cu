@@ -91,6 +91,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_kernel
   constexpr bool kQRegs = DP <= 128;             // query fragments live in registers
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ AttnShare share;
+  __shared__ int64_t warp_sum[kWarps];
   __shared__ float merge_m[kWarps][16], merge_l[kWarps][16];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t ring = smem_addr(smem);
@@ -98,7 +99,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_kernel
   const uint32_t q_smem = smem_addr(merge);      // row-split, DP 256: the query tile instead
 
   pdl_wait();
-  attn_share<TR, kKeys, kThreads>(p, &share);
+  attn_share<TR, kKeys, kThreads>(p, &share, warp_sum);
   const int64_t u0 = share.u0, u1 = share.u1;
   if (threadIdx.x == 0) p.head[blockIdx.x] = make_int4(-1, 0, 0, kPartNone);
   if (u1 <= u0) return;

@@ -110,11 +110,10 @@ struct AttnShare {
 };
 
 // This CTA's piece of the line.  All threads of the block call it; the place
-// is in shared memory on return.  Each thread sums the units of its own run of
+// is in shared memory on return.  warp_sum: [NT / 32] in shared memory.  Each thread sums the units of its own run of
 // requests; the one whose run holds an end of the piece walks to it.
 template <int TR, int KB, int NT>
-__device__ void attn_share(const AttnParams& p, AttnShare* s) {
-  __shared__ int64_t warp_sum[NT / 32];
+__device__ void attn_share(const AttnParams& p, AttnShare* s, int64_t* warp_sum) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int per = (p.n_req + NT - 1) / NT;
   const int b0 = min((int)threadIdx.x * per, p.n_req), b1 = min(b0 + per, p.n_req);

@@ -237,6 +237,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
   using C = Tc<DP>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ AttnShare share;
+  __shared__ int64_t warp_sum[kThreads / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const TcSmem m = carve<DP>(smem_raw);
 
@@ -262,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   pdl_wait();
-  attn_share<kTR, kKB, kThreads>(p, &share);
+  attn_share<kTR, kKB, kThreads>(p, &share, warp_sum);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
