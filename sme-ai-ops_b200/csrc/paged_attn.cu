@@ -58,10 +58,10 @@ struct Shape {
   static constexpr int kStages = DP == 64 ? 6 : 3;      // 96 KB in flight (192 KB at DP 256)
   static constexpr int kPerSm = DP == 256 ? 1 : 2;      // CTAs an SM
 };
-template <int DP, bool kRowSplit>
+template <int DP, int MT>
 constexpr size_t smem_bytes() {
   using S = Shape<DP>;
-  return (size_t)S::kStages * 2 * S::kTileBytes + (kRowSplit ? 64 * DP * 2 : 16 * DP * 4);
+  return (size_t)S::kStages * 2 * S::kTileBytes + (MT == 0 ? 64 * DP * 2 : 2 * 16 * DP * 4);
 }
 
 template <int DP>
@@ -69,26 +69,30 @@ __device__ __forceinline__ uint32_t chunk_addr(uint32_t base, int row, int chunk
   return base + row * Shape<DP>::kRowBytes + ((chunk ^ (row & 7)) << 4);
 }
 
-// kRowSplit false: tiles of 16 rows (a decode step's query heads of one key
-//   head).  All rows meet every key, and each warp takes 16 of a block's 64
-//   keys, with its own ring of keys in shared memory: warps never wait for one
-//   another before the tile's end, where their maxima, sums and contexts are
-//   merged.  Per 16 keys and 128 elements a warp issues 32 mma for 8 KB of
-//   cache; HBM's share of an SM (44 GB/s) leaves five times the issue slots
-//   that this takes, so the kernel is bound by the cache's bytes.
-// kRowSplit true: tiles of 64 rows, 16 a warp, every warp through all keys.
+// MT 1, 2: tiles of 16 or 32 rows (a decode step's query heads of one key
+//   head, or those of a few drafted tokens).  All rows meet every key, and each
+//   warp takes 16 of a block's 64 keys, with its own ring of keys in shared
+//   memory: warps never wait for one another before the tile's end, where
+//   their maxima, sums and contexts are merged.  Per 16 keys, 16 rows and 128
+//   elements a warp issues 32 mma for 8 KB of cache; HBM's share of an SM (44
+//   GB/s) leaves five times the issue slots that this takes, so the kernel is
+//   bound by the cache's bytes.
+// MT 0: tiles of 64 rows, 16 a warp, every warp through all keys (head_dim
+//   above 128 with many rows).
 //
 // Two CTAs an SM with 96 KB of keys and values in flight each cover HBM's
 // latency (44 GB/s x ~1 us = 44 KB an SM) through the ends of tiles.
 // Each lane looks up the page of one key a block ahead and hands the address
 // to the lanes that copy the row, so the table's latency hides behind a block.
-template <typename T, int DP, bool kRowSplit>
+template <typename T, int DP, int MT>
 __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_kernel(const AttnParams p) {
   using S = Shape<DP>;
-  constexpr int TR = kRowSplit ? 64 : 16;
+  constexpr bool kRowSplit = MT == 0;
+  constexpr int M = kRowSplit ? 1 : MT;          // 16-row fragments a warp computes with
+  constexpr int TR = kRowSplit ? 64 : 16 * MT;
   constexpr int NK = kRowSplit ? 64 : 16;        // keys a warp computes with per block
   constexpr int kChunks = DP / 8;                // 16-byte chunks a row
-  constexpr bool kQRegs = DP <= 128;             // query fragments live in registers
+  constexpr bool kQRegs = DP * M <= 128;         // query fragments live in registers, or the tile in shared memory
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ AttnShare share;
   __shared__ int64_t warp_sum[kWarps];
@@ -96,12 +100,12 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_kernel
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t ring = smem_addr(smem);
   float* merge = reinterpret_cast<float*>(smem + (size_t)S::kStages * 2 * S::kTileBytes);
-  const uint32_t q_smem = smem_addr(merge);      // row-split, DP 256: the query tile instead
+  const uint32_t q_smem = smem_addr(merge);      // the query tile, while nothing is merged
 
   pdl_wait();
   attn_share<TR, kKeys, kThreads>(p, &share, warp_sum);
   const int64_t u0 = share.u0, u1 = share.u1;
-  if (threadIdx.x == 0) p.head[blockIdx.x] = make_int4(-1, 0, 0, kPartNone);
+  if (threadIdx.x == 0) attn_no_parts(p);
   if (u1 <= u0) return;
 
   // ---- loading: `ld` walks ahead of the computation
@@ -150,44 +154,48 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_kernel
 
   // ---- computing
   const int g = lane >> 2, t4 = lane & 3;
-  uint32_t qf[kQRegs ? DP / 16 : 1][4];
-  float o[DP / 8][4];
-  float m[2], l[2];
-  int lim[2], lim_all = 0;
+  uint32_t qf[kQRegs ? DP / 16 : 1][M][4];
+  float o[M][DP / 8][4];
+  float m[M][2], l[M][2];
+  int lim[M][2], lim_all = 0;
   int tile_kb0 = w.kb;
-  // rows of this lane: packed rows row0 and row0 + 8
+  // rows of this lane in fragment f: f * 16 + g and f * 16 + g + 8 of the warp's
+  const int row_in = (kRowSplit ? warp * 16 : 0) + g;
   auto open_tile = [&]() {
     tile_kb0 = w.kb;
-    const int row0 = w.rt * TR + (kRowSplit ? warp * 16 : 0) + g;
     lim_all = min(w.r.kv, attn_limit(p, w.r, w.rt * TR));
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int row = row0 + 8 * i;
-      const bool live = row < w.r.rows;
-      lim[i] = live ? min(w.r.kv, attn_limit(p, w.r, row)) : 0;
-      m[i] = kNegInf;
-      l[i] = 0.f;
-    }
+    for (int f = 0; f < M; ++f) {
 #pragma unroll
-    for (int d = 0; d < DP / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
+      for (int i = 0; i < 2; ++i) {
+        const int row = w.rt * TR + row_in + f * 16 + 8 * i;
+        lim[f][i] = row < w.r.rows ? min(w.r.kv, attn_limit(p, w.r, row)) : 0;
+        m[f][i] = kNegInf;
+        l[f][i] = 0.f;
+      }
+#pragma unroll
+      for (int d = 0; d < DP / 8; ++d) o[f][d][0] = o[f][d][1] = o[f][d][2] = o[f][d][3] = 0.f;
+    }
     auto q_row = [&](int row) -> const char* {
       const int tok = row / p.group, hd = w.h * p.group + row % p.group;
       return p.q + (int64_t)(w.r.q0 + tok) * p.ld_q + (int64_t)hd * p.kv.dim * 2;
     };
     if (kQRegs) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int row = row0 + 8 * i;
-        const bool live = row < w.r.rows;
-        const char* src = q_row(live ? row : 0);
+      for (int f = 0; f < M; ++f)
 #pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) {
-          const int d = ks * 16 + 2 * t4;
-          qf[kQRegs ? ks : 0][i] = live && d < p.kv.dim ? *reinterpret_cast<const uint32_t*>(src + d * 2) : 0u;
-          qf[kQRegs ? ks : 0][i + 2] =
-              live && d + 8 < p.kv.dim ? *reinterpret_cast<const uint32_t*>(src + d * 2 + 16) : 0u;
+        for (int i = 0; i < 2; ++i) {
+          const int row = w.rt * TR + row_in + f * 16 + 8 * i;
+          const bool live = row < w.r.rows;
+          const char* src = q_row(live ? row : 0);
+#pragma unroll
+          for (int ks = 0; ks < DP / 16; ++ks) {
+            const int d = ks * 16 + 2 * t4;
+            qf[kQRegs ? ks : 0][f][i] = live && d < p.kv.dim ? *reinterpret_cast<const uint32_t*>(src + d * 2) : 0u;
+            qf[kQRegs ? ks : 0][f][i + 2] =
+                live && d + 8 < p.kv.dim ? *reinterpret_cast<const uint32_t*>(src + d * 2 + 16) : 0u;
+          }
         }
-      }
     } else {
       // the query tile in shared memory, in the layout of the keys
       __syncthreads();
@@ -211,77 +219,95 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_kernel
 
     const uint32_t kt = ring + (stage * 2) * S::kTileBytes, vt = kt + S::kTileBytes;
     const int krow0 = kRowSplit ? 0 : warp * 16;    // first of this warp's keys in the block
-    float s[NK / 8][4];
+    float s[M][NK / 8][4];
 #pragma unroll
-    for (int n = 0; n < NK / 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+    for (int f = 0; f < M; ++f)
+#pragma unroll
+      for (int n = 0; n < NK / 8; ++n) s[f][n][0] = s[f][n][1] = s[f][n][2] = s[f][n][3] = 0.f;
 #pragma unroll
     for (int ks = 0; ks < DP / 16; ++ks) {
-      uint32_t a[4];
-      if (kQRegs) {
+      uint32_t a[M][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) a[i] = qf[kQRegs ? ks : 0][i];
-      } else {
-        const int r = (kRowSplit ? warp * 16 : 0) + (lane & 7) + ((lane >> 3) & 1) * 8;
-        ldsm4(chunk_addr<DP>(q_smem, r, ks * 2 + (lane >> 4)), a);
+      for (int f = 0; f < M; ++f) {
+        if (kQRegs) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) a[f][i] = qf[kQRegs ? ks : 0][f][i];
+        } else {
+          const int r = (kRowSplit ? warp * 16 : f * 16) + (lane & 7) + ((lane >> 3) & 1) * 8;
+          ldsm4(chunk_addr<DP>(q_smem, r, ks * 2 + (lane >> 4)), a[f]);
+        }
       }
 #pragma unroll
       for (int n2 = 0; n2 < NK / 16; ++n2) {
         uint32_t b[4];
         const int r = krow0 + n2 * 16 + (lane & 7) + ((lane >> 4) & 1) * 8;
         ldsm4(chunk_addr<DP>(kt, r, ks * 2 + ((lane >> 3) & 1)), b);
-        mma16816<T>(s[2 * n2], a, b[0], b[1]);
-        mma16816<T>(s[2 * n2 + 1], a, b[2], b[3]);
+#pragma unroll
+        for (int f = 0; f < M; ++f) {
+          mma16816<T>(s[f][2 * n2], a[f], b[0], b[1]);
+          mma16816<T>(s[f][2 * n2 + 1], a[f], b[2], b[3]);
+        }
       }
     }
     const int key0 = w.kb * kKeys + krow0;
     const bool masked = key0 + NK > lim_all;
-    float mx[2] = {kNegInf, kNegInf};
 #pragma unroll
-    for (int n = 0; n < NK / 8; ++n)
+    for (int f = 0; f < M; ++f) {
+      float mx[2] = {kNegInf, kNegInf};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (masked && key0 + n * 8 + 2 * t4 + (i & 1) >= lim[i >> 1]) s[n][i] = kNegInf;
-        mx[i >> 1] = fmaxf(mx[i >> 1], s[n][i]);
-      }
+      for (int n = 0; n < NK / 8; ++n)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
-      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-      mx[i] = fmaxf(m[i], mx[i] * p.scale_log2);
-    }
-    if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
+        for (int i = 0; i < 4; ++i) {
+          if (masked && key0 + n * 8 + 2 * t4 + (i & 1) >= lim[f][i >> 1]) s[f][n][i] = kNegInf;
+          mx[i >> 1] = fmaxf(mx[i >> 1], s[f][n][i]);
+        }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float f = mx[i] > m[i] ? exp2_fast(m[i] - mx[i]) : 1.f;   // m = -inf: 0
-        m[i] = mx[i];
-        l[i] *= f;
+        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+        mx[i] = fmaxf(m[f][i], mx[i] * p.scale_log2);
+      }
+      if (__any_sync(0xffffffffu, mx[0] > m[f][0] || mx[1] > m[f][1])) {
 #pragma unroll
-        for (int d = 0; d < DP / 8; ++d) {
-          o[d][2 * i] *= f;
-          o[d][2 * i + 1] *= f;
+        for (int i = 0; i < 2; ++i) {
+          const float e = mx[i] > m[f][i] ? exp2_fast(m[f][i] - mx[i]) : 1.f;   // m = -inf: 0
+          m[f][i] = mx[i];
+          l[f][i] *= e;
+#pragma unroll
+          for (int d = 0; d < DP / 8; ++d) {
+            o[f][d][2 * i] *= e;
+            o[f][d][2 * i + 1] *= e;
+          }
         }
       }
+      const float sub[2] = {m[f][0] == kNegInf ? 0.f : Num<T>::kBias - m[f][0],
+                            m[f][1] == kNegInf ? 0.f : Num<T>::kBias - m[f][1]};
+#pragma unroll
+      for (int n = 0; n < NK / 8; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[f][n][i] = exp2_fast(fmaf(s[f][n][i], p.scale_log2, sub[i >> 1]));
+          l[f][i >> 1] += s[f][n][i];
+        }
     }
-    const float sub[2] = {m[0] == kNegInf ? 0.f : Num<T>::kBias - m[0], m[1] == kNegInf ? 0.f : Num<T>::kBias - m[1]};
-#pragma unroll
-    for (int n = 0; n < NK / 8; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[n][i] = exp2_fast(fmaf(s[n][i], p.scale_log2, sub[i >> 1]));
-        l[i >> 1] += s[n][i];
-      }
 #pragma unroll
     for (int k2 = 0; k2 < NK / 16; ++k2) {
-      const uint32_t a[4] = {Num<T>::pack(s[2 * k2][0], s[2 * k2][1]), Num<T>::pack(s[2 * k2][2], s[2 * k2][3]),
-                             Num<T>::pack(s[2 * k2 + 1][0], s[2 * k2 + 1][1]),
-                             Num<T>::pack(s[2 * k2 + 1][2], s[2 * k2 + 1][3])};
+      uint32_t a[M][4];
+#pragma unroll
+      for (int f = 0; f < M; ++f)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          a[f][i] = Num<T>::pack(s[f][2 * k2 + (i >> 1)][2 * (i & 1)], s[f][2 * k2 + (i >> 1)][2 * (i & 1) + 1]);
 #pragma unroll
       for (int d2 = 0; d2 < DP / 16; ++d2) {
         uint32_t b[4];
         const int r = krow0 + k2 * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
         ldsm4_t(chunk_addr<DP>(vt, r, d2 * 2 + (lane >> 4)), b);
-        mma16816<T>(o[2 * d2], a, b[0], b[1]);
-        mma16816<T>(o[2 * d2 + 1], a, b[2], b[3]);
+#pragma unroll
+        for (int f = 0; f < M; ++f) {
+          mma16816<T>(o[f][2 * d2], a[f], b[0], b[1]);
+          mma16816<T>(o[f][2 * d2 + 1], a[f], b[2], b[3]);
+        }
       }
     }
 
@@ -291,72 +317,80 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_kernel
       const bool whole = last && tile_kb0 == 0;
       // slot 0: a tile entered in the middle; slot 1: a tile left unfinished
       const int64_t slot = 2 * (int64_t)blockIdx.x + (tile_kb0 == 0 ? 1 : 0);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-      }
       auto out_row = [&](int row) -> char* {
         const int tok = row / p.group, hd = w.h * p.group + row % p.group;
         return p.out + (int64_t)(w.r.q0 + tok) * p.ld_out + (int64_t)hd * p.kv.dim * 2;
       };
-      if (kRowSplit) {
+#pragma unroll
+      for (int f = 0; f < M; ++f) {
+        const int frag_rows = w.r.rows - w.rt * TR - f * 16;   // rows from this fragment on
+        if (!kRowSplit && frag_rows <= 0) break;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int r = warp * 16 + g + 8 * i, row = w.rt * TR + r;
-          if (row >= w.r.rows) continue;
-          if (whole) {
-            const float inv = l[i] > 0.f ? 1.f / l[i] : (l[i] == 0.f ? 0.f : l[i]);
-            char* dst = out_row(row);
-#pragma unroll
-            for (int d = 0; d < DP / 8; ++d)
-              if (d * 8 < p.kv.dim)
-                *reinterpret_cast<uint32_t*>(dst + (d * 8 + 2 * t4) * 2) =
-                    Num<T>::pack(o[d][2 * i] * inv, o[d][2 * i + 1] * inv);
-          } else {
-            float* dst = p.part_o + (slot * TR + r) * DP;
-#pragma unroll
-            for (int d = 0; d < DP / 8; ++d)
-              *reinterpret_cast<float2*>(dst + d * 8 + 2 * t4) = make_float2(o[d][2 * i], o[d][2 * i + 1]);
-            if (t4 == 0) p.part_ml[slot * TR + r] = make_float2(m[i], l[i]);
-          }
+          l[f][i] += __shfl_xor_sync(0xffffffffu, l[f][i], 1);
+          l[f][i] += __shfl_xor_sync(0xffffffffu, l[f][i], 2);
         }
-      } else {
-        // merge the warps: their common maximum, then the contexts added up
-        // in warp order
+        if (kRowSplit) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int r = row_in + 8 * i, row = w.rt * TR + r;
+            if (row >= w.r.rows) continue;
+            if (whole) {
+              const float inv = l[f][i] > 0.f ? 1.f / l[f][i] : (l[f][i] == 0.f ? 0.f : l[f][i]);
+              char* dst = out_row(row);
+#pragma unroll
+              for (int d = 0; d < DP / 8; ++d)
+                if (d * 8 < p.kv.dim)
+                  *reinterpret_cast<uint32_t*>(dst + (d * 8 + 2 * t4) * 2) =
+                      Num<T>::pack(o[f][d][2 * i] * inv, o[f][d][2 * i + 1] * inv);
+            } else {
+              float* dst = p.part_o + (slot * TR + r) * DP;
+#pragma unroll
+              for (int d = 0; d < DP / 8; ++d)
+                *reinterpret_cast<float2*>(dst + d * 8 + 2 * t4) = make_float2(o[f][d][2 * i], o[f][d][2 * i + 1]);
+              if (t4 == 0) p.part_ml[slot * TR + r] = make_float2(m[f][i], l[f][i]);
+            }
+          }
+          continue;
+        }
+        // merge the warps: their common maximum, then the contexts added up in
+        // a fixed order
         if (t4 == 0) {
-          merge_m[warp][g] = m[0];
-          merge_m[warp][g + 8] = m[1];
+          merge_m[warp][g] = m[f][0];
+          merge_m[warp][g + 8] = m[f][1];
         }
         __syncthreads();
-        float top[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          top[i] = merge_m[0][g + 8 * i];
+          float top = merge_m[0][g + 8 * i];
 #pragma unroll
-          for (int ww = 1; ww < kWarps; ++ww) top[i] = fmaxf(top[i], merge_m[ww][g + 8 * i]);
-          const float f = m[i] == kNegInf ? 0.f : exp2_fast(m[i] - top[i]);
-          l[i] = l[i] * f;
+          for (int ww = 1; ww < kWarps; ++ww) top = fmaxf(top, merge_m[ww][g + 8 * i]);
+          const float e = m[f][i] == kNegInf ? 0.f : exp2_fast(m[f][i] - top);
+          l[f][i] *= e;
 #pragma unroll
           for (int d = 0; d < DP / 8; ++d) {
-            o[d][2 * i] *= f;
-            o[d][2 * i + 1] *= f;
+            o[f][d][2 * i] *= e;
+            o[f][d][2 * i + 1] *= e;
           }
         }
         if (t4 == 0) {
-          merge_l[warp][g] = l[0];
-          merge_l[warp][g + 8] = l[1];
+          merge_l[warp][g] = l[f][0];
+          merge_l[warp][g + 8] = l[f][1];
         }
-        for (int ww = 0; ww < kWarps; ++ww) {
-          if (warp == ww) {
+        // warps 2 and 3 leave theirs in a buffer each, warps 0 and 1 add their own
+        static_assert(kWarps == 4, "merge order");
+#pragma unroll
+        for (int step = 0; step < 2; ++step) {
+          if ((warp >> 1) != step) {
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
               for (int d = 0; d < DP / 8; ++d) {
                 // columns XORed with the row, so that the eight rows of a store take different banks
-                float2* dst = reinterpret_cast<float2*>(merge + (g + 8 * i) * DP + ((d * 8 + 2 * t4) ^ (g * 8)));
-                float2 v = make_float2(o[d][2 * i], o[d][2 * i + 1]);
-                if (ww) {
+                float2* dst = reinterpret_cast<float2*>(merge + (warp & 1) * 16 * DP + (g + 8 * i) * DP +
+                                                        ((d * 8 + 2 * t4) ^ (g * 8)));
+                float2 v = make_float2(o[f][d][2 * i], o[f][d][2 * i + 1]);
+                if (step) {
                   const float2 old = *dst;
                   v.x = old.x + v.x;
                   v.y = old.y + v.y;
@@ -367,39 +401,33 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_kernel
           __syncthreads();
         }
         for (int c = threadIdx.x; c < 16 * (DP / 8); c += kThreads) {
-          const int r = c / (DP / 8), d8 = c % (DP / 8), row = w.rt * TR + r;
-          if (row >= w.r.rows) continue;
+          const int r = c / (DP / 8), d8 = c % (DP / 8);
+          if (r >= frag_rows) break;
           const float4* src = reinterpret_cast<const float4*>(merge + r * DP + ((d8 * 8) ^ ((r & 7) * 8)));
-          const float4 a = src[0], b = src[1];
+          float4 a = src[0], b = src[1];
+          const float4 a1 = src[16 * DP / 4], b1 = src[16 * DP / 4 + 1];
+          a = make_float4(a.x + a1.x, a.y + a1.y, a.z + a1.z, a.w + a1.w);
+          b = make_float4(b.x + b1.x, b.y + b1.y, b.z + b1.z, b.w + b1.w);
           const float sum = merge_l[0][r] + merge_l[1][r] + merge_l[2][r] + merge_l[3][r];
           if (whole) {
             const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
             if (d8 * 8 < p.kv.dim)
-              *reinterpret_cast<uint4*>(out_row(row) + d8 * 16) =
+              *reinterpret_cast<uint4*>(out_row(w.rt * TR + f * 16 + r) + d8 * 16) =
                   make_uint4(Num<T>::pack(a.x * inv, a.y * inv), Num<T>::pack(a.z * inv, a.w * inv),
                              Num<T>::pack(b.x * inv, b.y * inv), Num<T>::pack(b.z * inv, b.w * inv));
           } else {
-            float4* dst = reinterpret_cast<float4*>(p.part_o + (slot * TR + r) * DP + d8 * 8);
+            float4* dst = reinterpret_cast<float4*>(p.part_o + (slot * TR + f * 16 + r) * DP + d8 * 8);
             dst[0] = a;
             dst[1] = b;
             if (d8 == 0) {
               const float top_m = fmaxf(fmaxf(merge_m[0][r], merge_m[1][r]), fmaxf(merge_m[2][r], merge_m[3][r]));
-              p.part_ml[slot * TR + r] = make_float2(top_m, sum);
+              p.part_ml[slot * TR + f * 16 + r] = make_float2(top_m, sum);
             }
           }
         }
         __syncthreads();
       }
-      if (!whole && threadIdx.x == 0) {
-        int4* hd = &p.head[blockIdx.x];
-        if (tile_kb0 == 0) {
-          hd->x = w.b;
-          hd->y = w.rt;
-          hd->z = w.h;
-        } else {
-          hd->w = last ? kPartEnds : kPartGoesOn;
-        }
-      }
+      if (!whole && threadIdx.x == 0) attn_leave_part(p, w, tile_kb0 == 0, last);
       if (u + 1 < u1) {
         attn_next_tile<TR, kKeys>(p, w);
         open_tile();
@@ -412,117 +440,114 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_kernel
   pdl_trigger();
 }
 
-// The pieces of the tile that CTA c left unfinished: c's slot 1, then slot 0 of
-// the CTAs after it up to the one where the tile ends.
-__device__ __forceinline__ int join_pieces(const AttnParams& p, int c, int ctas) {
-  const int lane = threadIdx.x & 31;
-  for (int i = c + 1;; i += 32) {
-    const int st = i + lane < ctas ? p.head[i + lane].w : kPartEnds;   // the last CTA ends the line
-    const unsigned ends = __ballot_sync(0xffffffffu, st == kPartEnds);
-    if (ends) return min(i + __ffs(ends) - c, ctas - c);
-  }
-}
-__device__ __forceinline__ int64_t join_slot(int c, int i) {
-  return i == 0 ? 2 * (int64_t)c + 1 : 2 * (int64_t)(c + i);
-}
-template <int TR>
-__device__ __forceinline__ float join_top(const AttnParams& p, int c, int n, int row_t) {
-  float top = kNegInf;
-  for (int i = threadIdx.x & 31; i < n; i += 32) top = fmaxf(top, p.part_ml[join_slot(c, i) * TR + row_t].x);
-#pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-  return top;
-}
-// a[], sum += pieces i0, i0 + step, ..; lane's columns: kCols consecutive ones a span of 32 * kCols
-template <int TR, int DP, int kCols>
-__device__ __forceinline__ void join_add(const AttnParams& p, int c, int n, int row_t, int i0, int step, float top,
-                                         float* a, float& sum) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll 4
-  for (int i = i0; i < n; i += step) {
-    const float2 ml = p.part_ml[join_slot(c, i) * TR + row_t];
-    const float* src = p.part_o + (join_slot(c, i) * TR + row_t) * DP + lane * kCols;
-    float v[DP / 32];
-#pragma unroll
-    for (int s = 0; s < DP / (32 * kCols); ++s) {
-      if (kCols == 4) *reinterpret_cast<float4*>(v + 4 * s) = *reinterpret_cast<const float4*>(src + s * 128);
-      else *reinterpret_cast<float2*>(v + 2 * s) = *reinterpret_cast<const float2*>(src + s * 64);
-    }
-    if (ml.y == 0.f) continue;      // saw no key; its context may not have been written
-    const float f = exp2_fast(ml.x - top);
-    sum = fmaf(ml.y, f, sum);
-#pragma unroll
-    for (int k = 0; k < DP / 32; ++k) a[k] = fmaf(v[k], f, a[k]);
-  }
-}
+constexpr int kJoinWarps = 32;
 
-// Joins the pieces of tiles that CTAs left unfinished, in key order.
-// kSplit (tiles of 16 rows, up to hundreds of pieces): a warp takes every
-// eighth piece of a row, and the warps' sums meet in shared memory in warp
-// order.  Otherwise a warp takes a row: tiles of 64 and 256 rows have few
-// pieces and many rows.
+// Joins the pieces of the tiles that CTAs left unfinished: CTA c's slot 1, then
+// slot 0 of the CTAs after it up to the one where the tile ends.  One CTA per
+// c (and slice of a tall tile's rows): its warps are dealt to the rows, several
+// a row when there are fewer rows, each taking every w-th piece with a running
+// maximum of its own; a row's warps meet in shared memory in warp order.  The
+// pieces were just written, so they come from L2; bound by the latency of
+// three dependent reads.
 template <typename T, int TR, int DP>
-__global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnParams p, int ctas) {
-  constexpr int kCols = DP >= 128 ? 4 : 2;
-  constexpr bool kSplit = TR == 16;
-  __shared__ float acc[kSplit ? 8 : 1][DP];
-  __shared__ float wsum[8];
+__global__ void __launch_bounds__(32 * kJoinWarps) paged_attn_join_kernel(const AttnParams p, int ctas) {
+  constexpr int kRows = TR < kJoinWarps ? TR : kJoinWarps;    // rows a CTA joins
+  constexpr int kCols = DP >= 128 ? 4 : 2;                    // consecutive columns a lane
+  constexpr int kN = DP / 32;                                 // columns a lane
+  __shared__ float acc[kJoinWarps][DP];
+  __shared__ float2 wml[kJoinWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x;
   pdl_wait();
   const int4 hd = p.head[c];
+  // the state of every CTA after c, 32 at a time, all loads in flight together
+  constexpr int kLook = 10;
+  int st[kLook];
+#pragma unroll
+  for (int i = 0; i < kLook; ++i) {
+    const int o = c + 1 + i * 32 + lane;
+    st[i] = o < ctas ? p.state[o] : kPartEnds;                // the last CTA ends the line
+  }
   if (hd.x < 0) return;
-  const int n = join_pieces(p, c, ctas);
-  const AttnReq r = attn_req(p, hd.x);
-  const int rows = min(TR, r.rows - hd.y * TR);
-  auto dst_row = [&](int row) {
-    const int tok = row / p.group, head = hd.z * p.group + row % p.group;
-    return p.out + (int64_t)(r.q0 + tok) * p.ld_out + (int64_t)head * p.kv.dim * 2;
-  };
-  if (kSplit) {
-    for (int row_t = blockIdx.y; row_t < rows; row_t += gridDim.y) {
-      const float top = join_top<TR>(p, c, n, row_t);
-      float a[DP / 32] = {}, sum = 0.f;
-      join_add<TR, DP, kCols>(p, c, n, row_t, warp, 8, top, a, sum);
+  int n = 0;
 #pragma unroll
-      for (int k = 0; k < DP / 32; ++k) acc[kSplit ? warp : 0][(k / kCols) * 32 * kCols + lane * kCols + k % kCols] = a[k];
-      if (lane == 0) wsum[warp] = sum;
-      __syncthreads();
-      float total = 0.f;
+  for (int i = 0; i < kLook; ++i) {
+    const unsigned ends = __ballot_sync(0xffffffffu, st[i] == kPartEnds);
+    if (n == 0 && ends) n = 1 + i * 32 + __ffs(ends);
+  }
+  for (int i = kLook; n == 0; ++i) {                          // GPUs with more SMs than that
+    const int o = c + 1 + i * 32 + lane;
+    const unsigned ends = __ballot_sync(0xffffffffu, o >= ctas || p.state[o] == kPartEnds);
+    if (ends) n = 1 + i * 32 + __ffs(ends);
+  }
+  n = min(n, ctas - c);
+  const int row0 = hd.z * TR + blockIdx.y * kRows;
+  const int rows = min(kRows, hd.y - row0);                   // of this CTA's
+  if (rows <= 0) return;
+  int share = 1;                                              // warps a row
+  while (share * 2 * rows <= kJoinWarps) share *= 2;
+  const int row_t = warp / share, part = warp % share;
+  float m = kNegInf, l = 0.f, a[kN] = {};
+  if (row_t < rows) {
+#pragma unroll 8
+    for (int i = part; i < n; i += share) {
+      const int64_t at = (i == 0 ? 2 * (int64_t)c + 1 : 2 * (int64_t)(c + i)) * TR + blockIdx.y * kRows + row_t;
+      const float2 ml = p.part_ml[at];
+      const float* src = p.part_o + at * DP + lane * kCols;
+      float v[kN];
 #pragma unroll
-      for (int ww = 0; ww < 8; ++ww) total += wsum[ww];
-      const float inv = total > 0.f ? 1.f / total : (total == 0.f ? 0.f : total);
-      uint16_t* dst = reinterpret_cast<uint16_t*>(dst_row(hd.y * TR + row_t));
-      for (int d = threadIdx.x; d < p.kv.dim; d += 256) {
-        float v = 0.f;
-#pragma unroll
-        for (int ww = 0; ww < 8; ++ww) v += acc[kSplit ? ww : 0][d];
-        dst[d] = Num<T>::one(v * inv);
+      for (int s = 0; s < kN / kCols; ++s) {
+        if (kCols == 4) *reinterpret_cast<float4*>(v + 4 * s) = *reinterpret_cast<const float4*>(src + s * 128);
+        else *reinterpret_cast<float2*>(v + 2 * s) = *reinterpret_cast<const float2*>(src + s * 64);
       }
-      __syncthreads();
-    }
-  } else {
-    for (int row_t = blockIdx.y * 8 + warp; row_t < rows; row_t += gridDim.y * 8) {
-      const float top = join_top<TR>(p, c, n, row_t);
-      float a[DP / 32] = {}, sum = 0.f;
-      join_add<TR, DP, kCols>(p, c, n, row_t, 0, 1, top, a, sum);
-      const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
-      char* dst = dst_row(hd.y * TR + row_t);
+      const bool some = ml.y != 0.f;    // or it saw no key, and its context may not have been written
+      const float top = some ? fmaxf(m, ml.x) : m;
+      const float f = m == top ? 1.f : exp2_fast(m - top), e = some ? exp2_fast(ml.x - top) : 0.f;
+      m = top;
+      l = fmaf(ml.y, e, l * f);
 #pragma unroll
-      for (int k = 0; k < DP / 32; k += 2) {
-        const int d = (k / kCols) * 32 * kCols + lane * kCols + k % kCols;
-        if (d < p.kv.dim) *reinterpret_cast<uint32_t*>(dst + d * 2) = Num<T>::pack(a[k] * inv, a[k + 1] * inv);
-      }
+      for (int k = 0; k < kN; ++k) a[k] = fmaf(some ? v[k] : 0.f, e, a[k] * f);
     }
+  }
+  if (share > 1) {
+    if (lane == 0) wml[warp] = make_float2(m, l);
+#pragma unroll
+    for (int k = 0; k < kN; ++k) acc[warp][(k / kCols) * 32 * kCols + lane * kCols + k % kCols] = a[k];
+    __syncthreads();
+    if (part || row_t >= rows) return;
+    float top = m;
+    for (int w = 1; w < share; ++w) top = fmaxf(top, wml[warp + w].x);
+    const float f = m == kNegInf ? 0.f : exp2_fast(m - top);
+    l *= f;
+#pragma unroll
+    for (int k = 0; k < kN; ++k) a[k] *= f;
+    for (int w = 1; w < share; ++w) {
+      const float2 ml = wml[warp + w];
+      if (ml.y == 0.f) continue;
+      const float e = exp2_fast(ml.x - top);
+      l = fmaf(ml.y, e, l);
+#pragma unroll
+      for (int k = 0; k < kN; ++k)
+        a[k] = fmaf(acc[warp + w][(k / kCols) * 32 * kCols + lane * kCols + k % kCols], e, a[k]);
+    }
+  }
+  if (row_t >= rows) return;
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  const int row = row0 + row_t, tok = row / p.group, head = hd.w * p.group + row % p.group;
+  char* dst = p.out + (int64_t)(hd.x + tok) * p.ld_out + (int64_t)head * p.kv.dim * 2;
+#pragma unroll
+  for (int k = 0; k < kN; k += 2) {
+    const int d = (k / kCols) * 32 * kCols + lane * kCols + k % kCols;
+    if (d < p.kv.dim) *reinterpret_cast<uint32_t*>(dst + d * 2) = Num<T>::pack(a[k] * inv, a[k + 1] * inv);
   }
 }
 
-template <typename T, int DP, bool kRowSplit>
+template <typename T, int DP, int MT>
 int run_class(AttnParams p, const PagedAttention& a, int sms, cudaStream_t stream) {
-  constexpr int TR = kRowSplit ? 64 : 16;
+  constexpr int TR = MT == 0 ? 64 : 16 * MT;
   const int ctas = sms * Shape<DP>::kPerSm;
   attn_carve<TR, DP>(p, a.workspace, ctas);
-  constexpr size_t smem = smem_bytes<DP, kRowSplit>();
-  auto kernel = paged_attn_kernel<T, DP, kRowSplit>;
+  constexpr size_t smem = smem_bytes<DP, MT>();
+  auto kernel = paged_attn_kernel<T, DP, MT>;
   SMEAI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   SMEAI_CUDA_TRY(launch(kernel, dim3((unsigned)ctas), dim3(kThreads), smem, stream, p));
   // a tile of up to 2 * kSnap blocks is never split
@@ -532,12 +557,15 @@ int run_class(AttnParams p, const PagedAttention& a, int sms, cudaStream_t strea
 
 // Which kernels a call needs, from what the host knows: the largest request's
 // packed rows and the total.
-//   up to 16 rows   the 16-row tiles: keys split over the warps
-//   up to 64        the 64-row tiles
+//   up to 16 rows   16-row tiles
+//   up to 32        32-row tiles: one reading of the keys for all rows
 //   more            the tensor-core kernel, and the 16-row tiles beside it for
 //                   requests of up to 16 rows (a step that mixes prompts and
-//                   decoding) unless the total says that there are none;
-//                   head_dim above 128: the 64-row tiles for all
+//                   decoding) unless the total says that there are none: one
+//                   row costs the tensor-core kernel's tile as much as 256,
+//                   and 8 requests, one of 860 rows, took 148 us without the
+//                   second kernel and 104 us with it
+// head_dim above 128: up to 16 rows as above, more the 64-row tiles for all.
 struct Classes {
   bool few, mid, many;
 };
@@ -545,7 +573,7 @@ Classes classes(const PagedAttention& a) {
   const int64_t group = a.n_heads / a.kv.n_kv, most = a.max_new * group;
   Classes c = {false, false, false};
   if (most <= 16) c.few = true;
-  else if (most <= 64 || a.kv.dim > 128) c.mid = true;
+  else if (most <= 32 || a.kv.dim > 128) c.mid = true;
   else {
     c.many = true;
     // with one request of r <= 16 / group rows the others, of max_new at most, could not make up n_tokens
@@ -562,14 +590,16 @@ int run_dim(const AttnParams& p, const PagedAttention& a, int sms, cudaStream_t 
   if (c.few) {
     AttnParams q = p;
     if (c.many) q.rows_hi = 16;
-    const int st = run_class<T, DP, false>(q, a, sms, stream);
+    const int st = run_class<T, DP, 1>(q, a, sms, stream);
     if (st) return st;
   }
-  if (c.mid) return run_class<T, DP, true>(p, a, sms, stream);
-  if (c.many && DP <= 128) {
-    AttnParams q = p;
-    if (c.few) q.rows_lo = 16;
-    return paged_attn_tc(q, DP, a.workspace, a.max_kv, sms, stream);
+  if (c.mid) return run_class<T, DP, DP <= 128 ? 2 : 0>(p, a, sms, stream);
+  if constexpr (DP <= 128) {
+    if (c.many) {
+      AttnParams q = p;
+      if (c.few) q.rows_lo = 16;
+      return paged_attn_tc(q, DP, a.workspace, a.max_kv, sms, stream);
+    }
   }
   return kOk;
 }
@@ -578,8 +608,8 @@ int run_dim(const AttnParams& p, const PagedAttention& a, int sms, cudaStream_t 
 
 template <typename T, int TR, int DP>
 cudaError_t attn_join(const AttnParams& p, int ctas, cudaStream_t stream) {
-  const unsigned slices = TR == 16 ? 4u : TR / 16;
-  return launch(paged_attn_join_kernel<T, TR, DP>, dim3((unsigned)ctas, slices), dim3(256), 0, stream, p, ctas);
+  return launch(paged_attn_join_kernel<T, TR, DP>, dim3((unsigned)ctas, (unsigned)((TR + kJoinWarps - 1) / kJoinWarps)),
+                dim3(32 * kJoinWarps), 0, stream, p, ctas);
 }
 template cudaError_t attn_join<__half, 256, 64>(const AttnParams&, int, cudaStream_t);
 template cudaError_t attn_join<__half, 256, 128>(const AttnParams&, int, cudaStream_t);
@@ -591,16 +621,14 @@ size_t paged_attention_workspace(const PagedAttention& a) {
   if (sm_count(&sms)) return 0;
   const Classes c = classes(a);
   const int dp = padded_dim(a.kv.dim);
-  size_t few = 0, mid = 0;
-  switch (dp) {
-    case 64: few = attn_part_bytes<16, 64>(2 * sms), mid = attn_part_bytes<64, 64>(2 * sms); break;
-    case 128: few = attn_part_bytes<16, 128>(2 * sms), mid = attn_part_bytes<64, 128>(2 * sms); break;
-    default: few = attn_part_bytes<16, 256>(sms), mid = attn_part_bytes<64, 256>(sms);
-  }
-  size_t need = c.few ? few : 0;
-  if (c.mid && mid > need) need = mid;
-  const size_t many = c.many ? paged_attn_tc_workspace(dp, sms) : 0;
-  return many > need ? many : need;
+  if (c.many) return paged_attn_tc_workspace(dp, sms);   // the 16-row tiles' need is smaller
+  if (c.mid)
+    return dp == 64    ? attn_part_bytes<32, 64>(2 * sms)
+           : dp == 128 ? attn_part_bytes<32, 128>(2 * sms)
+                       : attn_part_bytes<64, 256>(sms);
+  return dp == 64    ? attn_part_bytes<16, 64>(2 * sms)
+         : dp == 128 ? attn_part_bytes<16, 128>(2 * sms)
+                     : attn_part_bytes<16, 256>(sms);
 }
 
 int paged_attention(const PagedAttention& a, cudaStream_t stream) {

@@ -38,7 +38,9 @@ struct AttnParams {
   int rows_lo, rows_hi;   // requests with rows_lo < rows <= rows_hi are this launch's
   float* part_o;          // [2 * CTAs][TR][DP]
   float2* part_ml;        // [2 * CTAs][TR] running maximum (log2 units), sum
-  int4* head;             // [CTAs] {tile left unfinished at the end: request or -1, row tile, key head; state of slot 0}
+  int4* head;             // [CTAs] tile left unfinished at the end {first row of its request or -1, the
+                          // request's packed rows, row tile, key head}
+  int* state;             // [CTAs] state of slot 0
   unsigned* err;
 };
 
@@ -106,7 +108,7 @@ __device__ __forceinline__ void attn_next_tile(const AttnParams& p, AttnPos& w) 
 
 struct AttnShare {
   int64_t u0, u1;            // this CTA's units
-  int b, rt, h, kb;          // place of u0
+  AttnPos at;                // place of u0
 };
 
 // This CTA's piece of the line.  All threads of the block call it; the place
@@ -134,7 +136,9 @@ __device__ void attn_share(const AttnParams& p, AttnShare* s, int64_t* warp_sum)
     total += warp_sum[w];
   }
   const int64_t lo = before + incl - mine;   // units ahead of this thread's run
-  const int64_t per_cta = (total + gridDim.x - 1) / gridDim.x;
+  // 64-bit division is slow, and totals are rarely that large
+  const int64_t per_cta = total <= 0x7fff0000 ? ((uint32_t)total + gridDim.x - 1) / gridDim.x
+                                              : (total + gridDim.x - 1) / gridDim.x;
   const int64_t cut0 = min(total, per_cta * blockIdx.x), cut1 = min(total, cut0 + per_cta);
   if (threadIdx.x == 0) {
     if (cut0 >= total) s->u0 = total;
@@ -155,7 +159,8 @@ __device__ void attn_share(const AttnParams& p, AttnShare* s, int64_t* warp_sum)
           at += (int64_t)nkb * p.kv.n_kv;
           continue;
         }
-        int h = (int)((cut - at) / nkb), kb = (int)((cut - at) % nkb);
+        const unsigned in = (unsigned)(cut - at);      // below nkb * n_kv, which fits
+        int h = (int)(in / (unsigned)nkb), kb = (int)(in % (unsigned)nkb);
         int64_t u = cut;
         if (kb <= kSnap && kb <= nkb - kb) {
           u -= kb;
@@ -167,10 +172,7 @@ __device__ void attn_share(const AttnParams& p, AttnShare* s, int64_t* warp_sum)
         if (which) s->u1 = u;
         else {
           s->u0 = u;
-          s->b = b;
-          s->rt = rt;
-          s->h = h;
-          s->kb = kb;
+          s->at = {b, rt, h, kb, nkb, r};
         }
         b = b1;
         break;
@@ -182,13 +184,18 @@ __device__ void attn_share(const AttnParams& p, AttnShare* s, int64_t* warp_sum)
 
 template <int TR, int KB>
 __device__ __forceinline__ void attn_open(const AttnParams& p, const AttnShare& s, AttnPos& w) {
-  w.b = s.b;
-  w.rt = s.rt;
-  w.h = s.h;
-  w.r = attn_req(p, s.b);
-  w.nkb = attn_blocks<TR, KB>(p, w.r, s.rt);
-  w.kb = s.kb;
-  if (s.kb == w.nkb) attn_next_tile<TR, KB>(p, w);
+  w = s.at;
+  if (w.kb == w.nkb) attn_next_tile<TR, KB>(p, w);
+}
+
+// Thread 0 of a CTA: its headers before any tile, and a tile not finished here.
+__device__ __forceinline__ void attn_no_parts(const AttnParams& p) {
+  p.head[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  p.state[blockIdx.x] = kPartNone;
+}
+__device__ __forceinline__ void attn_leave_part(const AttnParams& p, const AttnPos& w, bool begun_here, bool ends) {
+  if (begun_here) p.head[blockIdx.x] = make_int4(w.r.q0, w.r.rows, w.rt, w.h);
+  else p.state[blockIdx.x] = ends ? kPartEnds : kPartGoesOn;
 }
 
 // ---- 16-bit types ---------------------------------------------------------------
@@ -236,7 +243,7 @@ __device__ __forceinline__ void cp_async_wait() {
 // Partial slots and headers of a launch with `ctas` CTAs.
 template <int TR, int DP>
 constexpr size_t attn_part_bytes(int ctas) {
-  return (size_t)2 * ctas * TR * (DP * sizeof(float) + sizeof(float2)) + (size_t)ctas * sizeof(int4);
+  return (size_t)2 * ctas * TR * (DP * sizeof(float) + sizeof(float2)) + (size_t)ctas * (sizeof(int4) + sizeof(int));
 }
 template <int TR, int DP>
 void attn_carve(AttnParams& p, void* ws, int ctas) {
@@ -246,6 +253,7 @@ void attn_carve(AttnParams& p, void* ws, int ctas) {
   p.part_ml = reinterpret_cast<float2*>(c);
   c += (size_t)2 * ctas * TR * sizeof(float2);
   p.head = reinterpret_cast<int4*>(c);
+  p.state = reinterpret_cast<int*>(c + (size_t)ctas * sizeof(int4));
 }
 
 // The tensor-core kernel of requests with many rows, head_dim up to 128

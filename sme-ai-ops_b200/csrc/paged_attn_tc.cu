@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
   tc_fence_after();
   const uint32_t tmem = *m.tmem;
   const int64_t units = share.u1 - share.u0;
-  if (threadIdx.x == 0) p.head[blockIdx.x] = make_int4(-1, 0, 0, kPartNone);
+  if (threadIdx.x == 0) attn_no_parts(p);
 
   if (units <= 0) {
     // nothing to do
@@ -536,11 +536,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
       const bool live = row < w.r.rows;
       const int lim = live ? min(w.r.kv, attn_limit(p, w.r, row)) : 0;
       const int lim_all = min(w.r.kv, attn_limit(p, w.r, w.rt * kTR + t * 128));
+      const bool dead = w.rt * kTR + t * 128 + (warp & 3) * 32 >= w.r.rows;
       float mx = kNegInf, l = 0.f;
       const int cnt = s.cnt[t];
       for (int b = 0; b < cnt; ++b) {
         if (!(ok = wait_warp(m, &m.s_full[t], sc & 1, p.err, limit_ns))) break;
         ++sc;
+        if (dead) {   // none of the warp's rows exists: whatever P holds there, nobody reads
+          if (lane == 0) mbar_arrive(&m.p_full[t]);
+          continue;
+        }
         tc_fence_after();
         float v[128];
 #pragma unroll
@@ -617,7 +622,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
       const int tok = row / p.group, hd = w.h * p.group + row % p.group;
       char* dst = p.out + (int64_t)(w.r.q0 + tok) * p.ld_out + (int64_t)hd * p.kv.dim * 2;
       float* part = p.part_o + (slot * kTR + t * 128 + r) * DP;
-      if (cnt > 0) {
+      if (cnt > 0 && !dead) {
 #pragma unroll 1
         for (int i = 0; i < DP / 32; ++i) {
           float o[32];
@@ -646,16 +651,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
       }
       // a half without blocks in this stretch leaves an empty sum: its context is not read
       if (!whole && live) p.part_ml[slot * kTR + t * 128 + r] = make_float2(mx, l);
-      if (!whole && threadIdx.x == 0) {
-        int4* h = &p.head[blockIdx.x];
-        if (s.kb0 == 0) {
-          h->x = w.b;
-          h->y = w.rt;
-          h->z = w.h;
-        } else {
-          h->w = s.last ? kPartEnds : kPartGoesOn;
-        }
-      }
+      if (!whole && threadIdx.x == 0) attn_leave_part(p, w, s.kb0 == 0, s.last);
       left -= s.n;
       if (left > 0) attn_next_tile<kTR, kKB>(p, w);
     }
