@@ -30,77 +30,428 @@ __device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
                : "r"(addr)
                : "memory");
 }
-template <typename T>
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
-template <>
-__device__ __forceinline__ void mma16816<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-template <>
-__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
-                                                        uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// d += a b, or d = a b for the first step of a sum.
+template <typename T, bool kFirst = false>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  const float z = 0.f;
+  if constexpr (kFirst && Num<T>::kIsBf16)
+    asm(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(z));
+  else if constexpr (kFirst)
+    asm(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(z));
+  else if constexpr (Num<T>::kIsBf16)
+    asm(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 // Shared-memory layout: [stages][K, V][kKeys rows][DP] 16-bit, the 16-byte
 // chunks of a row XORed with the row's index mod 8, so that ldmatrix's eight
-// rows fall on different banks; then the merge buffer.
+// rows fall on different banks; then the merge buffer or the query tile.
 template <int DP>
 struct Shape {
   static constexpr int kRowBytes = DP * 2;
   static constexpr int kTileBytes = kKeys * kRowBytes;
   static constexpr int kStages = DP == 64 ? 6 : 3;      // 96 KB in flight (192 KB at DP 256)
   static constexpr int kPerSm = DP == 256 ? 1 : 2;      // CTAs an SM
+  static constexpr int kPitch = DP + 4;                 // floats a row of the merge buffer
 };
-template <int DP, int MT>
-constexpr size_t smem_bytes() {
-  using S = Shape<DP>;
-  return (size_t)S::kStages * 2 * S::kTileBytes + (MT == 0 ? 64 * DP * 2 : 2 * 16 * DP * 4);
-}
 
 template <int DP>
 __device__ __forceinline__ uint32_t chunk_addr(uint32_t base, int row, int chunk) {
   return base + row * Shape<DP>::kRowBytes + ((chunk ^ (row & 7)) << 4);
 }
 
-// MT 1, 2: tiles of 16 or 32 rows (a decode step's query heads of one key
-//   head, or those of a few drafted tokens).  All rows meet every key, and each
-//   warp takes 16 of a block's 64 keys, with its own ring of keys in shared
-//   memory: warps never wait for one another before the tile's end, where
-//   their maxima, sums and contexts are merged.  Per 16 keys, 16 rows and 128
-//   elements a warp issues 32 mma for 8 KB of cache; HBM's share of an SM (44
-//   GB/s) leaves five times the issue slots that this takes, so the kernel is
-//   bound by the cache's bytes.
-// MT 0: tiles of 64 rows, 16 a warp, every warp through all keys (head_dim
-//   above 128 with many rows).
-//
-// Two CTAs an SM with 96 KB of keys and values in flight each cover HBM's
-// latency (44 GB/s x ~1 us = 44 KB an SM) through the ends of tiles.
-// Each lane looks up the page of one key a block ahead and hands the address
-// to the lanes that copy the row, so the table's latency hides behind a block.
-template <typename T, int DP, int MT>
-__global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_kernel(const AttnParams p) {
+// Walks a CTA's share ahead of the computation and copies blocks into the
+// ring.  Warp w copies rows 16w .. 16w + 15 of a block.  Each lane looks up the
+// page of one of these keys a block ahead, so that the table's latency hides
+// behind a block, and hands its address to the lanes that copy the row: eight
+// lanes take 128 contiguous bytes of it, four rows at a time.
+template <int DP, int TR>
+struct Loader {
   using S = Shape<DP>;
-  constexpr bool kRowSplit = MT == 0;
-  constexpr int M = kRowSplit ? 1 : MT;          // 16-row fragments a warp computes with
-  constexpr int TR = kRowSplit ? 64 : 16 * MT;
-  constexpr int NK = kRowSplit ? 64 : 16;        // keys a warp computes with per block
-  constexpr int kChunks = DP / 8;                // 16-byte chunks a row
-  constexpr bool kQRegs = DP * M <= 128;         // query fragments live in registers, or the tile in shared memory
+  AttnPos at;
+  int64_t left;
+  int page;             // of this lane's key in block `at`; -1: no such key, or a bad page
+  uint32_t even, odd;   // place of row i * 4 + lane / 8 of the warp's, for even and odd i, less i
+  int bytes[DP / 64];   // 0 past the head's elements
+
+  __device__ __forceinline__ void look_up(const AttnParams& p) {
+    const int lane = threadIdx.x & 31, key = at.kb * kKeys + (int)(threadIdx.x >> 5) * 16 + (lane & 15);
+    page = key < at.r.kv ? p.table[(int64_t)at.b * p.ld_table + (key >> p.kv.page_log2)] : -1;
+    if (key < at.r.kv && (page < 0 || page >= p.kv.n_pages)) {
+      raise_device_error(p.err, kDevErrBadIndex);
+      page = -1;
+    }
+  }
+  __device__ __forceinline__ void open(const AttnParams& p, const AttnPos& from, int64_t units) {
+    const int lane = threadIdx.x & 31, sub = lane >> 3, col = lane & 7, row0 = (int)(threadIdx.x >> 5) * 16;
+    at = from;
+    left = units;
+    even = (row0 + sub) * S::kRowBytes + ((col ^ sub) << 4);
+    odd = (row0 + sub) * S::kRowBytes + ((col ^ (sub + 4)) << 4);
+#pragma unroll
+    for (int cb = 0; cb < DP / 64; ++cb) bytes[cb] = cb * 64 + col * 8 < p.kv.dim ? 16 : 0;
+    look_up(p);
+  }
+  // the next block into `stage` (shared-memory address of its keys); one commit group
+  __device__ __forceinline__ void load(const AttnParams& p, uint32_t stage) {
+    if (left > 0) {
+      const int lane = threadIdx.x & 31, sub = lane >> 3, col = lane & 7;
+      const int key = at.kb * kKeys + (int)(threadIdx.x >> 5) * 16 + (lane & 15);
+      const int64_t off = page < 0 ? 0
+                                   : page * p.kv.page_bytes +
+                                         (key & ((1 << p.kv.page_log2) - 1)) * p.kv.token_bytes + at.h * p.kv.head_bytes;
+      const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
+      const char *k = p.kv.k + col * 16, *v = p.kv.v + col * 16;
+      const uint32_t d0 = stage + even, d1 = stage + odd;
+      if (there == 0xffffffffu) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int64_t o = __shfl_sync(0xffffffffu, off, i * 4 + sub);
+          const uint32_t d = (i & 1 ? d1 : d0) + i * 4 * S::kRowBytes;
+#pragma unroll
+          for (int cb = 0; cb < DP / 64; ++cb) {
+            cp_async16(d + cb * 128, k + o + cb * 128, bytes[cb]);
+            cp_async16(d + cb * 128 + S::kTileBytes, v + o + cb * 128, bytes[cb]);
+          }
+        }
+      } else {
+        // some keys do not exist: zeros, and nothing is read
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int64_t o = __shfl_sync(0xffffffffu, off, i * 4 + sub);
+          const bool ok = there >> (i * 4 + sub) & 1;
+          const uint32_t d = (i & 1 ? d1 : d0) + i * 4 * S::kRowBytes;
+#pragma unroll
+          for (int cb = 0; cb < DP / 64; ++cb) {
+            cp_async16(d + cb * 128, k + (ok ? o + cb * 128 : -col * 16), ok ? bytes[cb] : 0);
+            cp_async16(d + cb * 128 + S::kTileBytes, v + (ok ? o + cb * 128 : -col * 16), ok ? bytes[cb] : 0);
+          }
+        }
+      }
+      if (--left > 0) {
+        if (++at.kb == at.nkb) attn_next_tile<TR, kKeys>(p, at);
+        look_up(p);
+      }
+    }
+    cp_async_commit();
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ float row_scale(float sum) {   // 0 rows for a sum of nothing, NaN kept
+  return sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+}
+
+// ---- few rows -----------------------------------------------------------------
+// Tiles of 8 * NQ rows: a decode step's query heads of one key head, or those
+// of a few drafted tokens.  The products are taken transposed, with the keys
+// as the MMA's 16-wide dimension and eight rows as its 8-wide one,
+//   S^T = K Q^T,  O^T += V^T P^T
+// so eight rows cost DP/8 mma per 16 keys, half of what a 16-row fragment of
+// queries would.  All rows meet every key, and each warp takes 16 of a block's
+// 64 keys, with its own ring of keys in shared memory: warps never wait for
+// one another before the tile's end, where their maxima, sums and contexts
+// are merged.  A row's maximum is only raised when a score passes it by more
+// than 2^8, so most blocks need a vote and no reduction over the keys.
+// Two CTAs an SM with 96 KB of keys and values in flight each cover HBM's
+// latency (44 GB/s x ~1 us = 44 KB an SM) through the ends of tiles; bound by
+// the cache's bytes.
+constexpr float kRaise = 8.f;
+
+// 8x8 16-bit transpose across the warp.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+template <int DP>
+constexpr size_t few_smem() {
+  using S = Shape<DP>;
+  return (size_t)S::kStages * 2 * S::kTileBytes + 2 * 8 * S::kPitch * sizeof(float);
+}
+
+template <typename T, int DP, int NQ>
+__global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_few_kernel(const AttnParams p) {
+  using S = Shape<DP>;
+  constexpr int TR = 8 * NQ;
+  constexpr int kAhead = 4;          // ldmatrix in flight ahead of the products
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ AttnShare share;
   __shared__ int64_t warp_sum[kWarps];
-  __shared__ float merge_m[kWarps][16], merge_l[kWarps][16];
+  __shared__ float merge_m[kWarps][8], merge_l[kWarps][8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, t4 = lane & 3;
   const uint32_t ring = smem_addr(smem);
   float* merge = reinterpret_cast<float*>(smem + (size_t)S::kStages * 2 * S::kTileBytes);
-  const uint32_t q_smem = smem_addr(merge);      // the query tile, while nothing is merged
+
+  // every CTA is resident: the kernel behind can only take what these free
+  pdl_trigger();
+  pdl_wait();
+  attn_share<TR, kKeys, kThreads>(p, &share, warp_sum);
+  const int64_t u0 = share.u0, u1 = share.u1;
+  if (threadIdx.x == 0) attn_no_parts(p);
+  if (u1 <= u0) return;
+
+  AttnPos w;
+  attn_open<TR, kKeys>(p, share, w);
+  Loader<DP, TR> ld;
+  ld.open(p, w, u1 - u0);
+  for (int s = 0; s < S::kStages - 1; ++s) ld.load(p, ring + s * 2 * S::kTileBytes);
+
+  // Q^T fragments: row (n) g of each eight, elements (k) 2 t4 and 2 t4 + 8 on.
+  // Scores and contexts of this lane: rows 2 t4 and 2 t4 + 1 of each eight.
+  uint32_t qf[DP / 16][NQ][2];
+  float o[DP / 16][NQ][4];
+  float m[NQ][2], l[NQ][2];
+  float most[NQ][2];                   // scores (before the scale) that leave the maximum as it is
+  int lim[NQ][2], lim_all = 0;
+  int tile_kb0 = w.kb;
+  auto open_tile = [&]() {
+    tile_kb0 = w.kb;
+    lim_all = min(w.r.kv, attn_limit(p, w.r, w.rt * TR));
+#pragma unroll
+    for (int f = 0; f < NQ; ++f) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = w.rt * TR + f * 8 + 2 * t4 + i;
+        lim[f][i] = row < w.r.rows ? min(w.r.kv, attn_limit(p, w.r, row)) : 0;
+        m[f][i] = most[f][i] = kNegInf;
+        l[f][i] = 0.f;
+      }
+      const int row = w.rt * TR + f * 8 + g;
+      const bool live = row < w.r.rows;
+      const int tok = live ? row / p.group : 0, hd = w.h * p.group + (live ? row % p.group : 0);
+      const char* src = p.q + (int64_t)(w.r.q0 + tok) * p.ld_q + (int64_t)hd * p.kv.dim * 2;
+#pragma unroll
+      for (int ks = 0; ks < DP / 16; ++ks) {
+        const int d = ks * 16 + 2 * t4;
+        qf[ks][f][0] = live && d < p.kv.dim ? *reinterpret_cast<const uint32_t*>(src + d * 2) : 0u;
+        qf[ks][f][1] = live && d + 8 < p.kv.dim ? *reinterpret_cast<const uint32_t*>(src + d * 2 + 16) : 0u;
+        o[ks][f][0] = o[ks][f][1] = o[ks][f][2] = o[ks][f][3] = 0.f;
+      }
+    }
+  };
+  open_tile();
+  // this lane's ldmatrix rows, four 16-element steps of 128 bytes each
+  uint32_t k_off[4], v_off[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    k_off[i] = chunk_addr<DP>(0, warp * 16 + (lane & 15), i * 2 + (lane >> 4));
+    v_off[i] = chunk_addr<DP>(0, warp * 16 + (lane & 7) + (lane >> 4) * 8, i * 2 + ((lane >> 3) & 1));
+  }
+
+  int stage = 0;
+  for (int64_t u = u0; u < u1; ++u) {
+    cp_async_wait<S::kStages - 2>();
+    __syncwarp();
+    const uint32_t kt = ring + stage * 2 * S::kTileBytes, vt = kt + S::kTileBytes;
+    const int ahead = stage == 0 ? S::kStages - 1 : stage - 1;      // the stage computed with last
+    stage = stage + 1 == S::kStages ? 0 : stage + 1;
+    ld.load(p, ring + ahead * 2 * S::kTileBytes);
+
+    // S^T; for eight rows in two chains, as one would wait for its own products
+    constexpr int kChains = NQ == 1 ? 2 : 1;
+    float s[NQ * kChains][4];
+    uint32_t a[kAhead][4];             // 16 keys x 16 elements, fetched kAhead steps ahead
+#pragma unroll
+    for (int ks = 0; ks < kAhead; ++ks) ldsm4(kt + k_off[ks & 3] + (ks >> 2) * 128, a[ks]);
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) {
+#pragma unroll
+      for (int f = 0; f < NQ; ++f) {
+        if (ks < kChains) mma16816<T, true>(s[f + ks % kChains], a[ks % kAhead], qf[ks][f][0], qf[ks][f][1]);
+        else mma16816<T>(s[f + ks % kChains], a[ks % kAhead], qf[ks][f][0], qf[ks][f][1]);
+      }
+      const int next = ks + kAhead;    // then the values: 16 elements x 16 keys
+      if (next < DP / 16) ldsm4(kt + k_off[next & 3] + (next >> 2) * 128, a[ks % kAhead]);
+      else ldsm4_t(vt + v_off[(next - DP / 16) & 3], a[ks % kAhead]);
+    }
+    if (kChains == 2) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[0][i] += s[NQ * kChains - 1][i];
+    }
+    // element i: row 2 t4 + (i & 1), key g + 8 (i >> 1)
+    const int key0 = w.kb * kKeys + warp * 16;
+    if (key0 + 16 > lim_all) {
+#pragma unroll
+      for (int f = 0; f < NQ; ++f)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (key0 + g + 8 * (i >> 1) >= lim[f][i & 1]) s[f][i] = kNegInf;
+    }
+    bool raise = false;
+#pragma unroll
+    for (int f = 0; f < NQ; ++f)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) raise |= s[f][i] > most[f][i & 1];
+    if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+      for (int f = 0; f < NQ; ++f)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float top = fmaxf(s[f][i], s[f][i + 2]);
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+          top *= p.scale_log2;
+          if (top > m[f][i]) {
+            const float e = exp2_fast(m[f][i] - top);   // m = -inf: 0
+            m[f][i] = top;
+            most[f][i] = (top + kRaise) / p.scale_log2;
+            l[f][i] *= e;
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d) {
+              o[d][f][i] *= e;
+              o[d][f][i + 2] *= e;
+            }
+          }
+        }
+    }
+    uint32_t b[NQ][2];                 // P^T: 16 keys x 8 rows
+#pragma unroll
+    for (int f = 0; f < NQ; ++f) {
+      const float less[2] = {m[f][0] == kNegInf ? 0.f : Num<T>::kBias - m[f][0],
+                             m[f][1] == kNegInf ? 0.f : Num<T>::kBias - m[f][1]};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[f][i] = exp2_fast(fmaf(s[f][i], p.scale_log2, less[i & 1]));
+        l[f][i & 1] += s[f][i];
+      }
+      b[f][0] = transpose8(Num<T>::pack(s[f][0], s[f][1]));
+      b[f][1] = transpose8(Num<T>::pack(s[f][2], s[f][3]));
+    }
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) {
+#pragma unroll
+      for (int f = 0; f < NQ; ++f) mma16816<T>(o[d][f], a[d % kAhead], b[f][0], b[f][1]);
+      const int next = d + kAhead;
+      if (next < DP / 16) ldsm4_t(vt + v_off[next & 3] + (next >> 2) * 128, a[d % kAhead]);
+    }
+
+    // ---- end of the tile, or of this CTA's share of it
+    const bool last = w.kb + 1 == w.nkb;
+    if (!last && u + 1 < u1) {
+      ++w.kb;
+      continue;
+    }
+    const bool whole = last && tile_kb0 == 0;
+    // slot 0: a tile entered in the middle; slot 1: a tile left unfinished
+    const int64_t slot = 2 * (int64_t)blockIdx.x + (tile_kb0 == 0 ? 1 : 0);
+#pragma unroll
+    for (int f = 0; f < NQ; ++f) {
+      const int rows = w.r.rows - w.rt * TR - f * 8;   // rows from these eight on
+      if (rows <= 0) break;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) l[f][i] += __shfl_xor_sync(0xffffffffu, l[f][i], off);
+      // merge the warps: their common maximum, then the contexts added up in a
+      // fixed order
+      if (g == 0) *reinterpret_cast<float2*>(&merge_m[warp][2 * t4]) = make_float2(m[f][0], m[f][1]);
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float top = merge_m[0][2 * t4 + i];
+#pragma unroll
+        for (int ww = 1; ww < kWarps; ++ww) top = fmaxf(top, merge_m[ww][2 * t4 + i]);
+        const float e = m[f][i] == kNegInf ? 0.f : exp2_fast(m[f][i] - top);
+        l[f][i] *= e;
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d) {
+          o[d][f][i] *= e;
+          o[d][f][i + 2] *= e;
+        }
+      }
+      if (g == 0) *reinterpret_cast<float2*>(&merge_l[warp][2 * t4]) = make_float2(l[f][0], l[f][1]);
+      // warps 2 and 3 leave theirs in a buffer each, warps 0 and 1 add their
+      // own; a row's pitch of DP + 4 puts a store's 4 rows on different banks
+      static_assert(kWarps == 4, "merge order");
+#pragma unroll
+      for (int step = 0; step < 2; ++step) {
+        if ((warp >> 1) != step) {
+          float* mine = merge + (warp & 1) * 8 * S::kPitch + 2 * t4 * S::kPitch + g;
+#pragma unroll
+          for (int d = 0; d < DP / 16; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float* dst = mine + (i & 1) * S::kPitch + d * 16 + (i >> 1) * 8;
+              *dst = step ? *dst + o[d][f][i] : o[d][f][i];
+            }
+        }
+        __syncthreads();
+      }
+      for (int c = threadIdx.x; c < 8 * (DP / 8); c += kThreads) {
+        const int r = c / (DP / 8), d8 = c % (DP / 8);
+        if (r >= rows) break;
+        const float4* src = reinterpret_cast<const float4*>(merge + r * S::kPitch + d8 * 8);
+        float4 a = src[0], b4 = src[1];
+        const float4 a1 = src[8 * S::kPitch / 4], b1 = src[8 * S::kPitch / 4 + 1];
+        a = make_float4(a.x + a1.x, a.y + a1.y, a.z + a1.z, a.w + a1.w);
+        b4 = make_float4(b4.x + b1.x, b4.y + b1.y, b4.z + b1.z, b4.w + b1.w);
+        const float sum = merge_l[0][r] + merge_l[1][r] + merge_l[2][r] + merge_l[3][r];
+        const int row = w.rt * TR + f * 8 + r;
+        if (whole) {
+          const float inv = row_scale<T>(sum);
+          const int tok = row / p.group, hd = w.h * p.group + row % p.group;
+          if (d8 * 8 < p.kv.dim)
+            *reinterpret_cast<uint4*>(p.out + (int64_t)(w.r.q0 + tok) * p.ld_out + ((int64_t)hd * p.kv.dim + d8 * 8) * 2) =
+                make_uint4(Num<T>::pack(a.x * inv, a.y * inv), Num<T>::pack(a.z * inv, a.w * inv),
+                           Num<T>::pack(b4.x * inv, b4.y * inv), Num<T>::pack(b4.z * inv, b4.w * inv));
+        } else {
+          float4* dst = reinterpret_cast<float4*>(p.part_o + (slot * TR + f * 8 + r) * DP + d8 * 8);
+          dst[0] = a;
+          dst[1] = b4;
+          if (d8 == 0) {
+            const float top = fmaxf(fmaxf(merge_m[0][r], merge_m[1][r]), fmaxf(merge_m[2][r], merge_m[3][r]));
+            p.part_ml[slot * TR + f * 8 + r] = make_float2(top, sum);
+          }
+        }
+      }
+      __syncthreads();
+    }
+    if (!whole && threadIdx.x == 0) attn_leave_part(p, w, tile_kb0 == 0, last);
+    if (u + 1 < u1) {
+      attn_next_tile<TR, kKeys>(p, w);
+      open_tile();
+    }
+  }
+  cp_async_wait<0>();
+}
+
+// ---- more rows, head_dim above 128 ----------------------------------------------
+// Tiles of 64 rows, 16 a warp, every warp through all keys of a block; the
+// query tile stays in shared memory (its fragments would take the registers
+// that the context needs).
+template <int DP>
+constexpr size_t mid_smem() {
+  using S = Shape<DP>;
+  return (size_t)S::kStages * 2 * S::kTileBytes + 64 * DP * 2;
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_mid_kernel(const AttnParams p) {
+  using S = Shape<DP>;
+  constexpr int TR = 64, kChunks = DP / 8;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ AttnShare share;
+  __shared__ int64_t warp_sum[kWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t ring = smem_addr(smem);
+  uint8_t* q_tile = smem + (size_t)S::kStages * 2 * S::kTileBytes;
+  const uint32_t q_smem = smem_addr(q_tile);
 
   pdl_wait();
   attn_share<TR, kKeys, kThreads>(p, &share, warp_sum);
@@ -108,332 +459,153 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_kernel
   if (threadIdx.x == 0) attn_no_parts(p);
   if (u1 <= u0) return;
 
-  // ---- loading: `ld` walks ahead of the computation
-  AttnPos ld;
-  attn_open<TR, kKeys>(p, share, ld);
-  AttnPos w = ld;
-  int64_t to_load = u1 - u0;
-  const int page_mask = (1 << p.kv.page_log2) - 1;
-  int page = -1;                                  // page of this lane's key in block `ld`
-  auto look_up = [&]() {
-    const int key = ld.kb * kKeys + warp * 16 + (lane & 15);
-    page = key < ld.r.kv ? p.table[(int64_t)ld.b * p.ld_table + (key >> p.kv.page_log2)] : -1;
-    if (key < ld.r.kv && (page < 0 || page >= p.kv.n_pages)) {
-      raise_device_error(p.err, kDevErrBadIndex);
-      page = -1;
-    }
-  };
-  auto load_block = [&](int stage) {
-    if (to_load > 0) {
-      const int key = ld.kb * kKeys + warp * 16 + (lane & 15);
-      // byte offset of this lane's key row, or -1: nothing there, zeros instead
-      const int64_t off = page < 0 ? -1
-                                   : page * p.kv.page_bytes + (key & page_mask) * p.kv.token_bytes +
-                                         ld.h * p.kv.head_bytes;
-      const uint32_t kt = ring + (stage * 2) * S::kTileBytes, vt = kt + S::kTileBytes;
-      constexpr int kPer = 16 * kChunks / 32;     // chunks a lane copies of K, and of V
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const int c = i * 32 + lane, row = c / kChunks, col = c % kChunks;
-        const int64_t o = __shfl_sync(0xffffffffu, off, row);
-        const int n = o >= 0 && col * 8 < p.kv.dim ? 16 : 0;
-        const int64_t at = n ? o + col * 16 : 0;
-        const int r = warp * 16 + row;
-        cp_async16(chunk_addr<DP>(kt, r, col), p.kv.k + at, n);
-        cp_async16(chunk_addr<DP>(vt, r, col), p.kv.v + at, n);
-      }
-      if (--to_load > 0) {
-        if (++ld.kb == ld.nkb) attn_next_tile<TR, kKeys>(p, ld);
-        look_up();
-      }
-    }
-    cp_async_commit();
-  };
-  look_up();
-  for (int s = 0; s < S::kStages - 1; ++s) load_block(s);
+  AttnPos w;
+  attn_open<TR, kKeys>(p, share, w);
+  Loader<DP, TR> ld;
+  ld.open(p, w, u1 - u0);
+  for (int s = 0; s < S::kStages - 1; ++s) ld.load(p, ring + s * 2 * S::kTileBytes);
 
-  // ---- computing
   const int g = lane >> 2, t4 = lane & 3;
-  uint32_t qf[kQRegs ? DP / 16 : 1][M][4];
-  float o[M][DP / 8][4];
-  float m[M][2], l[M][2];
-  int lim[M][2], lim_all = 0;
+  float o[DP / 8][4];
+  float m[2], l[2];
+  int lim[2], lim_all = 0;
   int tile_kb0 = w.kb;
-  // rows of this lane in fragment f: f * 16 + g and f * 16 + g + 8 of the warp's
-  const int row_in = (kRowSplit ? warp * 16 : 0) + g;
   auto open_tile = [&]() {
     tile_kb0 = w.kb;
     lim_all = min(w.r.kv, attn_limit(p, w.r, w.rt * TR));
 #pragma unroll
-    for (int f = 0; f < M; ++f) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int row = w.rt * TR + row_in + f * 16 + 8 * i;
-        lim[f][i] = row < w.r.rows ? min(w.r.kv, attn_limit(p, w.r, row)) : 0;
-        m[f][i] = kNegInf;
-        l[f][i] = 0.f;
-      }
-#pragma unroll
-      for (int d = 0; d < DP / 8; ++d) o[f][d][0] = o[f][d][1] = o[f][d][2] = o[f][d][3] = 0.f;
+    for (int i = 0; i < 2; ++i) {
+      const int row = w.rt * TR + warp * 16 + g + 8 * i;
+      lim[i] = row < w.r.rows ? min(w.r.kv, attn_limit(p, w.r, row)) : 0;
+      m[i] = kNegInf;
+      l[i] = 0.f;
     }
-    auto q_row = [&](int row) -> const char* {
-      const int tok = row / p.group, hd = w.h * p.group + row % p.group;
-      return p.q + (int64_t)(w.r.q0 + tok) * p.ld_q + (int64_t)hd * p.kv.dim * 2;
-    };
-    if (kQRegs) {
 #pragma unroll
-      for (int f = 0; f < M; ++f)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int row = w.rt * TR + row_in + f * 16 + 8 * i;
-          const bool live = row < w.r.rows;
-          const char* src = q_row(live ? row : 0);
-#pragma unroll
-          for (int ks = 0; ks < DP / 16; ++ks) {
-            const int d = ks * 16 + 2 * t4;
-            qf[kQRegs ? ks : 0][f][i] = live && d < p.kv.dim ? *reinterpret_cast<const uint32_t*>(src + d * 2) : 0u;
-            qf[kQRegs ? ks : 0][f][i + 2] =
-                live && d + 8 < p.kv.dim ? *reinterpret_cast<const uint32_t*>(src + d * 2 + 16) : 0u;
-          }
-        }
-    } else {
-      // the query tile in shared memory, in the layout of the keys
-      __syncthreads();
-      for (int c = threadIdx.x; c < TR * kChunks; c += kThreads) {
-        const int r = c / kChunks, col = c % kChunks, row = w.rt * TR + r;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (row < w.r.rows && col * 8 < p.kv.dim) v = *reinterpret_cast<const uint4*>(q_row(row) + col * 16);
-        *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(merge) + (chunk_addr<DP>(0, r, col))) = v;
+    for (int d = 0; d < DP / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
+    // the query tile, in the layout of the keys
+    __syncthreads();
+    for (int c = threadIdx.x; c < TR * kChunks; c += kThreads) {
+      const int r = c / kChunks, col = c % kChunks, row = w.rt * TR + r;
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (row < w.r.rows && col * 8 < p.kv.dim) {
+        const int tok = row / p.group, hd = w.h * p.group + row % p.group;
+        v = *reinterpret_cast<const uint4*>(p.q + (int64_t)(w.r.q0 + tok) * p.ld_q + ((int64_t)hd * p.kv.dim + col * 8) * 2);
       }
-      __syncthreads();
+      *reinterpret_cast<uint4*>(q_tile + chunk_addr<DP>(0, r, col)) = v;
     }
+    __syncthreads();
   };
   open_tile();
 
+  int stage = 0;
   for (int64_t u = u0; u < u1; ++u) {
-    const int stage = (int)((u - u0) % S::kStages);
     cp_async_wait<S::kStages - 2>();
-    if (kRowSplit) __syncthreads();
-    else __syncwarp();
-    load_block((int)((u - u0 + S::kStages - 1) % S::kStages));
+    __syncthreads();
+    const uint32_t kt = ring + stage * 2 * S::kTileBytes, vt = kt + S::kTileBytes;
+    const int ahead = stage == 0 ? S::kStages - 1 : stage - 1;
+    stage = stage + 1 == S::kStages ? 0 : stage + 1;
+    ld.load(p, ring + ahead * 2 * S::kTileBytes);
 
-    const uint32_t kt = ring + (stage * 2) * S::kTileBytes, vt = kt + S::kTileBytes;
-    const int krow0 = kRowSplit ? 0 : warp * 16;    // first of this warp's keys in the block
-    float s[M][NK / 8][4];
+    float s[kKeys / 8][4];
 #pragma unroll
-    for (int f = 0; f < M; ++f)
-#pragma unroll
-      for (int n = 0; n < NK / 8; ++n) s[f][n][0] = s[f][n][1] = s[f][n][2] = s[f][n][3] = 0.f;
+    for (int n = 0; n < kKeys / 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
     for (int ks = 0; ks < DP / 16; ++ks) {
-      uint32_t a[M][4];
+      uint32_t a[4];
+      ldsm4(chunk_addr<DP>(q_smem, warp * 16 + (lane & 15), ks * 2 + (lane >> 4)), a);
 #pragma unroll
-      for (int f = 0; f < M; ++f) {
-        if (kQRegs) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) a[f][i] = qf[kQRegs ? ks : 0][f][i];
-        } else {
-          const int r = (kRowSplit ? warp * 16 : f * 16) + (lane & 7) + ((lane >> 3) & 1) * 8;
-          ldsm4(chunk_addr<DP>(q_smem, r, ks * 2 + (lane >> 4)), a[f]);
-        }
-      }
-#pragma unroll
-      for (int n2 = 0; n2 < NK / 16; ++n2) {
+      for (int n2 = 0; n2 < kKeys / 16; ++n2) {
         uint32_t b[4];
-        const int r = krow0 + n2 * 16 + (lane & 7) + ((lane >> 4) & 1) * 8;
-        ldsm4(chunk_addr<DP>(kt, r, ks * 2 + ((lane >> 3) & 1)), b);
-#pragma unroll
-        for (int f = 0; f < M; ++f) {
-          mma16816<T>(s[f][2 * n2], a[f], b[0], b[1]);
-          mma16816<T>(s[f][2 * n2 + 1], a[f], b[2], b[3]);
-        }
+        ldsm4(chunk_addr<DP>(kt, n2 * 16 + (lane & 7) + (lane >> 4) * 8, ks * 2 + ((lane >> 3) & 1)), b);
+        mma16816<T>(s[2 * n2], a, b[0], b[1]);
+        mma16816<T>(s[2 * n2 + 1], a, b[2], b[3]);
       }
     }
-    const int key0 = w.kb * kKeys + krow0;
-    const bool masked = key0 + NK > lim_all;
+    const int key0 = w.kb * kKeys;
+    const bool masked = key0 + kKeys > lim_all;
+    float mx[2] = {kNegInf, kNegInf};
 #pragma unroll
-    for (int f = 0; f < M; ++f) {
-      float mx[2] = {kNegInf, kNegInf};
+    for (int n = 0; n < kKeys / 8; ++n)
 #pragma unroll
-      for (int n = 0; n < NK / 8; ++n)
+      for (int i = 0; i < 4; ++i) {
+        if (masked && key0 + n * 8 + 2 * t4 + (i & 1) >= lim[i >> 1]) s[n][i] = kNegInf;
+        mx[i >> 1] = fmaxf(mx[i >> 1], s[n][i]);
+      }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (masked && key0 + n * 8 + 2 * t4 + (i & 1) >= lim[f][i >> 1]) s[f][n][i] = kNegInf;
-          mx[i >> 1] = fmaxf(mx[i >> 1], s[f][n][i]);
-        }
+    for (int i = 0; i < 2; ++i) {
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+      mx[i] = fmaxf(m[i], mx[i] * p.scale_log2);
+    }
+    if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
-        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-        mx[i] = fmaxf(m[f][i], mx[i] * p.scale_log2);
-      }
-      if (__any_sync(0xffffffffu, mx[0] > m[f][0] || mx[1] > m[f][1])) {
+        const float e = mx[i] > m[i] ? exp2_fast(m[i] - mx[i]) : 1.f;   // m = -inf: 0
+        m[i] = mx[i];
+        l[i] *= e;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float e = mx[i] > m[f][i] ? exp2_fast(m[f][i] - mx[i]) : 1.f;   // m = -inf: 0
-          m[f][i] = mx[i];
-          l[f][i] *= e;
-#pragma unroll
-          for (int d = 0; d < DP / 8; ++d) {
-            o[f][d][2 * i] *= e;
-            o[f][d][2 * i + 1] *= e;
-          }
+        for (int d = 0; d < DP / 8; ++d) {
+          o[d][2 * i] *= e;
+          o[d][2 * i + 1] *= e;
         }
       }
-      const float sub[2] = {m[f][0] == kNegInf ? 0.f : Num<T>::kBias - m[f][0],
-                            m[f][1] == kNegInf ? 0.f : Num<T>::kBias - m[f][1]};
-#pragma unroll
-      for (int n = 0; n < NK / 8; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[f][n][i] = exp2_fast(fmaf(s[f][n][i], p.scale_log2, sub[i >> 1]));
-          l[f][i >> 1] += s[f][n][i];
-        }
     }
+    const float sub[2] = {m[0] == kNegInf ? 0.f : Num<T>::kBias - m[0], m[1] == kNegInf ? 0.f : Num<T>::kBias - m[1]};
 #pragma unroll
-    for (int k2 = 0; k2 < NK / 16; ++k2) {
-      uint32_t a[M][4];
+    for (int n = 0; n < kKeys / 8; ++n)
 #pragma unroll
-      for (int f = 0; f < M; ++f)
+      for (int i = 0; i < 4; ++i) {
+        s[n][i] = exp2_fast(fmaf(s[n][i], p.scale_log2, sub[i >> 1]));
+        l[i >> 1] += s[n][i];
+      }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          a[f][i] = Num<T>::pack(s[f][2 * k2 + (i >> 1)][2 * (i & 1)], s[f][2 * k2 + (i >> 1)][2 * (i & 1) + 1]);
+    for (int k2 = 0; k2 < kKeys / 16; ++k2) {
+      uint32_t a[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = Num<T>::pack(s[2 * k2 + (i >> 1)][2 * (i & 1)], s[2 * k2 + (i >> 1)][2 * (i & 1) + 1]);
 #pragma unroll
       for (int d2 = 0; d2 < DP / 16; ++d2) {
         uint32_t b[4];
-        const int r = krow0 + k2 * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
-        ldsm4_t(chunk_addr<DP>(vt, r, d2 * 2 + (lane >> 4)), b);
-#pragma unroll
-        for (int f = 0; f < M; ++f) {
-          mma16816<T>(o[f][2 * d2], a[f], b[0], b[1]);
-          mma16816<T>(o[f][2 * d2 + 1], a[f], b[2], b[3]);
-        }
+        ldsm4_t(chunk_addr<DP>(vt, k2 * 16 + (lane & 15), d2 * 2 + (lane >> 4)), b);
+        mma16816<T>(o[2 * d2], a, b[0], b[1]);
+        mma16816<T>(o[2 * d2 + 1], a, b[2], b[3]);
       }
     }
 
     // ---- end of the tile, or of this CTA's share of it
     const bool last = w.kb + 1 == w.nkb;
-    if (last || u + 1 == u1) {
-      const bool whole = last && tile_kb0 == 0;
-      // slot 0: a tile entered in the middle; slot 1: a tile left unfinished
-      const int64_t slot = 2 * (int64_t)blockIdx.x + (tile_kb0 == 0 ? 1 : 0);
-      auto out_row = [&](int row) -> char* {
-        const int tok = row / p.group, hd = w.h * p.group + row % p.group;
-        return p.out + (int64_t)(w.r.q0 + tok) * p.ld_out + (int64_t)hd * p.kv.dim * 2;
-      };
-#pragma unroll
-      for (int f = 0; f < M; ++f) {
-        const int frag_rows = w.r.rows - w.rt * TR - f * 16;   // rows from this fragment on
-        if (!kRowSplit && frag_rows <= 0) break;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          l[f][i] += __shfl_xor_sync(0xffffffffu, l[f][i], 1);
-          l[f][i] += __shfl_xor_sync(0xffffffffu, l[f][i], 2);
-        }
-        if (kRowSplit) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int r = row_in + 8 * i, row = w.rt * TR + r;
-            if (row >= w.r.rows) continue;
-            if (whole) {
-              const float inv = l[f][i] > 0.f ? 1.f / l[f][i] : (l[f][i] == 0.f ? 0.f : l[f][i]);
-              char* dst = out_row(row);
-#pragma unroll
-              for (int d = 0; d < DP / 8; ++d)
-                if (d * 8 < p.kv.dim)
-                  *reinterpret_cast<uint32_t*>(dst + (d * 8 + 2 * t4) * 2) =
-                      Num<T>::pack(o[f][d][2 * i] * inv, o[f][d][2 * i + 1] * inv);
-            } else {
-              float* dst = p.part_o + (slot * TR + r) * DP;
-#pragma unroll
-              for (int d = 0; d < DP / 8; ++d)
-                *reinterpret_cast<float2*>(dst + d * 8 + 2 * t4) = make_float2(o[f][d][2 * i], o[f][d][2 * i + 1]);
-              if (t4 == 0) p.part_ml[slot * TR + r] = make_float2(m[f][i], l[f][i]);
-            }
-          }
-          continue;
-        }
-        // merge the warps: their common maximum, then the contexts added up in
-        // a fixed order
-        if (t4 == 0) {
-          merge_m[warp][g] = m[f][0];
-          merge_m[warp][g + 8] = m[f][1];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float top = merge_m[0][g + 8 * i];
-#pragma unroll
-          for (int ww = 1; ww < kWarps; ++ww) top = fmaxf(top, merge_m[ww][g + 8 * i]);
-          const float e = m[f][i] == kNegInf ? 0.f : exp2_fast(m[f][i] - top);
-          l[f][i] *= e;
-#pragma unroll
-          for (int d = 0; d < DP / 8; ++d) {
-            o[f][d][2 * i] *= e;
-            o[f][d][2 * i + 1] *= e;
-          }
-        }
-        if (t4 == 0) {
-          merge_l[warp][g] = l[f][0];
-          merge_l[warp][g + 8] = l[f][1];
-        }
-        // warps 2 and 3 leave theirs in a buffer each, warps 0 and 1 add their own
-        static_assert(kWarps == 4, "merge order");
-#pragma unroll
-        for (int step = 0; step < 2; ++step) {
-          if ((warp >> 1) != step) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-              for (int d = 0; d < DP / 8; ++d) {
-                // columns XORed with the row, so that the eight rows of a store take different banks
-                float2* dst = reinterpret_cast<float2*>(merge + (warp & 1) * 16 * DP + (g + 8 * i) * DP +
-                                                        ((d * 8 + 2 * t4) ^ (g * 8)));
-                float2 v = make_float2(o[f][d][2 * i], o[f][d][2 * i + 1]);
-                if (step) {
-                  const float2 old = *dst;
-                  v.x = old.x + v.x;
-                  v.y = old.y + v.y;
-                }
-                *dst = v;
-              }
-          }
-          __syncthreads();
-        }
-        for (int c = threadIdx.x; c < 16 * (DP / 8); c += kThreads) {
-          const int r = c / (DP / 8), d8 = c % (DP / 8);
-          if (r >= frag_rows) break;
-          const float4* src = reinterpret_cast<const float4*>(merge + r * DP + ((d8 * 8) ^ ((r & 7) * 8)));
-          float4 a = src[0], b = src[1];
-          const float4 a1 = src[16 * DP / 4], b1 = src[16 * DP / 4 + 1];
-          a = make_float4(a.x + a1.x, a.y + a1.y, a.z + a1.z, a.w + a1.w);
-          b = make_float4(b.x + b1.x, b.y + b1.y, b.z + b1.z, b.w + b1.w);
-          const float sum = merge_l[0][r] + merge_l[1][r] + merge_l[2][r] + merge_l[3][r];
-          if (whole) {
-            const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
-            if (d8 * 8 < p.kv.dim)
-              *reinterpret_cast<uint4*>(out_row(w.rt * TR + f * 16 + r) + d8 * 16) =
-                  make_uint4(Num<T>::pack(a.x * inv, a.y * inv), Num<T>::pack(a.z * inv, a.w * inv),
-                             Num<T>::pack(b.x * inv, b.y * inv), Num<T>::pack(b.z * inv, b.w * inv));
-          } else {
-            float4* dst = reinterpret_cast<float4*>(p.part_o + (slot * TR + f * 16 + r) * DP + d8 * 8);
-            dst[0] = a;
-            dst[1] = b;
-            if (d8 == 0) {
-              const float top_m = fmaxf(fmaxf(merge_m[0][r], merge_m[1][r]), fmaxf(merge_m[2][r], merge_m[3][r]));
-              p.part_ml[slot * TR + f * 16 + r] = make_float2(top_m, sum);
-            }
-          }
-        }
-        __syncthreads();
-      }
-      if (!whole && threadIdx.x == 0) attn_leave_part(p, w, tile_kb0 == 0, last);
-      if (u + 1 < u1) {
-        attn_next_tile<TR, kKeys>(p, w);
-        open_tile();
-      }
-    } else {
+    if (!last && u + 1 < u1) {
       ++w.kb;
+      continue;
+    }
+    const bool whole = last && tile_kb0 == 0;
+    const int64_t slot = 2 * (int64_t)blockIdx.x + (tile_kb0 == 0 ? 1 : 0);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+      const int r = warp * 16 + g + 8 * i, row = w.rt * TR + r;
+      if (row < w.r.rows && whole) {
+        const float inv = row_scale<T>(l[i]);
+        const int tok = row / p.group, hd = w.h * p.group + row % p.group;
+        char* dst = p.out + (int64_t)(w.r.q0 + tok) * p.ld_out + (int64_t)hd * p.kv.dim * 2;
+#pragma unroll
+        for (int d = 0; d < DP / 8; ++d)
+          if (d * 8 < p.kv.dim)
+            *reinterpret_cast<uint32_t*>(dst + (d * 8 + 2 * t4) * 2) = Num<T>::pack(o[d][2 * i] * inv, o[d][2 * i + 1] * inv);
+      } else if (row < w.r.rows) {
+        float* dst = p.part_o + (slot * TR + r) * DP;
+#pragma unroll
+        for (int d = 0; d < DP / 8; ++d)
+          *reinterpret_cast<float2*>(dst + d * 8 + 2 * t4) = make_float2(o[d][2 * i], o[d][2 * i + 1]);
+        if (t4 == 0) p.part_ml[slot * TR + r] = make_float2(m[i], l[i]);
+      }
+      __syncwarp();
+    }
+    if (!whole && threadIdx.x == 0) attn_leave_part(p, w, tile_kb0 == 0, last);
+    if (u + 1 < u1) {
+      attn_next_tile<TR, kKeys>(p, w);
+      open_tile();
     }
   }
   cp_async_wait<0>();
@@ -467,6 +639,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) paged_attn_join_kernel(const 
     const int o = c + 1 + i * 32 + lane;
     st[i] = o < ctas ? p.state[o] : kPartEnds;                // the last CTA ends the line
   }
+  pdl_trigger();
   if (hd.x < 0) return;
   int n = 0;
 #pragma unroll
@@ -531,7 +704,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) paged_attn_join_kernel(const 
     }
   }
   if (row_t >= rows) return;
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  const float inv = row_scale<T>(l);
   const int row = row0 + row_t, tok = row / p.group, head = hd.w * p.group + row % p.group;
   char* dst = p.out + (int64_t)(hd.x + tok) * p.ld_out + (int64_t)head * p.kv.dim * 2;
 #pragma unroll
@@ -541,13 +714,20 @@ __global__ void __launch_bounds__(32 * kJoinWarps) paged_attn_join_kernel(const 
   }
 }
 
-template <typename T, int DP, int MT>
+// TR rows a tile: 8 to 32 on the few-row kernel, 64 on the other.
+template <typename T, int DP, int TR>
 int run_class(AttnParams p, const PagedAttention& a, int sms, cudaStream_t stream) {
-  constexpr int TR = MT == 0 ? 64 : 16 * MT;
   const int ctas = sms * Shape<DP>::kPerSm;
   attn_carve<TR, DP>(p, a.workspace, ctas);
-  constexpr size_t smem = smem_bytes<DP, MT>();
-  auto kernel = paged_attn_kernel<T, DP, MT>;
+  void (*kernel)(AttnParams);
+  size_t smem;
+  if constexpr (TR == 64) {
+    kernel = paged_attn_mid_kernel<T, DP>;
+    smem = mid_smem<DP>();
+  } else {
+    kernel = paged_attn_few_kernel<T, DP, TR / 8>;
+    smem = few_smem<DP>();
+  }
   SMEAI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   SMEAI_CUDA_TRY(launch(kernel, dim3((unsigned)ctas), dim3(kThreads), smem, stream, p));
   // a tile of up to 2 * kSnap blocks is never split
@@ -557,27 +737,29 @@ int run_class(AttnParams p, const PagedAttention& a, int sms, cudaStream_t strea
 
 // Which kernels a call needs, from what the host knows: the largest request's
 // packed rows and the total.
-//   up to 16 rows   16-row tiles
-//   up to 32        32-row tiles: one reading of the keys for all rows
-//   more            the tensor-core kernel, and the 16-row tiles beside it for
-//                   requests of up to 16 rows (a step that mixes prompts and
-//                   decoding) unless the total says that there are none: one
-//                   row costs the tensor-core kernel's tile as much as 256,
-//                   and 8 requests, one of 860 rows, took 148 us without the
-//                   second kernel and 104 us with it
+//   up to 8, 16, 24, 32 rows  tiles of so many: one reading of the keys for all
+//   more                  the tensor-core kernel, and the 16-row tiles beside it
+//                         for requests of up to 16 rows (a step that mixes
+//                         prompts and decoding) unless the total says that
+//                         there are none: one row costs the tensor-core
+//                         kernel's tile as much as 128, and 8 requests, one of
+//                         860 rows, took 148 us without the second kernel and
+//                         104 us with it
 // head_dim above 128: up to 16 rows as above, more the 64-row tiles for all.
 struct Classes {
-  bool few, mid, many;
+  int few;      // rows a tile of the few-row kernel; 0: not needed
+  bool mid, many;
 };
 Classes classes(const PagedAttention& a) {
   const int64_t group = a.n_heads / a.kv.n_kv, most = a.max_new * group;
-  Classes c = {false, false, false};
-  if (most <= 16) c.few = true;
-  else if (most <= 32 || a.kv.dim > 128) c.mid = true;
+  Classes c = {0, false, false};
+  if (most <= 16) c.few = most <= 8 ? 8 : 16;
+  else if (a.kv.dim > 128) c.mid = true;
+  else if (most <= 32) c.few = most <= 24 ? 24 : 32;
   else {
     c.many = true;
     // with one request of r <= 16 / group rows the others, of max_new at most, could not make up n_tokens
-    c.few = a.n_tokens <= (a.n_req - 1) * a.max_new + 16 / group;
+    if (a.n_tokens <= (a.n_req - 1) * a.max_new + 16 / group) c.few = 16;
   }
   return c;
 }
@@ -590,16 +772,19 @@ int run_dim(const AttnParams& p, const PagedAttention& a, int sms, cudaStream_t 
   if (c.few) {
     AttnParams q = p;
     if (c.many) q.rows_hi = 16;
-    const int st = run_class<T, DP, 1>(q, a, sms, stream);
+    int st;
+    if (c.few == 8) st = run_class<T, DP, 8>(q, a, sms, stream);
+    else if (DP > 128 || c.few == 16) st = run_class<T, DP, 16>(q, a, sms, stream);
+    else if (c.few == 24) st = run_class<T, DP, DP <= 128 ? 24 : 16>(q, a, sms, stream);
+    else st = run_class<T, DP, DP <= 128 ? 32 : 16>(q, a, sms, stream);
     if (st) return st;
   }
-  if (c.mid) return run_class<T, DP, DP <= 128 ? 2 : 0>(p, a, sms, stream);
-  if constexpr (DP <= 128) {
-    if (c.many) {
-      AttnParams q = p;
-      if (c.few) q.rows_lo = 16;
-      return paged_attn_tc(q, DP, a.workspace, a.max_kv, sms, stream);
-    }
+  if constexpr (DP > 128) {
+    if (c.mid) return run_class<T, DP, 64>(p, a, sms, stream);
+  } else if (c.many) {
+    AttnParams q = p;
+    if (c.few) q.rows_lo = 16;
+    return paged_attn_tc(q, DP, a.workspace, a.max_kv, sms, stream);
   }
   return kOk;
 }
@@ -622,12 +807,9 @@ size_t paged_attention_workspace(const PagedAttention& a) {
   const Classes c = classes(a);
   const int dp = padded_dim(a.kv.dim);
   if (c.many) return paged_attn_tc_workspace(dp, sms);   // the 16-row tiles' need is smaller
-  if (c.mid)
-    return dp == 64    ? attn_part_bytes<32, 64>(2 * sms)
-           : dp == 128 ? attn_part_bytes<32, 128>(2 * sms)
-                       : attn_part_bytes<64, 256>(sms);
-  return dp == 64    ? attn_part_bytes<16, 64>(2 * sms)
-         : dp == 128 ? attn_part_bytes<16, 128>(2 * sms)
+  if (c.mid) return attn_part_bytes<64, 256>(sms);
+  return dp == 64    ? attn_part_bytes<32, 64>(2 * sms)  // of 32 rows, whichever tile it is
+         : dp == 128 ? attn_part_bytes<32, 128>(2 * sms)
                      : attn_part_bytes<16, 256>(sms);
 }
 

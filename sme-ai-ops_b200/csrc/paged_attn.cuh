@@ -208,6 +208,7 @@ struct Num;
 template <>
 struct Num<__half> {
   static constexpr float kBias = 7.f;
+  static constexpr bool kIsBf16 = false;
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -217,6 +218,7 @@ struct Num<__half> {
 template <>
 struct Num<__nv_bfloat16> {
   static constexpr float kBias = 0.f;
+  static constexpr bool kIsBf16 = true;
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);

@@ -184,15 +184,6 @@ __host__ __device__ constexpr uint32_t idesc(bool bf16, int n, bool b_n_major) {
          ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
 
-template <typename T>
-struct IsBf16 {
-  static constexpr bool value = false;
-};
-template <>
-struct IsBf16<__nv_bfloat16> {
-  static constexpr bool value = true;
-};
-
 // One CTA's stretch of a tile: key blocks kb0 .. kb0 + n of it; half t works on
 // the first cnt[t] of them (causal: the lower rows see fewer keys).
 struct Stretch {
@@ -427,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
     // registers; one elected lane issues.
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp == kMmaWarp) {
-      constexpr uint32_t kQk = idesc(IsBf16<T>::value, kKB, false), kPv = idesc(IsBf16<T>::value, DP, true);
+      constexpr uint32_t kQk = idesc(Num<T>::kIsBf16, kKB, false), kPv = idesc(Num<T>::kIsBf16, DP, true);
       AttnPos w;
       attn_open<kTR, kKB>(p, share, w);
       int64_t left = units;
