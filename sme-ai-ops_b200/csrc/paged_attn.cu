@@ -58,14 +58,13 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 
 // Shared-memory layout: [stages][K, V][kKeys rows][DP] 16-bit, the 16-byte
 // chunks of a row XORed with the row's index mod 8, so that ldmatrix's eight
-// rows fall on different banks; then the merge buffer or the query tile.
+// rows fall on different banks; then the query tiles in the same layout.
 template <int DP>
 struct Shape {
   static constexpr int kRowBytes = DP * 2;
   static constexpr int kTileBytes = kKeys * kRowBytes;
   static constexpr int kStages = DP == 64 ? 6 : 3;      // 96 KB in flight (192 KB at DP 256)
   static constexpr int kPerSm = DP == 256 ? 1 : 2;      // CTAs an SM
-  static constexpr int kPitch = DP + 4;                 // floats a row of the merge buffer
 };
 
 template <int DP>
@@ -164,7 +163,8 @@ __device__ __forceinline__ float row_scale(float sum) {   // 0 rows for a sum of
 // queries would.  All rows meet every key, and each warp takes 16 of a block's
 // 64 keys, with its own ring of keys in shared memory: warps never wait for
 // one another before the tile's end, where their maxima, sums and contexts
-// are merged.  A row's maximum is only raised when a score passes it by more
+// are merged (through the ring stage that the tile's last block left).  The
+// next tile's queries are copied while a tile is worked on.  A row's maximum is only raised when a score passes it by more
 // than 2^8, so most blocks need a vote and no reduction over the keys.
 // Two CTAs an SM with 96 KB of keys and values in flight each cover HBM's
 // latency (44 GB/s x ~1 us = 44 KB an SM) through the ends of tiles; bound by
@@ -178,10 +178,10 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   return r;
 }
 
-template <int DP>
+template <int DP, int NQ>
 constexpr size_t few_smem() {
   using S = Shape<DP>;
-  return (size_t)S::kStages * 2 * S::kTileBytes + 2 * 8 * S::kPitch * sizeof(float);
+  return (size_t)S::kStages * 2 * S::kTileBytes + 2 * 8 * NQ * S::kRowBytes;
 }
 
 template <typename T, int DP, int NQ>
@@ -189,14 +189,15 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_few_ke
   using S = Shape<DP>;
   constexpr int TR = 8 * NQ;
   constexpr int kAhead = 4;          // ldmatrix in flight ahead of the products
+  constexpr int kChunks = DP / 8;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ AttnShare share;
-  __shared__ int64_t warp_sum[kWarps];
-  __shared__ float merge_m[kWarps][8], merge_l[kWarps][8];
+  __shared__ int64_t warp_sum[2 * kWarps];
+  __shared__ float merge_m[kWarps][TR], merge_l[kWarps][TR];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t4 = lane & 3;
   const uint32_t ring = smem_addr(smem);
-  float* merge = reinterpret_cast<float*>(smem + (size_t)S::kStages * 2 * S::kTileBytes);
+  const uint32_t q_tiles = ring + S::kStages * 2 * S::kTileBytes;
 
   // every CTA is resident: the kernel behind can only take what these free
   pdl_trigger();
@@ -206,10 +207,26 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_few_ke
   if (threadIdx.x == 0) attn_no_parts(p);
   if (u1 <= u0) return;
 
+  auto out_offset = [&](const AttnPos& at, int row) {   // head and token of a packed row
+    const int tok = row / p.group;
+    return make_int2(at.r.q0 + tok, at.h * p.group + row - tok * p.group);
+  };
+  // the query rows of a tile, into one of the two tiles; with the next commit group
+  auto load_queries = [&](const AttnPos& at, int which) {
+    for (int c = threadIdx.x; c < TR * kChunks; c += kThreads) {
+      const int r = c / kChunks, col = c % kChunks, row = at.rt * TR + r;
+      const bool there = row < at.r.rows && col * 8 < p.kv.dim;
+      const int2 to = out_offset(at, there ? row : 0);
+      cp_async16(chunk_addr<DP>(q_tiles + which * TR * S::kRowBytes, r, col),
+                 p.q + (there ? (int64_t)to.x * p.ld_q + ((int64_t)to.y * p.kv.dim + col * 8) * 2 : 0), there ? 16 : 0);
+    }
+  };
+
   AttnPos w;
   attn_open<TR, kKeys>(p, share, w);
   Loader<DP, TR> ld;
   ld.open(p, w, u1 - u0);
+  load_queries(w, 0);
   for (int s = 0; s < S::kStages - 1; ++s) ld.load(p, ring + s * 2 * S::kTileBytes);
 
   // Q^T fragments: row (n) g of each eight, elements (k) 2 t4 and 2 t4 + 8 on.
@@ -219,33 +236,9 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_few_ke
   float m[NQ][2], l[NQ][2];
   float most[NQ][2];                   // scores (before the scale) that leave the maximum as it is
   int lim[NQ][2], lim_all = 0;
-  int tile_kb0 = w.kb;
-  auto open_tile = [&]() {
-    tile_kb0 = w.kb;
-    lim_all = min(w.r.kv, attn_limit(p, w.r, w.rt * TR));
-#pragma unroll
-    for (int f = 0; f < NQ; ++f) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int row = w.rt * TR + f * 8 + 2 * t4 + i;
-        lim[f][i] = row < w.r.rows ? min(w.r.kv, attn_limit(p, w.r, row)) : 0;
-        m[f][i] = most[f][i] = kNegInf;
-        l[f][i] = 0.f;
-      }
-      const int row = w.rt * TR + f * 8 + g;
-      const bool live = row < w.r.rows;
-      const int tok = live ? row / p.group : 0, hd = w.h * p.group + (live ? row % p.group : 0);
-      const char* src = p.q + (int64_t)(w.r.q0 + tok) * p.ld_q + (int64_t)hd * p.kv.dim * 2;
-#pragma unroll
-      for (int ks = 0; ks < DP / 16; ++ks) {
-        const int d = ks * 16 + 2 * t4;
-        qf[ks][f][0] = live && d < p.kv.dim ? *reinterpret_cast<const uint32_t*>(src + d * 2) : 0u;
-        qf[ks][f][1] = live && d + 8 < p.kv.dim ? *reinterpret_cast<const uint32_t*>(src + d * 2 + 16) : 0u;
-        o[ks][f][0] = o[ks][f][1] = o[ks][f][2] = o[ks][f][3] = 0.f;
-      }
-    }
-  };
-  open_tile();
+  AttnPos next = w;
+  int tile_kb0 = w.kb, tile = 0;
+  bool opened = false, brief = false;  // the tile is set up; the tile before it was so short that copies may be out
   // this lane's ldmatrix rows, four 16-element steps of 128 bytes each
   uint32_t k_off[4], v_off[4];
 #pragma unroll
@@ -257,8 +250,48 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_few_ke
   int stage = 0;
   for (int64_t u = u0; u < u1; ++u) {
     cp_async_wait<S::kStages - 2>();
-    __syncwarp();
+    if (opened) {
+      __syncwarp();
+    } else {
+      // a new tile: its queries were copied by all warps
+      opened = true;
+      tile_kb0 = w.kb;
+      if (brief) cp_async_wait<0>();
+      __syncthreads();
+#pragma unroll
+      for (int f = 0; f < NQ; ++f) {
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ks += 2) {
+          uint32_t b[4];
+          ldsm4(chunk_addr<DP>(q_tiles + (tile & 1) * TR * S::kRowBytes, f * 8 + (lane & 7), ks * 2 + (lane >> 3)), b);
+          qf[ks][f][0] = b[0];
+          qf[ks][f][1] = b[1];
+          qf[ks + 1][f][0] = b[2];
+          qf[ks + 1][f][1] = b[3];
+        }
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) o[ks][f][0] = o[ks][f][1] = o[ks][f][2] = o[ks][f][3] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int row = w.rt * TR + f * 8 + 2 * t4 + i;
+          lim[f][i] = row < w.r.rows ? min(w.r.kv, attn_limit(p, w.r, row)) : 0;
+          m[f][i] = most[f][i] = kNegInf;
+          l[f][i] = 0.f;
+        }
+      }
+      lim_all = min(w.r.kv, attn_limit(p, w.r, w.rt * TR));
+      // the tile after it; its queries' place was last read before the last merge
+      const int n = w.nkb - w.kb;
+      brief = n < S::kStages;
+      if (n < u1 - u) {
+        next = w;
+        attn_next_tile<TR, kKeys>(p, next);
+        load_queries(next, (tile & 1) ^ 1);
+      }
+      ++tile;
+    }
     const uint32_t kt = ring + stage * 2 * S::kTileBytes, vt = kt + S::kTileBytes;
+    float* const left = reinterpret_cast<float*>(smem + stage * 2 * S::kTileBytes);   // for the merge
     const int ahead = stage == 0 ? S::kStages - 1 : stage - 1;      // the stage computed with last
     stage = stage + 1 == S::kStages ? 0 : stage + 1;
     ld.load(p, ring + ahead * 2 * S::kTileBytes);
@@ -276,9 +309,9 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_few_ke
         if (ks < kChains) mma16816<T, true>(s[f + ks % kChains], a[ks % kAhead], qf[ks][f][0], qf[ks][f][1]);
         else mma16816<T>(s[f + ks % kChains], a[ks % kAhead], qf[ks][f][0], qf[ks][f][1]);
       }
-      const int next = ks + kAhead;    // then the values: 16 elements x 16 keys
-      if (next < DP / 16) ldsm4(kt + k_off[next & 3] + (next >> 2) * 128, a[ks % kAhead]);
-      else ldsm4_t(vt + v_off[(next - DP / 16) & 3], a[ks % kAhead]);
+      const int then = ks + kAhead;    // after the keys the values: 16 elements x 16 keys
+      if (then < DP / 16) ldsm4(kt + k_off[then & 3] + (then >> 2) * 128, a[ks % kAhead]);
+      else ldsm4_t(vt + v_off[(then - DP / 16) & 3], a[ks % kAhead]);
     }
     if (kChains == 2) {
 #pragma unroll
@@ -337,8 +370,8 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_few_ke
     for (int d = 0; d < DP / 16; ++d) {
 #pragma unroll
       for (int f = 0; f < NQ; ++f) mma16816<T>(o[d][f], a[d % kAhead], b[f][0], b[f][1]);
-      const int next = d + kAhead;
-      if (next < DP / 16) ldsm4_t(vt + v_off[next & 3] + (next >> 2) * 128, a[d % kAhead]);
+      const int then = d + kAhead;
+      if (then < DP / 16) ldsm4_t(vt + v_off[then & 3] + (then >> 2) * 128, a[d % kAhead]);
     }
 
     // ---- end of the tile, or of this CTA's share of it
@@ -350,83 +383,74 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_few_ke
     const bool whole = last && tile_kb0 == 0;
     // slot 0: a tile entered in the middle; slot 1: a tile left unfinished
     const int64_t slot = 2 * (int64_t)blockIdx.x + (tile_kb0 == 0 ? 1 : 0);
+    // The warps leave maxima, sums and contexts, sixteen rows at a time: eight
+    // where each warp's keys were, eight where its values were (16 x DP x 2
+    // bytes hold 8 x DP floats).  Columns are XORed with the row so that a
+    // store's four rows take different banks.
 #pragma unroll
-    for (int f = 0; f < NQ; ++f) {
-      const int rows = w.r.rows - w.rt * TR - f * 8;   // rows from these eight on
+    for (int f0 = 0; f0 < NQ; f0 += 2) {
+      const int rows = min(min(16, TR - f0 * 8), w.r.rows - w.rt * TR - f0 * 8);   // of this pass
       if (rows <= 0) break;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int f = f0; f < NQ && f < f0 + 2; ++f) {
+        float* mine = left + (f - f0) * (S::kTileBytes / 4) + warp * 8 * DP;
 #pragma unroll
-        for (int off = 4; off < 32; off <<= 1) l[f][i] += __shfl_xor_sync(0xffffffffu, l[f][i], off);
-      // merge the warps: their common maximum, then the contexts added up in a
-      // fixed order
-      if (g == 0) *reinterpret_cast<float2*>(&merge_m[warp][2 * t4]) = make_float2(m[f][0], m[f][1]);
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) l[f][i] += __shfl_xor_sync(0xffffffffu, l[f][i], off);
+#pragma unroll
+          for (int d = 0; d < DP / 16; ++d) {
+            mine[(2 * t4 + i) * DP + ((d * 16 + g) ^ (t4 * 8))] = o[d][f][i];
+            mine[(2 * t4 + i) * DP + ((d * 16 + 8 + g) ^ (t4 * 8))] = o[d][f][i + 2];
+          }
+        }
+        if (g == 0) {
+          *reinterpret_cast<float2*>(&merge_m[warp][f * 8 + 2 * t4]) = make_float2(m[f][0], m[f][1]);
+          *reinterpret_cast<float2*>(&merge_l[warp][f * 8 + 2 * t4]) = make_float2(l[f][0], l[f][1]);
+        }
+      }
       __syncthreads();
+      for (int c = threadIdx.x; c < rows * kChunks; c += kThreads) {
+        const int r = c / kChunks, d8 = c % kChunks;
+        float e[kWarps], top = kNegInf, sum = 0.f, v[8] = {};
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float top = merge_m[0][2 * t4 + i];
+        for (int ww = 0; ww < kWarps; ++ww) top = fmaxf(top, merge_m[ww][f0 * 8 + r]);
 #pragma unroll
-        for (int ww = 1; ww < kWarps; ++ww) top = fmaxf(top, merge_m[ww][2 * t4 + i]);
-        const float e = m[f][i] == kNegInf ? 0.f : exp2_fast(m[f][i] - top);
-        l[f][i] *= e;
-#pragma unroll
-        for (int d = 0; d < DP / 16; ++d) {
-          o[d][f][i] *= e;
-          o[d][f][i + 2] *= e;
+        for (int ww = 0; ww < kWarps; ++ww) {
+          const float mw = merge_m[ww][f0 * 8 + r];
+          e[ww] = mw == kNegInf ? 0.f : exp2_fast(mw - top);
+          sum = fmaf(merge_l[ww][f0 * 8 + r], e[ww], sum);
+          const float4* src = reinterpret_cast<const float4*>(left + (r >> 3) * (S::kTileBytes / 4) + ww * 8 * DP +
+                                                              (r & 7) * DP + ((d8 * 8) ^ (((r & 7) >> 1) * 8)));
+          const float4 x = src[0], y = src[1];
+          v[0] = fmaf(x.x, e[ww], v[0]);
+          v[1] = fmaf(x.y, e[ww], v[1]);
+          v[2] = fmaf(x.z, e[ww], v[2]);
+          v[3] = fmaf(x.w, e[ww], v[3]);
+          v[4] = fmaf(y.x, e[ww], v[4]);
+          v[5] = fmaf(y.y, e[ww], v[5]);
+          v[6] = fmaf(y.z, e[ww], v[6]);
+          v[7] = fmaf(y.w, e[ww], v[7]);
         }
-      }
-      if (g == 0) *reinterpret_cast<float2*>(&merge_l[warp][2 * t4]) = make_float2(l[f][0], l[f][1]);
-      // warps 2 and 3 leave theirs in a buffer each, warps 0 and 1 add their
-      // own; a row's pitch of DP + 4 puts a store's 4 rows on different banks
-      static_assert(kWarps == 4, "merge order");
-#pragma unroll
-      for (int step = 0; step < 2; ++step) {
-        if ((warp >> 1) != step) {
-          float* mine = merge + (warp & 1) * 8 * S::kPitch + 2 * t4 * S::kPitch + g;
-#pragma unroll
-          for (int d = 0; d < DP / 16; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              float* dst = mine + (i & 1) * S::kPitch + d * 16 + (i >> 1) * 8;
-              *dst = step ? *dst + o[d][f][i] : o[d][f][i];
-            }
-        }
-        __syncthreads();
-      }
-      for (int c = threadIdx.x; c < 8 * (DP / 8); c += kThreads) {
-        const int r = c / (DP / 8), d8 = c % (DP / 8);
-        if (r >= rows) break;
-        const float4* src = reinterpret_cast<const float4*>(merge + r * S::kPitch + d8 * 8);
-        float4 a = src[0], b4 = src[1];
-        const float4 a1 = src[8 * S::kPitch / 4], b1 = src[8 * S::kPitch / 4 + 1];
-        a = make_float4(a.x + a1.x, a.y + a1.y, a.z + a1.z, a.w + a1.w);
-        b4 = make_float4(b4.x + b1.x, b4.y + b1.y, b4.z + b1.z, b4.w + b1.w);
-        const float sum = merge_l[0][r] + merge_l[1][r] + merge_l[2][r] + merge_l[3][r];
-        const int row = w.rt * TR + f * 8 + r;
         if (whole) {
           const float inv = row_scale<T>(sum);
-          const int tok = row / p.group, hd = w.h * p.group + row % p.group;
+          const int2 to = out_offset(w, w.rt * TR + f0 * 8 + r);
           if (d8 * 8 < p.kv.dim)
-            *reinterpret_cast<uint4*>(p.out + (int64_t)(w.r.q0 + tok) * p.ld_out + ((int64_t)hd * p.kv.dim + d8 * 8) * 2) =
-                make_uint4(Num<T>::pack(a.x * inv, a.y * inv), Num<T>::pack(a.z * inv, a.w * inv),
-                           Num<T>::pack(b4.x * inv, b4.y * inv), Num<T>::pack(b4.z * inv, b4.w * inv));
+            *reinterpret_cast<uint4*>(p.out + (int64_t)to.x * p.ld_out + ((int64_t)to.y * p.kv.dim + d8 * 8) * 2) =
+                make_uint4(Num<T>::pack(v[0] * inv, v[1] * inv), Num<T>::pack(v[2] * inv, v[3] * inv),
+                           Num<T>::pack(v[4] * inv, v[5] * inv), Num<T>::pack(v[6] * inv, v[7] * inv));
         } else {
-          float4* dst = reinterpret_cast<float4*>(p.part_o + (slot * TR + f * 8 + r) * DP + d8 * 8);
-          dst[0] = a;
-          dst[1] = b4;
-          if (d8 == 0) {
-            const float top = fmaxf(fmaxf(merge_m[0][r], merge_m[1][r]), fmaxf(merge_m[2][r], merge_m[3][r]));
-            p.part_ml[slot * TR + f * 8 + r] = make_float2(top, sum);
-          }
+          float4* dst = reinterpret_cast<float4*>(p.part_o + (slot * TR + f0 * 8 + r) * DP + d8 * 8);
+          dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+          dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+          if (d8 == 0) p.part_ml[slot * TR + f0 * 8 + r] = make_float2(top, sum);
         }
       }
       __syncthreads();
     }
     if (!whole && threadIdx.x == 0) attn_leave_part(p, w, tile_kb0 == 0, last);
-    if (u + 1 < u1) {
-      attn_next_tile<TR, kKeys>(p, w);
-      open_tile();
-    }
+    w = next;
+    opened = false;
   }
   cp_async_wait<0>();
 }
@@ -447,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_mid_ke
   constexpr int TR = 64, kChunks = DP / 8;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ AttnShare share;
-  __shared__ int64_t warp_sum[kWarps];
+  __shared__ int64_t warp_sum[2 * kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t ring = smem_addr(smem);
   uint8_t* q_tile = smem + (size_t)S::kStages * 2 * S::kTileBytes;
@@ -714,7 +738,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) paged_attn_join_kernel(const 
   }
 }
 
-// TR rows a tile: 8 to 32 on the few-row kernel, 64 on the other.
+// TR rows a tile: 8 to 24 on the few-row kernel, 64 on the other.
 template <typename T, int DP, int TR>
 int run_class(AttnParams p, const PagedAttention& a, int sms, cudaStream_t stream) {
   const int ctas = sms * Shape<DP>::kPerSm;
@@ -726,7 +750,7 @@ int run_class(AttnParams p, const PagedAttention& a, int sms, cudaStream_t strea
     smem = mid_smem<DP>();
   } else {
     kernel = paged_attn_few_kernel<T, DP, TR / 8>;
-    smem = few_smem<DP>();
+    smem = few_smem<DP, TR / 8>();
   }
   SMEAI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   SMEAI_CUDA_TRY(launch(kernel, dim3((unsigned)ctas), dim3(kThreads), smem, stream, p));
@@ -737,7 +761,7 @@ int run_class(AttnParams p, const PagedAttention& a, int sms, cudaStream_t strea
 
 // Which kernels a call needs, from what the host knows: the largest request's
 // packed rows and the total.
-//   up to 8, 16, 24, 32 rows  tiles of so many: one reading of the keys for all
+//   up to 8, 16, 24 rows  tiles of so many: one reading of the keys for all
 //   more                  the tensor-core kernel, and the 16-row tiles beside it
 //                         for requests of up to 16 rows (a step that mixes
 //                         prompts and decoding) unless the total says that
@@ -755,7 +779,7 @@ Classes classes(const PagedAttention& a) {
   Classes c = {0, false, false};
   if (most <= 16) c.few = most <= 8 ? 8 : 16;
   else if (a.kv.dim > 128) c.mid = true;
-  else if (most <= 32) c.few = most <= 24 ? 24 : 32;
+  else if (most <= 24) c.few = 24;
   else {
     c.many = true;
     // with one request of r <= 16 / group rows the others, of max_new at most, could not make up n_tokens
@@ -775,8 +799,7 @@ int run_dim(const AttnParams& p, const PagedAttention& a, int sms, cudaStream_t 
     int st;
     if (c.few == 8) st = run_class<T, DP, 8>(q, a, sms, stream);
     else if (DP > 128 || c.few == 16) st = run_class<T, DP, 16>(q, a, sms, stream);
-    else if (c.few == 24) st = run_class<T, DP, DP <= 128 ? 24 : 16>(q, a, sms, stream);
-    else st = run_class<T, DP, DP <= 128 ? 32 : 16>(q, a, sms, stream);
+    else st = run_class<T, DP, DP <= 128 ? 24 : 16>(q, a, sms, stream);
     if (st) return st;
   }
   if constexpr (DP > 128) {
@@ -808,8 +831,8 @@ size_t paged_attention_workspace(const PagedAttention& a) {
   const int dp = padded_dim(a.kv.dim);
   if (c.many) return paged_attn_tc_workspace(dp, sms);   // the 16-row tiles' need is smaller
   if (c.mid) return attn_part_bytes<64, 256>(sms);
-  return dp == 64    ? attn_part_bytes<32, 64>(2 * sms)  // of 32 rows, whichever tile it is
-         : dp == 128 ? attn_part_bytes<32, 128>(2 * sms)
+  return dp == 64    ? attn_part_bytes<24, 64>(2 * sms)  // of 24 rows, whichever tile it is
+         : dp == 128 ? attn_part_bytes<24, 128>(2 * sms)
                      : attn_part_bytes<16, 256>(sms);
 }
 

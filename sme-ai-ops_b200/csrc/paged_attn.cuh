@@ -12,7 +12,10 @@
 // (running maximum, sum, unnormalized context; all fp32), which a second
 // kernel joins in key order, so results do not depend on timing.  Pieces are
 // snapped to a tile's edge when one is within kSnap units: short tiles are
-// never split and need no joining.
+// never split and need no joining.  On the line a tile is longer than its
+// blocks by what opening and ending it costs (measured: 5000 to 8000 cycles
+// against 2500 a block of 64 keys, 4000 against 3500 a block of 128), so a CTA
+// that gets many short tiles gets fewer blocks.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -23,6 +26,8 @@
 namespace smeai {
 
 constexpr int kSnap = 3;
+template <int KB>
+constexpr int kTileCost = KB == 64 ? 2 : 1;   // in blocks
 
 struct AttnParams {
   KvView kv;
@@ -72,15 +77,18 @@ __device__ __forceinline__ int attn_limit(const AttnParams& p, const AttnReq& r,
 // has its zeros to write).
 template <int TR, int KB>
 __device__ __forceinline__ int attn_blocks(const AttnParams& p, const AttnReq& r, int rt) {
-  const int last = min((rt + 1) * TR, r.rows) - 1;
-  return max(1, (min(r.kv, attn_limit(p, r, last)) + KB - 1) / KB);
+  const int end = (rt + 1) * TR;
+  const int keys = end >= r.rows ? r.kv : min(r.kv, attn_limit(p, r, end - 1));   // the last row sees them all
+  return max(1, (int)((unsigned)(keys + KB - 1) / KB));
 }
 
+// Key blocks of all tiles of a request; `tiles` gets their number.
 template <int TR, int KB>
-__device__ __forceinline__ int64_t attn_units(const AttnParams& p, const AttnReq& r) {
+__device__ __forceinline__ int64_t attn_units(const AttnParams& p, const AttnReq& r, int64_t& tiles) {
   int64_t u = 0;
   const int n_rt = (r.rows + TR - 1) / TR;
   for (int rt = 0; rt < n_rt; ++rt) u += attn_blocks<TR, KB>(p, r, rt);
+  tiles = (int64_t)n_rt * p.kv.n_kv;
   return u * p.kv.n_kv;
 }
 
@@ -107,68 +115,84 @@ __device__ __forceinline__ void attn_next_tile(const AttnParams& p, AttnPos& w) 
 }
 
 struct AttnShare {
-  int64_t u0, u1;            // this CTA's units
+  int64_t u0, u1;            // this CTA's units: key blocks, counted along the line
   AttnPos at;                // place of u0
 };
 
 // This CTA's piece of the line.  All threads of the block call it; the place
-// is in shared memory on return.  warp_sum: [NT / 32] in shared memory.  Each thread sums the units of its own run of
-// requests; the one whose run holds an end of the piece walks to it.
+// is in shared memory on return.  warp_sum: [2 * NT / 32] in shared memory.  Each
+// thread sums its own run of requests; the one whose run holds an end of the
+// piece walks to it.
 template <int TR, int KB, int NT>
 __device__ void attn_share(const AttnParams& p, AttnShare* s, int64_t* warp_sum) {
+  constexpr int kCost = kTileCost<KB>;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int per = (p.n_req + NT - 1) / NT;
   const int b0 = min((int)threadIdx.x * per, p.n_req), b1 = min(b0 + per, p.n_req);
-  int64_t mine = 0;
-  for (int b = b0; b < b1; ++b) mine += attn_units<TR, KB>(p, attn_req(p, b));
-  int64_t incl = mine;
+  int64_t mine = 0, mine_t = 0;               // blocks, tiles
+  for (int b = b0; b < b1; ++b) {
+    int64_t t;
+    mine += attn_units<TR, KB>(p, attn_req(p, b), t);
+    mine_t += t;
+  }
+  int64_t incl = mine, incl_t = mine_t;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
-    const int64_t t = __shfl_up_sync(0xffffffffu, incl, off);
-    if (lane >= off) incl += t;
+    const int64_t a = __shfl_up_sync(0xffffffffu, incl, off), t = __shfl_up_sync(0xffffffffu, incl_t, off);
+    if (lane >= off) {
+      incl += a;
+      incl_t += t;
+    }
   }
-  if (lane == 31) warp_sum[warp] = incl;
+  if (lane == 31) {
+    warp_sum[2 * warp] = incl;
+    warp_sum[2 * warp + 1] = incl_t;
+  }
   __syncthreads();
-  int64_t before = 0, total = 0;
+  int64_t lo = incl - mine, lo_t = incl_t - mine_t, total = 0, total_t = 0;
 #pragma unroll
   for (int w = 0; w < NT / 32; ++w) {
-    if (w < warp) before += warp_sum[w];
-    total += warp_sum[w];
+    const int64_t a = warp_sum[2 * w], t = warp_sum[2 * w + 1];
+    if (w < warp) {
+      lo += a;
+      lo_t += t;
+    }
+    total += a;
+    total_t += t;
   }
-  const int64_t lo = before + incl - mine;   // units ahead of this thread's run
-  // 64-bit division is slow, and totals are rarely that large
-  const int64_t per_cta = total <= 0x7fff0000 ? ((uint32_t)total + gridDim.x - 1) / gridDim.x
-                                              : (total + gridDim.x - 1) / gridDim.x;
-  const int64_t cut0 = min(total, per_cta * blockIdx.x), cut1 = min(total, cut0 + per_cta);
+  // lengths on the line, with the tiles' own costs
+  const int64_t line = total + kCost * total_t, line_lo = lo + kCost * lo_t, line_hi = line_lo + mine + kCost * mine_t;
+  // 64-bit division is slow, and lines are rarely that long
+  const int64_t per_cta = line <= 0x7fff0000 ? ((uint32_t)line + gridDim.x - 1) / gridDim.x
+                                             : (line + gridDim.x - 1) / gridDim.x;
+  const int64_t cut0 = min(line, per_cta * blockIdx.x), cut1 = min(line, cut0 + per_cta);
   if (threadIdx.x == 0) {
-    if (cut0 >= total) s->u0 = total;
-    if (cut1 >= total) s->u1 = total;
+    if (cut0 >= line) s->u0 = total;
+    if (cut1 >= line) s->u1 = total;
   }
   // walk to each cut that lies in this run: the tile around it, and the edge it snaps to
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     const int64_t cut = which ? cut1 : cut0;
-    if (cut < lo || cut >= lo + mine) continue;
-    int64_t at = lo;
+    if (cut < line_lo || cut >= line_hi) continue;
+    int64_t at = line_lo, u = lo;
     for (int b = b0; b < b1; ++b) {
       const AttnReq r = attn_req(p, b);
       const int n_rt = (r.rows + TR - 1) / TR;
       for (int rt = 0; rt < n_rt; ++rt) {
         const int nkb = attn_blocks<TR, KB>(p, r, rt);
-        if (cut >= at + (int64_t)nkb * p.kv.n_kv) {
-          at += (int64_t)nkb * p.kv.n_kv;
+        const int64_t len = (int64_t)(nkb + kCost) * p.kv.n_kv;
+        if (cut >= at + len) {
+          at += len;
+          u += (int64_t)nkb * p.kv.n_kv;
           continue;
         }
-        const unsigned in = (unsigned)(cut - at);      // below nkb * n_kv, which fits
-        int h = (int)(in / (unsigned)nkb), kb = (int)(in % (unsigned)nkb);
-        int64_t u = cut;
-        if (kb <= kSnap && kb <= nkb - kb) {
-          u -= kb;
-          kb = 0;
-        } else if (nkb - kb <= kSnap) {
-          u += nkb - kb;
-          kb = nkb;        // the start of the next tile
-        }
+        const int64_t in = cut - at;
+        const int h = len <= 0x7fffffff ? (int)((unsigned)in / (unsigned)(nkb + kCost)) : (int)(in / (nkb + kCost));
+        int kb = max(0, (int)(in - (int64_t)h * (nkb + kCost)) - kCost);
+        if (kb <= kSnap && kb <= nkb - kb) kb = 0;
+        else if (nkb - kb <= kSnap) kb = nkb;           // the start of the next tile
+        u += (int64_t)h * nkb + kb;
         if (which) s->u1 = u;
         else {
           s->u0 = u;
