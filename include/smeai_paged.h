@@ -100,8 +100,10 @@ int smeai_paged_append(const smeai_kv_cache *cache, const float *k, int64_t ld_k
  * request only (with causal, possibly a chunk's rows before it).
  * max_new is the largest number of new tokens of a request (larger ones still
  * come out right, more slowly); a captured call keeps it.
- * workspace: at least smeai_paged_attention_workspace bytes, 256-byte aligned,
- * in use until the call's work is done, by one call at a time; need not be
+ * workspace: at least smeai_paged_attention_workspace bytes (0, and then NULL
+ * will do, when a table row names too few keys for a request ever to be split
+ * over CTAs, and for sizes that the call refuses), 256-byte aligned, in use
+ * until the call's work is done, by one call at a time; need not be
  * initialised and holds nothing afterwards. */
 size_t smeai_paged_attention_workspace(const smeai_kv_cache *cache, int n_heads, int64_t n_tokens, int64_t n_req,
                                        int64_t max_blocks, int64_t max_new);

@@ -1,6 +1,8 @@
 // api_paged.cu -- the C-ABI of include/smeai_paged.h.
 #include <math.h>
 
+#include <atomic>
+
 #include "common.cuh"
 #include "paged.h"
 #include "runtime.h"
@@ -56,8 +58,16 @@ int view(const char* what, const smeai_kv_cache* c, KvView* v) {
   return kOk;
 }
 
+// Whether the current device can run the kernels; what was found is kept, a
+// device's compute capability does not change.
 int ready(const char* what) {
-  if (device_ready()) return kOk;
+  static std::atomic<uint64_t> good{0};
+  int dev = 0;
+  if (good.load() && cudaGetDevice(&dev) == cudaSuccess && dev < 64 && (good.load() >> dev & 1)) return kOk;
+  if (device_ready()) {
+    if (cudaGetDevice(&dev) == cudaSuccess && dev < 64) good.fetch_or((uint64_t)1 << dev);
+    return kOk;
+  }
   set_last_error("%s: no compute-capability-10.x device", what);
   return kUnsupported;
 }
@@ -162,7 +172,7 @@ int smeai_paged_attention(const smeai_kv_cache* cache, const void* q, int64_t ld
   st = ready(what);
   if (st) return st;
   const size_t need = paged_attention_workspace(a);
-  if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255)) {
+  if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255))) {
     set_last_error("%s: needs a 256-byte aligned workspace of %zu bytes", what, need);
     return !workspace || workspace_bytes < need ? kWorkspaceTooSmall : kBadArgument;
   }

@@ -742,7 +742,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) paged_attn_join_kernel(const 
 template <typename T, int DP, int TR>
 int run_class(AttnParams p, const PagedAttention& a, int sms, cudaStream_t stream) {
   const int ctas = sms * Shape<DP>::kPerSm;
-  attn_carve<TR, DP>(p, a.workspace, ctas);
+  const bool splits = attn_splits<kKeys>(a.max_kv);
+  attn_carve<TR, DP>(p, splits ? a.workspace : nullptr, ctas);
   void (*kernel)(AttnParams);
   size_t smem;
   if constexpr (TR == 64) {
@@ -752,10 +753,10 @@ int run_class(AttnParams p, const PagedAttention& a, int sms, cudaStream_t strea
     kernel = paged_attn_few_kernel<T, DP, TR / 8>;
     smem = few_smem<DP, TR / 8>();
   }
-  SMEAI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  static std::atomic<uint64_t> allowed{0};
+  SMEAI_CUDA_TRY(attn_allow_smem(kernel, smem, allowed));
   SMEAI_CUDA_TRY(launch(kernel, dim3((unsigned)ctas), dim3(kThreads), smem, stream, p));
-  // a tile of up to 2 * kSnap blocks is never split
-  if (a.max_kv > 2 * kSnap * kKeys) SMEAI_CUDA_TRY((attn_join<T, TR, DP>(p, ctas, stream)));
+  if (splits) SMEAI_CUDA_TRY((attn_join<T, TR, DP>(p, ctas, stream)));
   return kOk;
 }
 
@@ -829,7 +830,9 @@ size_t paged_attention_workspace(const PagedAttention& a) {
   if (sm_count(&sms)) return 0;
   const Classes c = classes(a);
   const int dp = padded_dim(a.kv.dim);
-  if (c.many) return paged_attn_tc_workspace(dp, sms);   // the 16-row tiles' need is smaller
+  const size_t many = c.many ? paged_attn_tc_workspace(dp, a.max_kv, sms) : 0;
+  if (many) return many;                                 // the 16-row tiles' need is smaller
+  if ((c.many && !c.few) || !attn_splits<kKeys>(a.max_kv)) return 0;
   if (c.mid) return attn_part_bytes<64, 256>(sms);
   return dp == 64    ? attn_part_bytes<24, 64>(2 * sms)  // of 24 rows, whichever tile it is
          : dp == 128 ? attn_part_bytes<24, 128>(2 * sms)

@@ -20,6 +20,8 @@
 
 #include <cuda_bf16.h>
 
+#include <atomic>
+
 #include "common.cuh"
 #include "paged.h"
 
@@ -214,6 +216,7 @@ __device__ __forceinline__ void attn_open(const AttnParams& p, const AttnShare& 
 
 // Thread 0 of a CTA: its headers before any tile, and a tile not finished here.
 __device__ __forceinline__ void attn_no_parts(const AttnParams& p) {
+  if (!p.head) return;       // no tile can be split
   p.head[blockIdx.x] = make_int4(-1, 0, 0, 0);
   p.state[blockIdx.x] = kPartNone;
 }
@@ -266,6 +269,12 @@ __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// Whether any tile can be split: those of up to 2 * kSnap blocks never are.
+template <int KB>
+constexpr bool attn_splits(int max_kv) {
+  return max_kv > 2 * kSnap * KB;
+}
+
 // Partial slots and headers of a launch with `ctas` CTAs.
 template <int TR, int DP>
 constexpr size_t attn_part_bytes(int ctas) {
@@ -273,7 +282,12 @@ constexpr size_t attn_part_bytes(int ctas) {
 }
 template <int TR, int DP>
 void attn_carve(AttnParams& p, void* ws, int ctas) {
+  p.part_o = nullptr;
+  p.part_ml = nullptr;
+  p.head = nullptr;
+  p.state = nullptr;
   char* c = static_cast<char*>(ws);
+  if (!c) return;
   p.part_o = reinterpret_cast<float*>(c);
   c += (size_t)2 * ctas * TR * DP * sizeof(float);
   p.part_ml = reinterpret_cast<float2*>(c);
@@ -284,8 +298,21 @@ void attn_carve(AttnParams& p, void* ws, int ctas) {
 
 // The tensor-core kernel of requests with many rows, head_dim up to 128
 // (paged_attn_tc.cu): one CTA an SM.
-size_t paged_attn_tc_workspace(int padded_dim, int sms);
+size_t paged_attn_tc_workspace(int padded_dim, int max_kv, int sms);
 int paged_attn_tc(const AttnParams& p, int padded_dim, void* workspace, int max_kv, int sms, cudaStream_t stream);
+
+// The kernel's dynamic shared memory limit, set once a device.
+template <typename K>
+cudaError_t attn_allow_smem(K kernel, size_t bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
+  if (done.load() & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess) done.fetch_or(bit);
+  return e;
+}
 
 // Joins the partial results (paged_attn.cu).
 template <typename T, int TR, int DP>

@@ -33,8 +33,6 @@
 #include <cuda.h>
 #include <string.h>
 
-#include <atomic>
-
 #include "paged_attn.cuh"
 #include "tcgen05.cuh"
 
@@ -695,14 +693,16 @@ bool cache_map(const KvView& kv, const void* base, int box_rows, CUtensorMap* ma
 template <typename T, int DP, bool kTma>
 int run_kernel(const AttnParams& p, const TcMaps& maps, int sms, cudaStream_t stream) {
   auto kernel = paged_attn_tc_kernel<T, DP, kTma>;
-  SMEAI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Tc<DP>::kSmem));
+  static std::atomic<uint64_t> allowed{0};
+  SMEAI_CUDA_TRY(attn_allow_smem(kernel, Tc<DP>::kSmem, allowed));
   SMEAI_CUDA_TRY(launch(kernel, dim3((unsigned)sms), dim3(kThreads), Tc<DP>::kSmem, stream, p, maps, wait_timeout_ns()));
   return kOk;
 }
 
 template <typename T, int DP>
 int run_tc(AttnParams p, void* workspace, int max_kv, int sms, cudaStream_t stream) {
-  attn_carve<kTR, DP>(p, workspace, sms);
+  const bool splits = attn_splits<kKB>(max_kv);
+  attn_carve<kTR, DP>(p, splits ? workspace : nullptr, sms);
   TcMaps maps;
   memset(&maps, 0, sizeof(maps));
   maps.box_log2 = p.kv.page_log2 < 6 ? p.kv.page_log2 : 6;
@@ -710,13 +710,14 @@ int run_tc(AttnParams p, void* workspace, int max_kv, int sms, cudaStream_t stre
                    cache_map(p.kv, p.kv.v, 1 << maps.box_log2, &maps.v);
   const int st = tma ? run_kernel<T, DP, true>(p, maps, sms, stream) : run_kernel<T, DP, false>(p, maps, sms, stream);
   if (st) return st;
-  if (max_kv > 2 * kSnap * kKB) SMEAI_CUDA_TRY((attn_join<T, kTR, DP>(p, sms, stream)));
+  if (splits) SMEAI_CUDA_TRY((attn_join<T, kTR, DP>(p, sms, stream)));
   return kOk;
 }
 
 }  // namespace
 
-size_t paged_attn_tc_workspace(int padded_dim, int sms) {
+size_t paged_attn_tc_workspace(int padded_dim, int max_kv, int sms) {
+  if (!attn_splits<kKB>(max_kv)) return 0;
   return padded_dim == 64 ? attn_part_bytes<kTR, 64>(sms) : attn_part_bytes<kTR, 128>(sms);
 }
 

@@ -3,6 +3,8 @@
 // and values into their slots.
 #include <cuda_bf16.h>
 
+#include <atomic>
+
 #include "common.cuh"
 #include "paged.h"
 
@@ -197,9 +199,12 @@ __global__ void __launch_bounds__(256) paged_slots_kernel(const PlanParams p) {
 }  // namespace
 
 int sm_count(int* n) {
+  static std::atomic<int> known[64];
   int dev = 0;
   SMEAI_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 64 && (*n = known[dev].load())) return kOk;
   SMEAI_CUDA_TRY(cudaDeviceGetAttribute(n, cudaDevAttrMultiProcessorCount, dev));
+  if (dev < 64) known[dev].store(*n);
   return kOk;
 }
 

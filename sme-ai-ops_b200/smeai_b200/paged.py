@@ -17,7 +17,7 @@ import ctypes
 import torch
 
 from . import KV_BF16, KV_F16, KVCache, check, lib
-from .q2k import on_device
+from .q2k import call
 
 _TYPES = {torch.float16: KV_F16, torch.bfloat16: KV_BF16}
 
@@ -45,6 +45,7 @@ class PagedKV:
         self.struct = KVCache(k.data_ptr(), v.data_ptr(), _TYPES[k.dtype], self.page_size, self.n_kv_heads, self.head_dim,
                               self.n_pages, k.stride(0), k.stride(1), k.stride(2))
         self.ref = ctypes.byref(self.struct)
+        self._workspace = {}         # bytes of attention()'s workspace, by sizes
 
     @classmethod
     def empty(cls, n_pages: int, n_kv_heads: int, page_size: int, head_dim: int, dtype=torch.float16, device=None) -> "PagedKV":
@@ -80,23 +81,22 @@ class PagedPlan:
         which advances (in place, or into used_out)."""
         if used_out is None:
             used_out = n_used
-        for t, n in ((cached_len, self.n_req), (new_len, self.n_req), (free_pages, None), (n_used, 1), (used_out, 1)):
-            assert t.dtype == torch.int32 and t.device == self.device and t.is_contiguous()
-            assert n is None or t.numel() == n
-        with on_device(self.device) as stream:
-            check(lib().smeai_paged_plan(cached_len.data_ptr(), new_len.data_ptr(), self.n_req, self.page_size,
-                                         free_pages.data_ptr(), free_pages.numel(), n_used.data_ptr(), used_out.data_ptr(),
-                                         *self._out, stream), "paged_plan")
+        i32, dev, n = torch.int32, self.device, self.n_req
+        assert cached_len.dtype == new_len.dtype == free_pages.dtype == n_used.dtype == used_out.dtype == i32
+        assert cached_len.device == new_len.device == free_pages.device == n_used.device == used_out.device == dev
+        assert cached_len.numel() == new_len.numel() == n and n_used.numel() == used_out.numel() == 1
+        assert cached_len.is_contiguous() and new_len.is_contiguous() and free_pages.is_contiguous()
+        call(dev, lib().smeai_paged_plan, "paged_plan", cached_len.data_ptr(), new_len.data_ptr(), n, self.page_size,
+             free_pages.data_ptr(), free_pages.numel(), n_used.data_ptr(), used_out.data_ptr(), *self._out)
         return self
 
 
-def _rows(x: torch.Tensor, heads: int, dim: int, dtype, dev) -> int:
-    """The row stride of [n_tokens, heads, dim] whose rows are contiguous."""
-    assert x.dim() == 3 and x.shape[1] == heads and x.shape[2] == dim and x.dtype == dtype and x.device == dev
-    n, row = x.shape[0], heads * dim
+def _rows(x: torch.Tensor, n: int, heads: int, dim: int, dtype, dev) -> int:
+    """The row stride of x [n, heads, dim], a token's heads next to one another."""
+    assert x.shape == (n, heads, dim) and x.dtype == dtype and x.device == dev
     st = x.stride()
     assert (st[2] == 1 or dim == 1) and (st[1] == dim or heads == 1), "a token's heads lie next to one another"
-    return st[0] if n > 1 else max(row, st[0])
+    return st[0] if n > 1 else heads * dim        # a single row's stride says nothing
 
 
 def append(kv: PagedKV, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, q: torch.Tensor | None = None,
@@ -107,30 +107,25 @@ def append(kv: PagedKV, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, q
     element pairs, or halves) at positions (int32) when given, and returns q
     (fp32 [n_tokens, n_heads, head_dim]) rotated the same way, in the cache's type."""
     dev, dim, n = kv.device, kv.head_dim, k.shape[0]
-    ld_k, ld_v = _rows(k, kv.n_kv_heads, dim, torch.float32, dev), _rows(v, kv.n_kv_heads, dim, torch.float32, dev)
-    assert v.shape[0] == n and slots.dtype == torch.int64 and slots.device == dev and slots.numel() == n and slots.is_contiguous()
+    ld_k, ld_v = _rows(k, n, kv.n_kv_heads, dim, torch.float32, dev), _rows(v, n, kv.n_kv_heads, dim, torch.float32, dev)
+    assert slots.dtype == torch.int64 and slots.device == dev and slots.shape == (n,) and slots.is_contiguous()
     heads = ld_q = ld_qo = n_rope = 0
+    q_ptr = qo_ptr = pos_ptr = rope_ptr = None
     if q is not None:
         heads = q.shape[1]
-        ld_q = _rows(q, heads, dim, torch.float32, dev)
         if q_out is None:
             q_out = torch.empty((n, heads, dim), dtype=kv.dtype, device=dev)
-        ld_qo = _rows(q_out, heads, dim, kv.dtype, dev)
-        assert q.shape[0] == q_out.shape[0] == n
+        ld_q, ld_qo = _rows(q, n, heads, dim, torch.float32, dev), _rows(q_out, n, heads, dim, kv.dtype, dev)
+        q_ptr, qo_ptr = q.data_ptr(), q_out.data_ptr()
     else:
         assert q_out is None
     if rope is not None:
-        assert rope.dtype == torch.float32 and rope.device == dev and rope.dim() == 2 and rope.shape[1] == dim and rope.is_contiguous()
-        assert positions is not None and positions.dtype == torch.int32 and positions.device == dev
-        assert positions.numel() == n and positions.is_contiguous()
-        n_rope = rope.shape[0]
-    if n == 0:
-        return q_out
-    with on_device(dev) as stream:
-        check(lib().smeai_paged_append(kv.ref, k.data_ptr(), ld_k, v.data_ptr(), ld_v, q.data_ptr() if heads else None, ld_q,
-                                       heads, q_out.data_ptr() if heads else None, ld_qo, n, slots.data_ptr(),
-                                       positions.data_ptr() if n_rope else None, rope.data_ptr() if n_rope else None, n_rope,
-                                       halves, stream), "paged_append")
+        n_rope, pos_ptr, rope_ptr = rope.shape[0], positions.data_ptr(), rope.data_ptr()
+        assert rope.dtype == torch.float32 and rope.device == dev and rope.shape == (n_rope, dim) and rope.is_contiguous()
+        assert positions.dtype == torch.int32 and positions.device == dev and positions.shape == (n,) and positions.is_contiguous()
+    if n:
+        call(dev, lib().smeai_paged_append, "paged_append", kv.ref, k.data_ptr(), ld_k, v.data_ptr(), ld_v, q_ptr, ld_q, heads,
+             qo_ptr, ld_qo, n, slots.data_ptr(), pos_ptr, rope_ptr, n_rope, halves)
     return q_out
 
 
@@ -145,34 +140,40 @@ def attention(q: torch.Tensor, kv: PagedKV, block_table: torch.Tensor, q_start: 
     flight; by default it is allocated for this call."""
     dev, dim = kv.device, kv.head_dim
     n, heads = q.shape[0], q.shape[1]
-    ld_q = _rows(q, heads, dim, kv.dtype, dev)
+    ld_q = _rows(q, n, heads, dim, kv.dtype, dev)
     if out is None:
         out = torch.empty((n, heads, dim), dtype=kv.dtype, device=dev)
-    ld_out = _rows(out, heads, dim, kv.dtype, dev)
+        ld_out = heads * dim
+    else:
+        ld_out = _rows(out, n, heads, dim, kv.dtype, dev)
     n_req, max_blocks = block_table.shape
-    assert out.shape[0] == n and block_table.dtype == q_start.dtype == kv_len.dtype == torch.int32
-    assert block_table.device == q_start.device == kv_len.device == dev and (block_table.stride(1) == 1 or max_blocks <= 1)
-    assert q_start.numel() == n_req + 1 and kv_len.numel() == n_req and q_start.is_contiguous() and kv_len.is_contiguous()
-    L = lib()
+    ld_table, one = block_table.stride()
+    assert block_table.dtype == q_start.dtype == kv_len.dtype == torch.int32
+    assert block_table.device == q_start.device == kv_len.device == dev and (one == 1 or max_blocks <= 1)
+    assert q_start.shape == (n_req + 1,) and kv_len.shape == (n_req,) and q_start.is_contiguous() and kv_len.is_contiguous()
     if n == 0:
         return out
-    with on_device(dev) as stream:
-        if workspace is None:
-            workspace = torch.empty(L.smeai_paged_attention_workspace(kv.ref, heads, n, n_req, max_blocks, max_new),
-                                    dtype=torch.uint8, device=dev)
-        check(L.smeai_paged_attention(kv.ref, q.data_ptr(), ld_q, heads, n, q_start.data_ptr(), kv_len.data_ptr(), n_req,
-                                      block_table.data_ptr(), max(max_blocks, block_table.stride(0)), max_blocks, max_new,
-                                      dim ** -0.5 if scale is None else scale, causal, out.data_ptr(), ld_out,
-                                      workspace.data_ptr(), workspace.numel(), stream), "paged_attention")
+    ws_ptr, ws_bytes = None, attention_workspace(kv, heads, n, n_req, max_blocks, max_new)
+    if workspace is not None:
+        assert workspace.dtype == torch.uint8 and workspace.device == dev and workspace.is_contiguous()
+        ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel()
+    elif ws_bytes:
+        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        ws_ptr = workspace.data_ptr()
+    call(dev, lib().smeai_paged_attention, "paged_attention", kv.ref, q.data_ptr(), ld_q, heads, n, q_start.data_ptr(),
+         kv_len.data_ptr(), n_req, block_table.data_ptr(), max(max_blocks, ld_table), max_blocks, max_new,
+         dim ** -0.5 if scale is None else scale, causal, out.data_ptr(), ld_out, ws_ptr, ws_bytes)
     return out
 
 
 def attention_workspace(kv: PagedKV, n_heads: int, n_tokens: int, n_req: int, max_blocks: int, max_new: int) -> int:
-    """Bytes of attention()'s workspace for calls of at most these sizes."""
-    with on_device(kv.device):
-        n = lib().smeai_paged_attention_workspace(kv.ref, n_heads, n_tokens, n_req, max_blocks, max_new)
-    if n == 0:
-        check(-1, "paged_attention_workspace")
+    """Bytes of attention()'s workspace for a call of these sizes; 0 when the
+    table's rows are too short for a request's keys ever to be split."""
+    key = (n_heads, n_tokens, n_req, max_blocks, max_new)
+    n = kv._workspace.get(key)
+    if n is None:
+        with torch.cuda.device(kv.device):
+            n = kv._workspace[key] = lib().smeai_paged_attention_workspace(kv.ref, *key)
     return n
 
 

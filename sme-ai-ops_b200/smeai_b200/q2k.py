@@ -18,29 +18,20 @@ def cur_stream() -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-class on_device:
-    """The stream of a device's current work, with that device current inside
-    the block (a call on another device's tensors launches there)."""
-    __slots__ = ("want", "had")
-
-    def __init__(self, dev: torch.device):
-        self.want = dev.index
-
-    def __enter__(self):
-        self.had = torch.cuda.current_device()
-        if self.want is not None and self.had != self.want:
-            torch.cuda.set_device(self.want)
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *exc):
-        if self.want is not None and self.had != self.want:
-            torch.cuda.set_device(self.had)
-        return False
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _ld(x: torch.Tensor) -> int:
-    """Row stride of a 2-d tensor; a single row's stride says nothing."""
-    return x.stride(0) if x.shape[0] > 1 else max(x.shape[1], x.stride(0))
+def call(dev: torch.device, fn, what: str, *args) -> None:
+    """fn(*args, stream) on the current stream of tensors' device `dev`, with
+    that device current, and its status checked."""
+    index = dev.index
+    if index == torch.cuda.current_device():
+        status = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, _raw_stream(index))
+    if status:
+        check(status, what)
 
 
 def quantize_q8k(x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -85,17 +76,17 @@ def add_rms_quantize_q8k(x: torch.Tensor, resid: torch.Tensor, eps: float, out: 
         out = torch.empty((n, k // QK_K * Q8K_BLOCK_BYTES), dtype=torch.uint8, device=dev)
     assert x.is_cuda and x.dtype == resid.dtype == sum_out.dtype == torch.float32
     assert resid.shape == sum_out.shape == x.shape and resid.device == sum_out.device == out.device == dev
-    assert k == 1 or x.stride(1) == resid.stride(1) == sum_out.stride(1) == 1
+    lx, lr, ls = x.stride(), resid.stride(), sum_out.stride()
+    assert lx[1] == lr[1] == ls[1] == 1 or k == 1
     assert out.dtype == torch.uint8 and out.is_contiguous() and out.numel() == n * (k // QK_K) * Q8K_BLOCK_BYTES
     if norm_w is not None:
         assert norm_w.dtype == torch.float32 and norm_w.device == dev and norm_w.numel() == k and norm_w.is_contiguous()
     if n == 0:
         return sum_out, out
-    with on_device(dev) as stream:
-        check(lib().smeai_add_rms_q8k_quantize(x.data_ptr(), _ld(x), resid.data_ptr(), _ld(resid), n, k,
-                                               None if norm_w is None else norm_w.data_ptr(), eps,
-                                               sum_out.data_ptr(), _ld(sum_out), out.data_ptr(), stream),
-              "add_rms_q8k_quantize")
+    # a single row's stride says nothing
+    lx, lr, ls = (lx[0], lr[0], ls[0]) if n > 1 else (k, k, k)
+    call(dev, lib().smeai_add_rms_q8k_quantize, "add_rms_q8k_quantize", x.data_ptr(), lx, resid.data_ptr(), lr, n, k,
+         None if norm_w is None else norm_w.data_ptr(), eps, sum_out.data_ptr(), ls, out.data_ptr())
     return sum_out, out
 
 
