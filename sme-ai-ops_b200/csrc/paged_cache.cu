@@ -79,14 +79,15 @@ struct PlanParams {
 };
 
 // One CTA: two running sums over the requests (rows, pages) decide who is
-// served, a warp a request writes the new table entries, and, for a step of up
-// to kPlanOwnTokens rows, each thread maps rows to slots -- a new page straight
-// from the pool, an old one from the table, so nothing waits for the table's
-// writes.  A few KB of traffic: bound by the latency of its dependent loads.
+// served, a thread a page writes the new table entries, and, for a step of up
+// to kPlanOwnTokens rows, a thread a row maps rows to slots -- a new page
+// straight from the pool, an old one from the table, so nothing waits for the
+// table's writes.  A few KB of traffic: bound by the latency of its dependent
+// loads.
 __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanParams p) {
   extern __shared__ int plan_smem[];
   int* start = plan_smem;              // [n_req] first row of each request, cut at n_tokens
-  int* first = plan_smem + p.n_req;    // [n_req] pool index of its first new page
+  int* first = plan_smem + p.n_req;    // [n_req] pages asked for ahead of it, its own pool index if it is served
   __shared__ int64_t warp_sum[32][2];
   __shared__ long long taken;
   __shared__ int rows;
@@ -129,7 +130,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanPara
       const bool ok = fits && (need == 0 || used + upto <= p.n_free);
       const int64_t s = end - n;
       start[r] = (int)(s < p.n_tokens ? s : p.n_tokens);
-      first[r] = ok ? (int)(used + upto - need) : -1;
+      first[r] = (int)min(upto - need, (int64_t)0x7fffffff);
       p.q_start[r] = start[r];
       p.kv_len[r] = ok ? c + n : 0;
       if (r == p.n_req - 1) {
@@ -142,13 +143,13 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanPara
   __syncthreads();
   if (threadIdx.x == 0) *p.n_used_out = (int)(used + taken);
 
-  const int lane = threadIdx.x & 31;
-  for (int r = threadIdx.x >> 5; r < p.n_req; r += blockDim.x >> 5) {
-    if (first[r] < 0) continue;
-    const int c = max(p.cached[r], 0), n = max(p.fresh[r], 0);
-    const int64_t held = ((int64_t)c + page_mask) >> p.page_log2;
-    const int64_t want = ((int64_t)c + n + page_mask) >> p.page_log2;
-    for (int64_t b = held + lane; b < want; b += 32) p.table[r * p.ld_table + b] = p.free_pages[first[r] + b - held];
+  // The pages handed out are the first `taken` asked for; page i belongs to the
+  // last request that starts at or before it and asked for some.
+  const int32_t* pool = p.free_pages + used;
+  for (int i = threadIdx.x; i < (int)taken; i += blockDim.x) {
+    const int r = row_request(first, p.n_req, i);
+    const int64_t held = ((int64_t)max(p.cached[r], 0) + page_mask) >> p.page_log2;
+    p.table[r * p.ld_table + held + i - first[r]] = pool[i];
   }
   if (p.n_tokens > kPlanOwnTokens) return;
   for (int t = threadIdx.x; t < p.n_tokens; t += blockDim.x) {
@@ -156,11 +157,11 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanPara
     int pos = 0;
     if (t < rows) {
       const int r = row_request(start, p.n_req, t);
-      if (first[r] >= 0) {
+      if (p.kv_len[r] > 0) {           // written by this CTA above
         const int c = max(p.cached[r], 0);
         pos = c + t - start[r];
         const int64_t held = ((int64_t)c + page_mask) >> p.page_log2, b = pos >> p.page_log2;
-        const int32_t page = b < held ? p.table[r * p.ld_table + b] : p.free_pages[first[r] + b - held];
+        const int32_t page = b < held ? p.table[r * p.ld_table + b] : pool[first[r] + b - held];
         slot = ((int64_t)page << p.page_log2) + (pos & page_mask);
       }
     }
@@ -238,8 +239,9 @@ int paged_plan(const int32_t* cached_len, const int32_t* new_len, int n_req, int
   static_assert(2 * kPlanMaxReq * sizeof(int) <= 64 * 1024, "planning kernel's shared memory");
   if (smem > 48 * 1024 - 1024)
     SMEAI_CUDA_TRY(cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024));
-  // enough threads for the requests and, where this CTA maps them, the rows
+  // enough threads for the requests, their pages (as many as rows, at most) and, where this CTA maps them, the rows
   int64_t work = n_req;
+  if (n_tokens > kPlanOwnTokens) work = kPlanThreads;
   if (n_tokens <= kPlanOwnTokens && n_tokens > work) work = n_tokens;
   const int threads = work >= kPlanThreads ? kPlanThreads : (int)((work + 31) / 32 * 32);
   SMEAI_CUDA_TRY(launch(paged_plan_kernel, dim3(1), dim3(threads < 128 ? 128 : threads), smem, stream, p));

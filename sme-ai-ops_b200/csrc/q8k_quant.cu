@@ -65,7 +65,8 @@ __global__ void rms_q8k_quantize_kernel(const float* __restrict__ x, int64_t ld_
 // Residual addition + RMSNorm + quantization, one CTA per row: h = x + resid
 // is formed once and kept in registers (kKeep 256-value blocks a warp) between
 // the two passes that the norm needs, so a row costs one read of x and of
-// resid, one write of h and one of the blocks: 13.1 bytes a value.  Blocks
+// resid, one write of h and one of the blocks: 13.1 bytes a value.  All loads
+// of a warp (the weight's too) go out together before anything waits; blocks
 // past kKeep a warp are read back from h by the lanes that wrote it.  No
 // __restrict__ on h: it may be x or resid.
 template <int kKeep>
@@ -78,58 +79,61 @@ __global__ void __launch_bounds__(512) add_rms_q8k_quantize_kernel(const float* 
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
   const int64_t row = blockIdx.x;
-  const float *xr = x + row * ld_x, *rr = resid + row * ld_r;
-  float* hr = h + row * ld_h;
-  float v[kKeep][8], a[8];
+  const float *xr = x + row * ld_x + lane * 8, *rr = resid + row * ld_r + lane * 8, *wr = norm_w + lane * 8;
+  float* hr = h + row * ld_h + lane * 8;
+  float v[kKeep][8], a[kKeep][8], g[kKeep][8];
 #pragma unroll
   for (int i = 0; i < kKeep; ++i) {
     const int b = warp + i * nwarps;
-    if (b < nb) load8(xr + b * QK_K + lane * 8, v[i]);
+    if (b < nb) {
+      load8(xr + b * QK_K, v[i]);
+      load8(rr + b * QK_K, a[i]);
+      if (norm_w) load8(wr + b * QK_K, g[i]);
+    }
   }
 #pragma unroll
   for (int i = 0; i < kKeep; ++i) {
     const int b = warp + i * nwarps;
     if (b < nb) {
-      load8(rr + b * QK_K + lane * 8, a);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = __fadd_rn(v[i][j], a[j]);
-      store8(hr + b * QK_K + lane * 8, v[i]);
+      for (int j = 0; j < 8; ++j) v[i][j] = __fadd_rn(v[i][j], a[i][j]);
+      store8(hr + b * QK_K, v[i]);
       const float s = group_sumsq_load8(v[i]);
       if ((lane & 3) == 0) sm_gsum[b * 8 + (lane >> 2)] = s;
     }
   }
   for (int b = warp + kKeep * nwarps; b < nb; b += nwarps) {
-    float t[8];
-    load8(xr + b * QK_K + lane * 8, t);
-    load8(rr + b * QK_K + lane * 8, a);
+    float t[8], u[8];
+    load8(xr + b * QK_K, t);
+    load8(rr + b * QK_K, u);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) t[j] = __fadd_rn(t[j], a[j]);
-    store8(hr + b * QK_K + lane * 8, t);
+    for (int j = 0; j < 8; ++j) t[j] = __fadd_rn(t[j], u[j]);
+    store8(hr + b * QK_K, t);
     const float s = group_sumsq_load8(t);
     if ((lane & 3) == 0) sm_gsum[b * 8 + (lane >> 2)] = s;
   }
   __syncthreads();
   // every warp folds the group sums itself: the same order, one barrier less
   const float inv = rms_inv_from_sum(rms_fold_groups(sm_gsum, nb * 8), nb * QK_K, eps);
-  auto finish = [&](float (&t)[8], int b) {
+  auto finish = [&](float (&t)[8], const float (&w)[8], int b) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) t[j] = __fmul_rn(t[j], inv);
     if (norm_w) {
-      load8(norm_w + b * QK_K + lane * 8, a);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) t[j] = __fmul_rn(t[j], a[j]);
+      for (int j = 0; j < 8; ++j) t[j] = __fmul_rn(t[j], w[j]);
     }
     q8k_store_global(q8k_quantize_lane(t), y + (row * nb + b) * Q8K_BLOCK_BYTES);
   };
 #pragma unroll
   for (int i = 0; i < kKeep; ++i) {
     const int b = warp + i * nwarps;
-    if (b < nb) finish(v[i], b);
+    if (b < nb) finish(v[i], g[i], b);
   }
   for (int b = warp + kKeep * nwarps; b < nb; b += nwarps) {
-    float t[8];
-    load8(hr + b * QK_K + lane * 8, t);
-    finish(t, b);
+    float t[8], w[8];
+    load8(hr + b * QK_K, t);
+    if (norm_w) load8(wr + b * QK_K, w);
+    finish(t, w, b);
   }
 }
 
@@ -173,9 +177,15 @@ int add_rms_q8k_quantize(const float* x, int64_t ld_x, const float* resid, int64
   const int nb = (int)(k / QK_K);
   const size_t smem = (size_t)8 * nb * 4;
   uint8_t* out = static_cast<uint8_t*>(y);
-  const int warps = nb < 16 ? nb : 16;
-  SMEAI_CUDA_TRY(launch(add_rms_q8k_quantize_kernel<2>, dim3((unsigned)n_rows), dim3(32 * warps), smem, stream, x,
-                        ld_x, resid, ld_r, nb, eps, norm_w, h, ld_h, out));
+  // Few rows: one block a warp, the shortest way through a row.  Many: two, so
+  // that twice the loads are in flight for every wait at the barrier.
+  const int per = n_rows <= 148 ? 1 : 2, warps = (nb + per - 1) / per < 16 ? (nb + per - 1) / per : 16;
+  if (nb <= warps)
+    SMEAI_CUDA_TRY(launch(add_rms_q8k_quantize_kernel<1>, dim3((unsigned)n_rows), dim3(32 * warps), smem, stream, x,
+                          ld_x, resid, ld_r, nb, eps, norm_w, h, ld_h, out));
+  else
+    SMEAI_CUDA_TRY(launch(add_rms_q8k_quantize_kernel<2>, dim3((unsigned)n_rows), dim3(32 * warps), smem, stream, x,
+                          ld_x, resid, ld_r, nb, eps, norm_w, h, ld_h, out));
   return kOk;
 }
 
