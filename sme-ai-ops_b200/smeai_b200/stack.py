@@ -14,6 +14,9 @@ attn_norm / ffn_norm / output_norm do):
     x   = x + Wd Q8_K(h)
 then logits = Wlm Q8_K(rmsnorm(x) * output_norm).
 
+step_cached runs the same layers for the new tokens of running sequences, with
+each layer's attention over a paged key/value cache (paged.py).
+
 Multi-GPU: every weight is row-sharded over the ranks (32-row aligned slices
 of each of Wq/Wk/Wv/Wo/Wg/Wu/Wd/Wlm); activations are replicated and each
 linear's output slices are all-gathered over NCCL.  Weights are drawn from a
@@ -316,6 +319,37 @@ class Q2KDecodeStack:
             L(self.lm, self.x, self.lg_loc, rms=True, qbuf=self.xq, norm_w=self.out_norm)
             self._gather(self.logits, self.lg_loc, self.v_lo, self.v_hi)
         return self.logits
+
+    # --------------------------------------------------------------- tokens of running sequences
+    def step_cached(self, x: torch.Tensor, plan, caches, max_new: int, rope: torch.Tensor | None = None) -> torch.Tensor:
+        """One step of a serving loop: x [T, hidden] fp32 holds the new tokens
+        of all requests behind one another (one each while decoding, a chunk of
+        a prompt, both), `plan` their PagedPlan, built, `caches` one PagedKV a
+        layer (hidden / head_dim key heads), rope a paged.rope_table.  Every
+        layer's attention is taken over the request's cached tokens; returns
+        logits [T, vocab].  Rows behind the last request's hold anything.  One
+        GPU; queued on the current stream without waiting."""
+        from . import paged
+        assert self.world == 1 and len(caches) == self.L and x.shape == (plan.n_tokens, self.H)
+        T, H, e = x.shape[0], self.H, self.eps
+        heads, D = caches[0].n_kv_heads, caches[0].head_dim
+        assert heads * D == H
+
+        def linear(m, xq, epilogue=EPI_STORE):
+            return (m.mul_mat_tc if T >= 16 else m.mul_mat)(xq, T, epilogue=epilogue)
+
+        h = x.clone()
+        xq = Q.rms_quantize_q8k(h, e, norm_w=self.attn_norm[0])
+        for li, (wqkv, wo, wgu, wd) in enumerate(self.layers):
+            q, k, v = linear(wqkv, xq).view(T, 3, heads, D).unbind(1)
+            q = paged.append(caches[li], k, v, plan.slots, q=q, positions=plan.positions, rope=rope)
+            ctx = paged.attention(q, caches[li], plan.block_table, plan.q_start, plan.kv_len, max_new)
+            y = linear(wo, Q.quantize_q8k(ctx.view(T, H).float()))
+            h, xq = Q.add_rms_quantize_q8k(y, h, e, norm_w=self.ffn_norm[li], sum_out=h)
+            y = linear(wd, Q.quantize_q8k(linear(wgu, xq, EPI_SILU_MUL)))
+            h, xq = Q.add_rms_quantize_q8k(y, h, e, sum_out=h,
+                                           norm_w=self.attn_norm[li + 1] if li + 1 < self.L else self.out_norm)
+        return linear(self.lm, xq)
 
     def _build_program(self):
         from . import IN_F32, IN_F32_RMS
