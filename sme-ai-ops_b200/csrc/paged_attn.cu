@@ -353,7 +353,12 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_few_ke
           }
         }
     }
-    uint32_t b[NQ][2];                 // P^T: 16 keys x 8 rows
+    // P^T, 16 keys x 8 rows: the weights rounded to the cache's type and, up to
+    // 16 rows, what the rounding left, rounded again: without it the weights'
+    // rounding adds as much error as the result's own.  The second product
+    // costs 1% there (the cache's bytes bound the kernel), 3 to 7% with 24 rows.
+    constexpr int kParts = NQ <= 2 ? 2 : 1;
+    uint32_t b[NQ * kParts][2];
 #pragma unroll
     for (int f = 0; f < NQ; ++f) {
       const float less[2] = {m[f][0] == kNegInf ? 0.f : Num<T>::kBias - m[f][0],
@@ -363,13 +368,24 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_few_ke
         s[f][i] = exp2_fast(fmaf(s[f][i], p.scale_log2, less[i & 1]));
         l[f][i & 1] += s[f][i];
       }
-      b[f][0] = transpose8(Num<T>::pack(s[f][0], s[f][1]));
-      b[f][1] = transpose8(Num<T>::pack(s[f][2], s[f][3]));
+#pragma unroll
+      for (int part = 0; part < kParts; ++part) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t two = Num<T>::pack(s[f][2 * i], s[f][2 * i + 1]);
+          b[f * kParts + part][i] = transpose8(two);
+          if (part + 1 < kParts) {
+            const float2 kept = Num<T>::unpack(two);
+            s[f][2 * i] -= kept.x;
+            s[f][2 * i + 1] -= kept.y;
+          }
+        }
+      }
     }
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d) {
 #pragma unroll
-      for (int f = 0; f < NQ; ++f) mma16816<T>(o[d][f], a[d % kAhead], b[f][0], b[f][1]);
+      for (int f = 0; f < NQ * kParts; ++f) mma16816<T>(o[d][f / kParts], a[d % kAhead], b[f][0], b[f][1]);
       const int then = d + kAhead;
       if (then < DP / 16) ldsm4_t(vt + v_off[then & 3] + (then >> 2) * 128, a[d % kAhead]);
     }
@@ -738,12 +754,12 @@ __global__ void __launch_bounds__(32 * kJoinWarps) paged_attn_join_kernel(const 
   }
 }
 
-// TR rows a tile: 8 to 24 on the few-row kernel, 64 on the other.
+// TR rows a tile: 8 to 24 on the few-row kernel, 64 on the other.  The joining
+// comes behind all kernels of a call (run_join).
 template <typename T, int DP, int TR>
-int run_class(AttnParams p, const PagedAttention& a, int sms, cudaStream_t stream) {
+int run_class(AttnParams& p, void* workspace, bool splits, int sms, cudaStream_t stream) {
   const int ctas = sms * Shape<DP>::kPerSm;
-  const bool splits = attn_splits<kKeys>(a.max_kv);
-  attn_carve<TR, DP>(p, splits ? a.workspace : nullptr, ctas);
+  attn_carve<TR, DP>(p, splits ? workspace : nullptr, ctas);
   void (*kernel)(AttnParams);
   size_t smem;
   if constexpr (TR == 64) {
@@ -756,20 +772,24 @@ int run_class(AttnParams p, const PagedAttention& a, int sms, cudaStream_t strea
   static std::atomic<uint64_t> allowed{0};
   SMEAI_CUDA_TRY(attn_allow_smem(kernel, smem, allowed));
   SMEAI_CUDA_TRY(launch(kernel, dim3((unsigned)ctas), dim3(kThreads), smem, stream, p));
-  if (splits) SMEAI_CUDA_TRY((attn_join<T, TR, DP>(p, ctas, stream)));
+  return kOk;
+}
+template <typename T, int DP, int TR>
+int run_join(const AttnParams& p, int sms, cudaStream_t stream) {
+  if (p.head) SMEAI_CUDA_TRY((attn_join<T, TR, DP>(p, sms * Shape<DP>::kPerSm, stream)));
   return kOk;
 }
 
 // Which kernels a call needs, from what the host knows: the largest request's
 // packed rows and the total.
 //   up to 8, 16, 24 rows  tiles of so many: one reading of the keys for all
-//   more                  the tensor-core kernel, and the 16-row tiles beside it
-//                         for requests of up to 16 rows (a step that mixes
-//                         prompts and decoding) unless the total says that
-//                         there are none: one row costs the tensor-core
-//                         kernel's tile as much as 128, and 8 requests, one of
-//                         860 rows, took 148 us without the second kernel and
-//                         104 us with it
+//   more                  the tensor-core kernel, and beside it the 8-row tiles
+//                         (16 with more than 8 heads a key head) for requests
+//                         of so few rows (a step that mixes prompts and
+//                         decoding) unless the total says that there are none:
+//                         one row costs the tensor-core kernel's tile as much
+//                         as 128, and 8 requests, one of 860 rows, took 148 us
+//                         without the second kernel and 104 us with it
 // head_dim above 128: up to 16 rows as above, more the 64-row tiles for all.
 struct Classes {
   int few;      // rows a tile of the few-row kernel; 0: not needed
@@ -783,34 +803,57 @@ Classes classes(const PagedAttention& a) {
   else if (most <= 24) c.few = 24;
   else {
     c.many = true;
-    // with one request of r <= 16 / group rows the others, of max_new at most, could not make up n_tokens
-    if (a.n_tokens <= (a.n_req - 1) * a.max_new + 16 / group) c.few = 16;
+    // with one request of so few rows the others, of max_new at most, could not make up more tokens
+    const int tile = group <= 8 ? 8 : 16;
+    if (a.n_tokens <= (a.n_req - 1) * a.max_new + tile / group) c.few = tile;
   }
   return c;
 }
 
 int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
+// Workspace of the few-row kernel, whichever its tile, a multiple of 256 bytes.
+size_t few_part_bytes(int dp, int max_kv, int sms) {
+  if (!attn_splits<kKeys>(max_kv)) return 0;
+  const size_t n = dp == 64    ? attn_part_bytes<24, 64>(2 * sms)
+                   : dp == 128 ? attn_part_bytes<24, 128>(2 * sms)
+                               : attn_part_bytes<16, 256>(sms);
+  return (n + 255) / 256 * 256;
+}
+
+template <typename T, int DP, int TR>
+int run_few(AttnParams p, const PagedAttention& a, const Classes& c, int sms, cudaStream_t stream) {
+  if (c.many) p.rows_hi = TR;
+  const bool splits = attn_splits<kKeys>(a.max_kv);
+  int st = run_class<T, DP, TR>(p, a.workspace, splits, sms, stream);
+  if (st) return st;
+  if constexpr (DP <= 128 && TR <= 16) {
+    if (c.many) {
+      // the tensor-core kernel in between: it has nothing to do with these
+      // partial results, and its set-up hides behind the first kernel's end
+      AttnParams q = p;
+      q.rows_hi = 0x7fffffff;
+      q.rows_lo = TR;
+      st = paged_attn_tc(q, DP, static_cast<char*>(a.workspace) + few_part_bytes(DP, a.max_kv, sms), a.max_kv, sms, stream);
+      if (st) return st;
+    }
+  }
+  return run_join<T, DP, TR>(p, sms, stream);
+}
+
 template <typename T, int DP>
 int run_dim(const AttnParams& p, const PagedAttention& a, int sms, cudaStream_t stream) {
   const Classes c = classes(a);
-  if (c.few) {
-    AttnParams q = p;
-    if (c.many) q.rows_hi = 16;
-    int st;
-    if (c.few == 8) st = run_class<T, DP, 8>(q, a, sms, stream);
-    else if (DP > 128 || c.few == 16) st = run_class<T, DP, 16>(q, a, sms, stream);
-    else st = run_class<T, DP, DP <= 128 ? 24 : 16>(q, a, sms, stream);
-    if (st) return st;
-  }
+  if (c.few == 8) return run_few<T, DP, 8>(p, a, c, sms, stream);
+  if (c.few == 16) return run_few<T, DP, 16>(p, a, c, sms, stream);
   if constexpr (DP > 128) {
-    if (c.mid) return run_class<T, DP, 64>(p, a, sms, stream);
-  } else if (c.many) {
     AttnParams q = p;
-    if (c.few) q.rows_lo = 16;
-    return paged_attn_tc(q, DP, a.workspace, a.max_kv, sms, stream);
+    const int st = run_class<T, DP, 64>(q, a.workspace, attn_splits<kKeys>(a.max_kv), sms, stream);
+    return st ? st : run_join<T, DP, 64>(q, sms, stream);
+  } else {
+    if (c.few == 24) return run_few<T, DP, 24>(p, a, c, sms, stream);
+    return paged_attn_tc(p, DP, a.workspace, a.max_kv, sms, stream);
   }
-  return kOk;
 }
 
 }  // namespace
@@ -830,13 +873,11 @@ size_t paged_attention_workspace(const PagedAttention& a) {
   if (sm_count(&sms)) return 0;
   const Classes c = classes(a);
   const int dp = padded_dim(a.kv.dim);
-  const size_t many = c.many ? paged_attn_tc_workspace(dp, a.max_kv, sms) : 0;
-  if (many) return many;                                 // the 16-row tiles' need is smaller
-  if ((c.many && !c.few) || !attn_splits<kKeys>(a.max_kv)) return 0;
-  if (c.mid) return attn_part_bytes<64, 256>(sms);
-  return dp == 64    ? attn_part_bytes<24, 64>(2 * sms)  // of 24 rows, whichever tile it is
-         : dp == 128 ? attn_part_bytes<24, 128>(2 * sms)
-                     : attn_part_bytes<16, 256>(sms);
+  size_t need = 0;
+  if (c.few) need += few_part_bytes(dp, a.max_kv, sms);
+  if (c.mid && attn_splits<kKeys>(a.max_kv)) need += attn_part_bytes<64, 256>(sms);
+  if (c.many) need += paged_attn_tc_workspace(dp, a.max_kv, sms);
+  return need;
 }
 
 int paged_attention(const PagedAttention& a, cudaStream_t stream) {
