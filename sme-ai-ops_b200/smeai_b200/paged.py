@@ -42,8 +42,10 @@ class PagedKV:
         self.k, self.v = k, v
         self.device, self.dtype = k.device, k.dtype
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
+        # the stride of a dimension of one element says nothing
+        strides = [st if n > 1 else self.head_dim for n, st in zip(k.shape, k.stride()[:3])]
         self.struct = KVCache(k.data_ptr(), v.data_ptr(), _TYPES[k.dtype], self.page_size, self.n_kv_heads, self.head_dim,
-                              self.n_pages, k.stride(0), k.stride(1), k.stride(2))
+                              self.n_pages, strides[0], strides[1], strides[2])
         self.ref = ctypes.byref(self.struct)
         self._workspace = {}         # bytes of attention()'s workspace, by sizes
 
@@ -61,16 +63,16 @@ class PagedPlan:
 
     def __init__(self, block_table: torch.Tensor, page_size: int, n_tokens: int):
         assert block_table.dim() == 2 and block_table.dtype == torch.int32 and block_table.is_cuda
-        assert block_table.stride(1) == 1 or block_table.shape[1] == 1
         self.block_table, self.page_size, self.n_tokens = block_table, page_size, n_tokens
         self.n_req, self.max_blocks = block_table.shape
+        ld_table = _table_stride(block_table)
         dev = block_table.device
         self.device = dev
         self.q_start = torch.zeros(self.n_req + 1, dtype=torch.int32, device=dev)
         self.kv_len = torch.zeros(self.n_req, dtype=torch.int32, device=dev)
         self.slots = torch.full((n_tokens,), -1, dtype=torch.int64, device=dev)
         self.positions = torch.zeros(n_tokens, dtype=torch.int32, device=dev)
-        self._out = (block_table.data_ptr(), max(self.max_blocks, block_table.stride(0)), self.max_blocks,
+        self._out = (block_table.data_ptr(), ld_table, self.max_blocks,
                      self.q_start.data_ptr(), self.kv_len.data_ptr(), self.slots.data_ptr(), self.positions.data_ptr(),
                      n_tokens)
 
@@ -89,6 +91,14 @@ class PagedPlan:
         call(dev, lib().smeai_paged_plan, "paged_plan", cached_len.data_ptr(), new_len.data_ptr(), n, self.page_size,
              free_pages.data_ptr(), free_pages.numel(), n_used.data_ptr(), used_out.data_ptr(), *self._out)
         return self
+
+
+def _table_stride(table: torch.Tensor) -> int:
+    """Entries between a block table's rows."""
+    n, blocks = table.shape
+    ld, one = table.stride()
+    assert (one == 1 or blocks <= 1) and (ld >= blocks or n <= 1), "a table's rows are contiguous and apart"
+    return ld if n > 1 else blocks
 
 
 def _rows(x: torch.Tensor, n: int, heads: int, dim: int, dtype, dev) -> int:
@@ -147,9 +157,9 @@ def attention(q: torch.Tensor, kv: PagedKV, block_table: torch.Tensor, q_start: 
     else:
         ld_out = _rows(out, n, heads, dim, kv.dtype, dev)
     n_req, max_blocks = block_table.shape
-    ld_table, one = block_table.stride()
+    ld_table = _table_stride(block_table)
     assert block_table.dtype == q_start.dtype == kv_len.dtype == torch.int32
-    assert block_table.device == q_start.device == kv_len.device == dev and (one == 1 or max_blocks <= 1)
+    assert block_table.device == q_start.device == kv_len.device == dev
     assert q_start.shape == (n_req + 1,) and kv_len.shape == (n_req,) and q_start.is_contiguous() and kv_len.is_contiguous()
     if n == 0:
         return out
@@ -161,7 +171,7 @@ def attention(q: torch.Tensor, kv: PagedKV, block_table: torch.Tensor, q_start: 
         workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         ws_ptr = workspace.data_ptr()
     call(dev, lib().smeai_paged_attention, "paged_attention", kv.ref, q.data_ptr(), ld_q, heads, n, q_start.data_ptr(),
-         kv_len.data_ptr(), n_req, block_table.data_ptr(), max(max_blocks, ld_table), max_blocks, max_new,
+         kv_len.data_ptr(), n_req, block_table.data_ptr(), ld_table, max_blocks, max_new,
          dim ** -0.5 if scale is None else scale, causal, out.data_ptr(), ld_out, ws_ptr, ws_bytes)
     return out
 

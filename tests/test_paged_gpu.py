@@ -391,3 +391,79 @@ def test_attention_streams_and_graphs(cuda):
     short = Problem(cuda, [(1, 5000), (1, 3)], 8, 2, 128, 16, F16, seed=10)
     short.kv_len.copy_(a.kv_len)
     assert torch.equal(oa, short.run())
+
+
+@pytest.mark.parametrize("n_req,chunk", [(130, 0), (700, 0), (400, 90)])
+def test_attention_many_requests(cuda, n_req, chunk):
+    """More requests than a CTA has threads; with a chunk both kernels run."""
+    g = torch.Generator().manual_seed(n_req)
+    lens = [(int(n), int(m)) for n, m in zip(torch.randint(0, 3, (n_req,), generator=g), torch.randint(0, 200, (n_req,), generator=g))]
+    if chunk:
+        lens[n_req // 2] = (chunk, 300)
+    p = Problem(cuda, lens, 4, 2, 64, 16, BF16, seed=13)
+    p.check(p.run())
+
+
+@pytest.mark.parametrize("n", [1, 90])
+def test_attention_rows_before_the_first_request(cuda, n):
+    p = Problem(cuda, [(n, 100), (n, 450)], 4, 2, 128, 16, F16, pad=6, seed=14)
+    p.q = p.q.roll(4, 0)
+    p.q_start += 4
+    p.starts = [s + 4 for s in p.starts]
+    out = torch.full_like(p.q, 3.0)
+    p.check(p.run(out=out))
+    assert (out[:4] == 3).all() and (out[4 + 2 * n:] == 3).all()
+
+
+@pytest.mark.parametrize("n,page", [(1, 16), (200, 16), (200, 4)])
+def test_attention_and_append_far_into_a_large_cache(cuda, n, page):
+    """Pages that lie more than 2^32 bytes apart."""
+    K, D, step = 2, 128, 1 << 27
+    blocks, far = -(-300 // page), 18
+    base = torch.zeros((far + 1) * step, dtype=F16, device=cuda)
+    shape, stride = (far + 1, K, page, D), (step, page * D, D, 1)
+    spread = [base.as_strided(shape, stride, o) for o in (0, 1 << 20)]
+    order = list(range(far, -1, -1))[:blocks]       # the last page first
+    m = min(300, len(order) * page)
+    p = Problem(cuda, [(n, m)], 4, K, D, page, F16, seed=16)
+    kr, vr = p.rows[0]
+    kv = paged.PagedKV(*spread)
+    pos = torch.arange(m, device=cuda)
+    slots = torch.tensor(order, device=cuda)[pos // page] * page + pos % page
+    paged.append(kv, kr.float(), vr.float(), slots)
+    table = torch.tensor([order], dtype=torch.int32, device=cuda)
+    assert torch.equal(spread[0][order[0], :, 0], kr[0]) and torch.equal(spread[1][order[1], :, 0], vr[page])
+    n_new = torch.tensor([0, n], dtype=torch.int32, device=cuda)
+    out = paged.attention(p.q, kv, table, n_new, p.kv_len, n)
+    p.check(out)
+
+
+def test_attention_bad_page_of_a_chunk_is_reported(cuda):
+    p = Problem(cuda, [(100, 300), (100, 300)], 4, 2, 128, 16, F16, seed=17)
+    want = p.run().clone()
+    table = p.table.clone()
+    table[1, 3], table[1, 7] = -5, 1 << 30
+    out = paged.attention(p.q, p.kv, table, p.q_start, p.kv_len, 100)
+    assert S.take_device_error() == 2 and torch.equal(out[:100], want[:100])
+
+
+def test_refused_tensors(cuda):
+    p = Problem(cuda, [(1, 40), (1, 40)], 2, 1, 64, 16, F16, seed=18)
+    args = (p.q_start, p.kv_len, 1)
+    with pytest.raises(AssertionError):      # one row for all requests
+        paged.attention(p.q, p.kv, p.table[:1].expand(2, -1), *args)
+    with pytest.raises(AssertionError):
+        paged.attention(p.q.float(), p.kv, p.table, *args)
+    with pytest.raises(AssertionError):
+        paged.attention(p.q, p.kv, p.table, p.q_start[:2], p.kv_len, 1)
+    with pytest.raises(AssertionError):
+        paged.attention(p.q.cpu(), p.kv, p.table, *args)
+    with pytest.raises(S.SmeaiError, match="workspace"):
+        big = torch.full((2, 100), -1, dtype=torch.int32, device=cuda)
+        paged.attention(p.q, p.kv, big, *args, workspace=torch.empty(256, dtype=torch.uint8, device=cuda))
+    with pytest.raises(S.SmeaiError, match="scale"):
+        paged.attention(p.q, p.kv, p.table, *args, scale=0.0)
+    one = p.k.new_empty((1, 1, 1, 64)).expand(3, -1, -1, -1)
+    with pytest.raises(S.SmeaiError, match="overlap"):
+        paged.append(paged.PagedKV(one, one), torch.zeros((1, 1, 64), device=cuda), torch.zeros((1, 1, 64), device=cuda),
+                     torch.zeros(1, dtype=torch.int64, device=cuda))
