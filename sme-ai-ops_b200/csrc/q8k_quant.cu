@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(512) add_rms_q8k_quantize_kernel(const float* 
                                                                    int64_t ld_r, int nb, float eps,
                                                                    const float* __restrict__ norm_w, float* h,
                                                                    int64_t ld_h, uint8_t* __restrict__ y) {
-  extern __shared__ float sm_gsum[];  // 8 group sums per block
+  extern __shared__ float sm_gsum[];  // 8 group sums per block, then 1/rms
   pdl_trigger();
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
@@ -140,8 +140,12 @@ __global__ void __launch_bounds__(512) add_rms_q8k_quantize_kernel(const float* 
     add_store(t, u, b);
   }
   __syncthreads();
-  // every warp folds the group sums itself: the same order, one barrier less
-  const float inv = rms_inv_from_sum(rms_fold_groups(sm_gsum, nb * 8), nb * QK_K, eps);
+  if (warp == 0) {
+    const float total = rms_fold_groups(sm_gsum, nb * 8);
+    if (lane == 0) sm_gsum[nb * 8] = rms_inv_from_sum(total, nb * QK_K, eps);
+  }
+  __syncthreads();
+  const float inv = sm_gsum[nb * 8];
 #pragma unroll
   for (int i = 0; i < kKeep; ++i) {
     const int b = warp + i * nwarps;
@@ -193,7 +197,7 @@ int add_rms_q8k_quantize(const float* x, int64_t ld_x, const float* resid, int64
     return kBadArgument;
   }
   const int nb = (int)(k / QK_K);
-  const size_t smem = (size_t)8 * nb * 4;
+  const size_t smem = (size_t)(8 * nb + 1) * 4;
   uint8_t* out = static_cast<uint8_t*>(y);
   auto wide = [](const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 4 == 0; };
   const bool aligned = wide(x, ld_x) && wide(resid, ld_r) && wide(h, ld_h) && wide(norm_w, 0);

@@ -152,7 +152,7 @@ def attention(q: torch.Tensor, kv: PagedKV, block_table: torch.Tensor, q_start: 
     n, heads = q.shape[0], q.shape[1]
     ld_q = _rows(q, n, heads, dim, kv.dtype, dev)
     if out is None:
-        out = torch.empty((n, heads, dim), dtype=kv.dtype, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         ld_out = heads * dim
     else:
         ld_out = _rows(out, n, heads, dim, kv.dtype, dev)

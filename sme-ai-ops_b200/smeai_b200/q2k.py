@@ -71,7 +71,7 @@ def add_rms_quantize_q8k(x: torch.Tensor, resid: torch.Tensor, eps: float, out: 
     n, k = x.shape
     dev = x.device
     if sum_out is None:
-        sum_out = torch.empty((n, k), dtype=torch.float32, device=dev)
+        sum_out = torch.empty_like(x, memory_format=torch.contiguous_format)
     if out is None:
         out = torch.empty((n, k // QK_K * Q8K_BLOCK_BYTES), dtype=torch.uint8, device=dev)
     assert x.is_cuda and x.dtype == resid.dtype == sum_out.dtype == torch.float32
