@@ -84,13 +84,35 @@ __device__ __forceinline__ int attn_blocks(const AttnParams& p, const AttnReq& r
   return max(1, (int)((unsigned)(keys + KB - 1) / KB));
 }
 
+// The same for every row tile of a request in turn, cheaply: where the group
+// divides TR a tile's last row is a fixed number of tokens behind the one
+// before's, and no division is left.
+template <int TR, int KB>
+struct AttnTiles {
+  int n_rt, step, keys;      // keys: what the last row of the next tile sees, before clamping
+  bool even;
+  __device__ __forceinline__ AttnTiles(const AttnParams& p, const AttnReq& r) {
+    n_rt = (int)((unsigned)(r.rows + TR - 1) / TR);
+    even = !p.causal || n_rt <= 1 || TR % p.group == 0;
+    step = !p.causal || n_rt <= 1 ? 0 : TR / p.group;
+    keys = step ? r.kv - r.n_new : r.kv;
+  }
+  // blocks of tile rt; called for rt = 0, 1, ..
+  __device__ __forceinline__ int next(const AttnParams& p, const AttnReq& r, int rt) {
+    if (!even) return attn_blocks<TR, KB>(p, r, rt);
+    keys += step;
+    const int k = rt + 1 == n_rt ? r.kv : max(0, min(r.kv, keys));
+    return max(1, (int)((unsigned)(k + KB - 1) / KB));
+  }
+};
+
 // Key blocks of all tiles of a request; `tiles` gets their number.
 template <int TR, int KB>
 __device__ __forceinline__ int64_t attn_units(const AttnParams& p, const AttnReq& r, int64_t& tiles) {
   int64_t u = 0;
-  const int n_rt = (r.rows + TR - 1) / TR;
-  for (int rt = 0; rt < n_rt; ++rt) u += attn_blocks<TR, KB>(p, r, rt);
-  tiles = (int64_t)n_rt * p.kv.n_kv;
+  AttnTiles<TR, KB> t(p, r);
+  for (int rt = 0; rt < t.n_rt; ++rt) u += t.next(p, r, rt);
+  tiles = (int64_t)t.n_rt * p.kv.n_kv;
   return u * p.kv.n_kv;
 }
 
@@ -180,9 +202,9 @@ __device__ void attn_share(const AttnParams& p, AttnShare* s, int64_t* warp_sum)
     int64_t at = line_lo, u = lo;
     for (int b = b0; b < b1; ++b) {
       const AttnReq r = attn_req(p, b);
-      const int n_rt = (r.rows + TR - 1) / TR;
-      for (int rt = 0; rt < n_rt; ++rt) {
-        const int nkb = attn_blocks<TR, KB>(p, r, rt);
+      AttnTiles<TR, KB> t(p, r);
+      for (int rt = 0; rt < t.n_rt; ++rt) {
+        const int nkb = t.next(p, r, rt);
         const int64_t len = (int64_t)(nkb + kCost) * p.kv.n_kv;
         if (cut >= at + len) {
           at += len;

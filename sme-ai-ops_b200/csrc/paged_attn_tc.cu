@@ -261,6 +261,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  if (kTma && threadIdx.x < 2)
+    asm volatile("prefetch.tensormap [%0];" ::"l"(threadIdx.x ? &maps.v : &maps.k) : "memory");
   pdl_wait();
   attn_share<kTR, kKB, kThreads>(p, &share, warp_sum);
   tc_fence_before();
