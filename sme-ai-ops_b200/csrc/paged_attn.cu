@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_few_ke
   constexpr int kChunks = DP / 8;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ AttnShare share;
-  __shared__ int64_t warp_sum[2 * kWarps];
+  __shared__ int64_t warp_sum[3 * kWarps];
   __shared__ float merge_m[kWarps][TR], merge_l[kWarps][TR];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t4 = lane & 3;
@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_mid_ke
   constexpr int TR = 64, kChunks = DP / 8;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ AttnShare share;
-  __shared__ int64_t warp_sum[2 * kWarps];
+  __shared__ int64_t warp_sum[3 * kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t ring = smem_addr(smem);
   uint8_t* q_tile = smem + (size_t)S::kStages * 2 * S::kTileBytes;

@@ -15,7 +15,10 @@
 // never split and need no joining.  On the line a tile is longer than its
 // blocks by what opening and ending it costs (measured: 5000 to 8000 cycles
 // against 2500 a block of 64 keys, 4000 against 3500 a block of 128), so a CTA
-// that gets many short tiles gets fewer blocks.
+// that gets many short tiles gets fewer blocks.  Where whole tiles dealt out by
+// their number take no longer than equal pieces and the splitting (kSplitCost
+// blocks), no tile is split: 128 tiles of 5 to 8 blocks on 148 CTAs are one
+// each, not none, one or two.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -30,6 +33,7 @@ namespace smeai {
 constexpr int kSnap = 3;
 template <int KB>
 constexpr int kTileCost = KB == 64 ? 2 : 1;   // in blocks
+constexpr int kSplitCost = 4;
 
 struct AttnParams {
   KvView kv;
@@ -106,12 +110,18 @@ struct AttnTiles {
   }
 };
 
-// Key blocks of all tiles of a request; `tiles` gets their number.
+// Key blocks of all tiles of a request; `tiles` gets their number, `most` is
+// raised to the longest one's blocks.
 template <int TR, int KB>
-__device__ __forceinline__ int64_t attn_units(const AttnParams& p, const AttnReq& r, int64_t& tiles) {
+__device__ __forceinline__ int64_t attn_units(const AttnParams& p, const AttnReq& r, int64_t& tiles, int& most) {
   int64_t u = 0;
   AttnTiles<TR, KB> t(p, r);
-  for (int rt = 0; rt < t.n_rt; ++rt) u += t.next(p, r, rt);
+#pragma unroll 1
+  for (int rt = 0; rt < t.n_rt; ++rt) {
+    const int nkb = t.next(p, r, rt);
+    u += nkb;
+    most = max(most, nkb);
+  }
   tiles = (int64_t)t.n_rt * p.kv.n_kv;
   return u * p.kv.n_kv;
 }
@@ -144,7 +154,7 @@ struct AttnShare {
 };
 
 // This CTA's piece of the line.  All threads of the block call it; the place
-// is in shared memory on return.  warp_sum: [2 * NT / 32] in shared memory.  Each
+// is in shared memory on return.  warp_sum: [3 * NT / 32] in shared memory.  Each
 // thread sums its own run of requests; the one whose run holds an end of the
 // piece walks to it.
 template <int TR, int KB, int NT>
@@ -154,9 +164,11 @@ __device__ void attn_share(const AttnParams& p, AttnShare* s, int64_t* warp_sum)
   const int per = (p.n_req + NT - 1) / NT;
   const int b0 = min((int)threadIdx.x * per, p.n_req), b1 = min(b0 + per, p.n_req);
   int64_t mine = 0, mine_t = 0;               // blocks, tiles
+  int most = 0;                               // blocks of the longest tile
+#pragma unroll 1
   for (int b = b0; b < b1; ++b) {
     int64_t t;
-    mine += attn_units<TR, KB>(p, attn_req(p, b), t);
+    mine += attn_units<TR, KB>(p, attn_req(p, b), t, most);
     mine_t += t;
   }
   int64_t incl = mine, incl_t = mine_t;
@@ -168,15 +180,18 @@ __device__ void attn_share(const AttnParams& p, AttnShare* s, int64_t* warp_sum)
       incl_t += t;
     }
   }
+  most = __reduce_max_sync(0xffffffffu, most);
   if (lane == 31) {
-    warp_sum[2 * warp] = incl;
-    warp_sum[2 * warp + 1] = incl_t;
+    warp_sum[3 * warp] = incl;
+    warp_sum[3 * warp + 1] = incl_t;
+    warp_sum[3 * warp + 2] = most;
   }
   __syncthreads();
   int64_t lo = incl - mine, lo_t = incl_t - mine_t, total = 0, total_t = 0;
 #pragma unroll
   for (int w = 0; w < NT / 32; ++w) {
-    const int64_t a = warp_sum[2 * w], t = warp_sum[2 * w + 1];
+    const int64_t a = warp_sum[3 * w], t = warp_sum[3 * w + 1];
+    most = max(most, (int)warp_sum[3 * w + 2]);
     if (w < warp) {
       lo += a;
       lo_t += t;
@@ -184,36 +199,48 @@ __device__ void attn_share(const AttnParams& p, AttnShare* s, int64_t* warp_sum)
     total += a;
     total_t += t;
   }
-  // lengths on the line, with the tiles' own costs
-  const int64_t line = total + kCost * total_t, line_lo = lo + kCost * lo_t, line_hi = line_lo + mine + kCost * mine_t;
-  // 64-bit division is slow, and lines are rarely that long
-  const int64_t per_cta = line <= 0x7fff0000 ? ((uint32_t)line + gridDim.x - 1) / gridDim.x
-                                             : (line + gridDim.x - 1) / gridDim.x;
+  // 64-bit division is slow, and these numbers are rarely that large
+  auto up = [](int64_t n, unsigned d) {
+    return n <= 0x7fff0000 ? (int64_t)(((uint32_t)n + d - 1) / d) : (n + d - 1) / d;
+  };
+  // lengths on the line: the tiles' blocks with their own costs, or 1 a tile
+  int64_t line = total + kCost * total_t, per_cta = up(line, gridDim.x);
+  const bool whole = up(total_t, gridDim.x) * (most + kCost) <= per_cta + kSplitCost;
+  int64_t line_lo = lo + kCost * lo_t, line_hi = line_lo + mine + kCost * mine_t;
+  if (whole) {
+    line = total_t;
+    per_cta = up(line, gridDim.x);
+    line_lo = lo_t;
+    line_hi = lo_t + mine_t;
+  }
   const int64_t cut0 = min(line, per_cta * blockIdx.x), cut1 = min(line, cut0 + per_cta);
   if (threadIdx.x == 0) {
     if (cut0 >= line) s->u0 = total;
     if (cut1 >= line) s->u1 = total;
   }
   // walk to each cut that lies in this run: the tile around it, and the edge it snaps to
-#pragma unroll
+#pragma unroll 1
   for (int which = 0; which < 2; ++which) {
     const int64_t cut = which ? cut1 : cut0;
     if (cut < line_lo || cut >= line_hi) continue;
     int64_t at = line_lo, u = lo;
+#pragma unroll 1
     for (int b = b0; b < b1; ++b) {
       const AttnReq r = attn_req(p, b);
       AttnTiles<TR, KB> t(p, r);
+#pragma unroll 1
       for (int rt = 0; rt < t.n_rt; ++rt) {
         const int nkb = t.next(p, r, rt);
-        const int64_t len = (int64_t)(nkb + kCost) * p.kv.n_kv;
+        const int one = whole ? 1 : nkb + kCost;
+        const int64_t len = (int64_t)one * p.kv.n_kv;
         if (cut >= at + len) {
           at += len;
           u += (int64_t)nkb * p.kv.n_kv;
           continue;
         }
         const int64_t in = cut - at;
-        const int h = len <= 0x7fffffff ? (int)((unsigned)in / (unsigned)(nkb + kCost)) : (int)(in / (nkb + kCost));
-        int kb = max(0, (int)(in - (int64_t)h * (nkb + kCost)) - kCost);
+        const int h = len <= 0x7fffffff ? (int)((unsigned)in / (unsigned)one) : (int)(in / one);
+        int kb = max(0, (int)(in - (int64_t)h * one) - kCost);   // 0 with whole tiles
         if (kb <= kSnap && kb <= nkb - kb) kb = 0;
         else if (nkb - kb <= kSnap) kb = nkb;           // the start of the next tile
         u += (int64_t)h * nkb + kb;

@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
   using C = Tc<DP>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ AttnShare share;
-  __shared__ int64_t warp_sum[2 * kThreads / 32];
+  __shared__ int64_t warp_sum[3 * kThreads / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const TcSmem m = carve<DP>(smem_raw);
 
