@@ -164,8 +164,9 @@ __device__ __forceinline__ float row_scale(float sum) {   // 0 rows for a sum of
 // 64 keys, with its own ring of keys in shared memory: warps never wait for
 // one another before the tile's end, where their maxima, sums and contexts
 // are merged (through the ring stage that the tile's last block left).  The
-// next tile's queries are copied while a tile is worked on.  A row's maximum is only raised when a score passes it by more
-// than 2^8, so most blocks need a vote and no reduction over the keys.
+// next tile's queries are copied while a tile is worked on.  A row's maximum is
+// only raised when a score passes it by more than 2^8, so most blocks need a
+// vote and no reduction over the keys.
 // Two CTAs an SM with 96 KB of keys and values in flight each cover HBM's
 // latency (44 GB/s x ~1 us = 44 KB an SM) through the ends of tiles; bound by
 // the cache's bytes.  Measured: 64 requests of 17 to 8192 keys, 32 query and 8
@@ -809,7 +810,7 @@ Classes classes(const PagedAttention& a) {
     c.many = true;
     // with one request of so few rows the others, of max_new at most, could not make up more tokens
     const int tile = group <= 8 ? 8 : 16;
-    if (a.n_tokens <= (a.n_req - 1) * a.max_new + tile / group) c.few = tile;
+    if (group <= tile && a.n_tokens <= (a.n_req - 1) * a.max_new + tile / group) c.few = tile;
   }
   return c;
 }

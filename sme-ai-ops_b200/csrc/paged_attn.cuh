@@ -277,8 +277,8 @@ __device__ __forceinline__ void attn_leave_part(const AttnParams& p, const AttnP
 // ---- 16-bit types ---------------------------------------------------------------
 // kBias: softmax weights are kept as 2^(kBias + s - m).  Half has 14 exponent
 // steps below 1; the bias moves the weights up so that ones as small as
-// 2^-24 of the largest keep their 11 bits, and 2^(kBias) and its 2^-8 lazily
-// updated maximum stay below 65504.  bfloat16 has fp32's range and needs none.
+// 2^-21 of the largest keep their 11 bits; with the 2^8 by which the maximum may
+// lag they stay below 65504.  bfloat16 has fp32's range and needs none.
 template <typename T>
 struct Num;
 template <>

@@ -18,7 +18,7 @@ def cur_stream() -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)     # None: a torch without CUDA
 
 
 def call(dev: torch.device, fn, what: str, *args) -> None:
