@@ -149,11 +149,6 @@ struct Loader {
   }
 };
 
-template <typename T>
-__device__ __forceinline__ float row_scale(float sum) {   // 0 rows for a sum of nothing, NaN kept
-  return sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
-}
-
 // ---- few rows -----------------------------------------------------------------
 // Tiles of 8 * NQ rows: a decode step's query heads of one key head, or those
 // of a few drafted tokens.  The products are taken transposed, with the keys
@@ -454,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_few_ke
           v[7] = fmaf(y.w, e[ww], v[7]);
         }
         if (whole) {
-          const float inv = row_scale<T>(sum);
+          const float inv = row_scale(sum);
           const int2 to = out_offset(w, w.rt * TR + f0 * 8 + r);
           if (d8 * 8 < p.kv.dim)
             *reinterpret_cast<uint4*>(p.out + (int64_t)to.x * p.ld_out + ((int64_t)to.y * p.kv.dim + d8 * 8) * 2) =
@@ -631,7 +626,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_mid_ke
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
       const int r = warp * 16 + g + 8 * i, row = w.rt * TR + r;
       if (row < w.r.rows && whole) {
-        const float inv = row_scale<T>(l[i]);
+        const float inv = row_scale(l[i]);
         const int tok = row / p.group, hd = w.h * p.group + row % p.group;
         char* dst = p.out + (int64_t)(w.r.q0 + tok) * p.ld_out + (int64_t)hd * p.kv.dim * 2;
 #pragma unroll
@@ -749,7 +744,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) paged_attn_join_kernel(const 
     }
   }
   if (row_t >= rows) return;
-  const float inv = row_scale<T>(l);
+  const float inv = row_scale(l);
   const int row = row0 + row_t, tok = row / p.group, head = hd.w * p.group + row % p.group;
   char* dst = p.out + (int64_t)(hd.x + tok) * p.ld_out + (int64_t)head * p.kv.dim * 2;
 #pragma unroll

@@ -306,6 +306,10 @@ struct Num<__nv_bfloat16> {
   }
 };
 
+// What a row's context is multiplied by in the end: nothing seen gives zeros,
+// NaN stays.
+__device__ __forceinline__ float row_scale(float sum) { return sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum); }
+
 // 2^x, the hardware's approximation (2 ulp; 2^-inf = 0).
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;

@@ -287,6 +287,19 @@ def test_attention_many_rows(cuda, dtype, causal, H, K, D, page):
     p.check(p.run(causal=causal), causal=causal)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype,H,K,D,page", [(F16, 8, 8, 128, 16), (BF16, 8, 8, 64, 32), (F16, 16, 8, 80, 4)])
+def test_attention_half_filled_tiles(cuda, dtype, causal, H, K, D, page):
+    """Rows for one half of a 256-row tile only, over one to nine blocks of 128
+    keys, so many of them that a CTA takes several, whole tiles in between."""
+    lens = [(n, m) for m in (1, 128, 129, 256, 300, 384, 385, 520, 1030, 1152) for n in (128 * K // H, 25, 64)]
+    lens += [(128 * K // H - 1, 100), (300, 700), (127, 64), (33, 2000), (1, 900), (256, 513), (26, 0), (31, 3000)]
+    p = Problem(cuda, lens, H, K, D, page, dtype, seed=20, spread=4.0)
+    out = p.run(causal=causal)
+    p.check(out, causal=causal)
+    assert torch.equal(out, p.run(causal=causal))
+
+
 @pytest.mark.parametrize("H,K,D,n,m", [(4, 1, 128, 1, 20000), (1, 1, 64, 1, 50001), (32, 8, 128, 3, 3001), (2, 1, 256, 1, 9000),
                                        (8, 8, 128, 300, 2500), (2, 1, 64, 1000, 1000), (1, 1, 128, 2, 30000)])
 def test_attention_split_over_ctas(cuda, H, K, D, n, m):
