@@ -14,8 +14,9 @@
 // snapped to a tile's edge when one is within kSnap units: short tiles are
 // never split and need no joining.  On the line a tile is longer than its
 // blocks by what opening and ending it costs (measured: 5000 to 8000 cycles
-// against 2500 a block of 64 keys, 4000 against 3500 a block of 128), so a CTA
-// that gets many short tiles gets fewer blocks.  Where whole tiles dealt out by
+// against 2500 a block of 64 keys, 8000 against 3000 a block of 128 and up to
+// 128 rows), so a CTA that gets many short tiles gets fewer blocks (24 requests
+// of 64 rows over 300 to 4096 keys: 1 block 76, 2 blocks 75.5, 3 blocks 67 us).  Where whole tiles dealt out by
 // their number take no longer than equal pieces and the splitting (kSplitCost
 // blocks), no tile is split: 128 tiles of 5 to 8 blocks on 148 CTAs are one
 // each, not none, one or two.
@@ -32,7 +33,7 @@ namespace smeai {
 
 constexpr int kSnap = 3;
 template <int KB>
-constexpr int kTileCost = KB == 64 ? 2 : 1;   // in blocks
+constexpr int kTileCost = KB == 64 ? 2 : 3;   // in blocks
 constexpr int kSplitCost = 4;
 
 struct AttnParams {
