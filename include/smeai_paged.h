@@ -63,6 +63,9 @@ typedef struct smeai_kv_cache {
  *                for a refused request's and for rows behind the last token
  *   positions    [n_tokens] the token's place in its sequence; 0 without slot
  *   n_used_out   *n_used plus the pages taken; may be n_used itself
+ * The lengths are read before anything is written: kv_len may be cached_len
+ * itself, so that one step's result is the next one's input (a refused
+ * request's length is then gone), and new_len may lie in q_start or kv_len.
  * n_req is at most 8192; n_tokens may be 0. */
 int smeai_paged_plan(const int32_t *cached_len, const int32_t *new_len, int64_t n_req, int page_size,
                      const int32_t *free_pages, int64_t n_free, const int32_t *n_used, int32_t *n_used_out,

@@ -82,16 +82,17 @@ struct PlanParams {
 // served, a thread a page writes the new table entries, and, for a step of up
 // to kPlanOwnTokens rows, a thread a row maps rows to slots -- a new page
 // straight from the pool, an old one from the table, so nothing waits for the
-// table's writes.  A few KB of traffic: bound by the latency of its dependent
-// loads.  Measured: 3.4 us for 48 decoding requests, 7.7 us for 200 prompts of
-// 51k rows, the second kernel included.
+// table's writes.  The lengths are read once, before anything is written, so
+// they may lie where kv_len or q_start go.  A few KB of traffic: bound by the
+// latency of its dependent loads.  Measured: 3.4 us for 48 decoding requests,
+// 7.7 us for 200 prompts of 51k rows, the second kernel included.
 __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanParams p) {
   extern __shared__ int plan_smem[];
-  int* start = plan_smem;              // [n_req] first row of each request, cut at n_tokens
-  int* first = plan_smem + p.n_req;    // [n_req] pages asked for ahead of it, its own pool index if it is served
+  int* start = plan_smem;                    // [n_req + 1] first row of each request, cut at n_tokens
+  int* first = plan_smem + p.n_req + 1;      // [n_req] pages asked for ahead of it, its own pool index if it is served
+  int* held_len = first + p.n_req;           // [n_req] cached tokens; ~ of it for a refused request
   __shared__ int64_t warp_sum[32][2];
   __shared__ long long taken;
-  __shared__ int rows;
   pdl_trigger();
   pdl_wait();
   const int page_mask = (1 << p.page_log2) - 1;
@@ -129,37 +130,37 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanPara
     carry[1] = c1[0];
     if (r < p.n_req) {
       const bool ok = fits && (need == 0 || used + upto <= p.n_free);
-      const int64_t s = end - n;
-      start[r] = (int)(s < p.n_tokens ? s : p.n_tokens);
+      start[r] = (int)min(end - n, p.n_tokens);
       first[r] = (int)min(upto - need, (int64_t)0x7fffffff);
-      p.q_start[r] = start[r];
-      p.kv_len[r] = ok ? c + n : 0;
-      if (r == p.n_req - 1) {
-        rows = (int)(end < p.n_tokens ? end : p.n_tokens);
-        p.q_start[p.n_req] = rows;
-      }
+      held_len[r] = ok ? c : ~c;
+      if (r == p.n_req - 1) start[p.n_req] = (int)min(end, p.n_tokens);
       if (ok && need > 0) atomicMax(&taken, (long long)upto);
     }
   }
   __syncthreads();
   if (threadIdx.x == 0) *p.n_used_out = (int)(used + taken);
+  for (int r = threadIdx.x; r <= p.n_req; r += blockDim.x) {
+    p.q_start[r] = start[r];
+    // a served request's rows all fit: they are its new tokens
+    if (r < p.n_req) p.kv_len[r] = held_len[r] < 0 ? 0 : held_len[r] + start[r + 1] - start[r];
+  }
 
   // The pages handed out are the first `taken` asked for; page i belongs to the
   // last request that starts at or before it and asked for some.
   const int32_t* pool = p.free_pages + used;
   for (int i = threadIdx.x; i < (int)taken; i += blockDim.x) {
     const int r = row_request(first, p.n_req, i);
-    const int64_t held = ((int64_t)max(p.cached[r], 0) + page_mask) >> p.page_log2;
+    const int64_t held = ((int64_t)held_len[r] + page_mask) >> p.page_log2;
     p.table[r * p.ld_table + held + i - first[r]] = pool[i];
   }
   if (p.n_tokens > kPlanOwnTokens) return;
   for (int t = threadIdx.x; t < p.n_tokens; t += blockDim.x) {
     int64_t slot = -1;
     int pos = 0;
-    if (t < rows) {
+    if (t < start[p.n_req]) {
       const int r = row_request(start, p.n_req, t);
-      if (p.kv_len[r] > 0) {           // written by this CTA above
-        const int c = max(p.cached[r], 0);
+      const int c = held_len[r];
+      if (c >= 0) {
         pos = c + t - start[r];
         const int64_t held = ((int64_t)c + page_mask) >> p.page_log2, b = pos >> p.page_log2;
         const int32_t page = b < held ? p.table[r * p.ld_table + b] : pool[first[r] + b - held];
@@ -188,7 +189,7 @@ __global__ void __launch_bounds__(256) paged_slots_kernel(const PlanParams p) {
     if (t < rows) {
       const int r = row_request(plan_smem, p.n_req, t);
       if (p.kv_len[r] > 0) {
-        pos = max(p.cached[r], 0) + t - plan_smem[r];
+        pos = p.kv_len[r] - (plan_smem[r + 1] - t);    // the last row is the last key
         const int32_t page = p.table[r * p.ld_table + (pos >> p.page_log2)];
         slot = ((int64_t)page << p.page_log2) + (pos & page_mask);
       }
@@ -236,10 +237,10 @@ int paged_plan(const int32_t* cached_len, const int32_t* new_len, int n_req, int
     set_last_error("paged_plan: no device error word");
     return kCudaError;
   }
-  const size_t smem = (size_t)2 * n_req * sizeof(int);
-  static_assert(2 * kPlanMaxReq * sizeof(int) <= 64 * 1024, "planning kernel's shared memory");
+  const size_t smem = ((size_t)3 * n_req + 1) * sizeof(int);
+  constexpr int kMaxSmem = (3 * kPlanMaxReq + 1) * (int)sizeof(int);
   if (smem > 48 * 1024 - 1024)
-    SMEAI_CUDA_TRY(cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024));
+    SMEAI_CUDA_TRY(cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
   // enough threads for the requests, their pages (as many as rows, at most) and, where this CTA maps them, the rows
   int64_t work = n_req;
   if (n_tokens > kPlanOwnTokens) work = kPlanThreads;

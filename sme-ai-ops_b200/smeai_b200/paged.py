@@ -80,7 +80,8 @@ class PagedPlan:
               used_out: torch.Tensor | None = None) -> "PagedPlan":
         """Fills the buffers for requests that hold cached_len tokens and bring
         new_len more; new pages come from free_pages, from index n_used[0] on,
-        which advances (in place, or into used_out)."""
+        which advances (in place, or into used_out).  cached_len may be this
+        plan's own kv_len (a refused request's length is then gone)."""
         if used_out is None:
             used_out = n_used
         i32, dev, n = torch.int32, self.device, self.n_req

@@ -108,6 +108,32 @@ def test_plan_negative_lengths_are_reported(cuda):
     assert plan.slots.tolist()[:2] == [50 * 4, 50 * 4 + 1] and plan.kv_len.tolist()[0] == 6
 
 
+@pytest.mark.parametrize("n_req,lo,hi,steps", [(3, 1, 1, 40), (1200, 0, 3, 6), (50, 100, 400, 3), (1, 9000, 9000, 2)])
+def test_plan_over_its_own_lengths(cuda, n_req, lo, hi, steps):
+    """One step's kv_len is the next one's cached_len, in place; rows on both
+    sides of the one-kernel limit.  New lengths lie in q_start every other step."""
+    page, g = 16, torch.Generator().manual_seed(n_req)
+    news = [torch.randint(lo, hi + 1, (n_req,), generator=g) for _ in range(steps)]
+    blocks = -(-hi * steps // page) + 1
+    T = n_req * hi + 3
+    pages = torch.randperm(n_req * blocks, generator=g).tolist()
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    plan = paged.PagedPlan(torch.full((n_req, blocks), -1, dtype=torch.int32, device=cuda), page, T)
+    free, used = i32(pages), i32([0])
+    cached, table, taken = [0] * n_req, [[-1] * blocks for _ in range(n_req)], 0
+    for step, new in enumerate(news):
+        new_len = new.to(torch.int32).to(cuda)
+        if step % 2:
+            plan.q_start[:n_req] = new_len
+            new_len = plan.q_start[:n_req]
+        plan.build(plan.kv_len, new_len, free, used)
+        table, start, cached, slots, pos, taken = plan_reference(cached, new.tolist(), page, pages, taken, table, T, blocks)
+        assert plan.kv_len.tolist() == cached and plan.q_start.tolist() == start and used.item() == taken
+        assert plan.block_table.tolist() == table
+        assert plan.slots.tolist() == slots and plan.positions.tolist() == pos
+    assert S.take_device_error() == 0
+
+
 # ---- append ------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
