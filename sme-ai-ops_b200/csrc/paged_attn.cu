@@ -2,11 +2,11 @@
 // requests that bring few rows (a decoding step, drafted tokens, short
 // chunks), and the joining of partial results.
 //
-//   o_r = sum_j p_rj v_j / sum_j p_rj,   p_rj = 2^(c s_rj - m_r),
-//   s_rj = q_r . k_j,  c = scale log2(e),  m_r = max over the keys seen so far of c s_rj
+//   o_r = sum_j p_rj v_j / sum_j p_rj,   p_rj = 2^(c (s_rj - m_r)),
+//   s_rj = q_r . k_j,  c = scale log2(e),  m_r = max over the keys seen so far of s_rj
 //
 // in one pass over the keys: when m_r grows by d, the sum and the context
-// gathered so far are multiplied by 2^-d.
+// gathered so far are multiplied by 2^(-c d).
 #include "paged_attn.cuh"
 
 namespace smeai {
@@ -169,7 +169,6 @@ struct Loader {
 // of 64: 38 us (28 of them here, 5 until the first block is computed, the rest
 // the joining); 24 requests with 2 to 6 drafted tokens (24-row tiles): 54 us =
 // 4.3 TB/s, where opening and ending a tile costs 2 to 3 us of a CTA's time.
-constexpr float kRaise = 8.f;
 
 // 8x8 16-bit transpose across the warp.
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
@@ -233,8 +232,8 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_few_ke
   // Scores and contexts of this lane: rows 2 t4 and 2 t4 + 1 of each eight.
   uint32_t qf[DP / 16][NQ][2];
   float o[DP / 16][NQ][4];
-  float m[NQ][2], l[NQ][2];
-  float most[NQ][2];                   // scores (before the scale) that leave the maximum as it is
+  float m[NQ][2], base[NQ][2], l[NQ][2];
+  const float lag = raise_lag(p.scale_log2);
   int lim[NQ][2], lim_all = 0;
   AttnPos next = w;
   int tile_kb0 = w.kb, tile = 0;
@@ -275,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_few_ke
         for (int i = 0; i < 2; ++i) {
           const int row = w.rt * TR + f * 8 + 2 * t4 + i;
           lim[f][i] = row < w.r.rows ? min(w.r.kv, attn_limit(p, w.r, row)) : 0;
-          m[f][i] = most[f][i] = kNegInf;
+          m[f][i] = base[f][i] = kNegInf;
           l[f][i] = 0.f;
         }
       }
@@ -330,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_few_ke
 #pragma unroll
     for (int f = 0; f < NQ; ++f)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) raise |= s[f][i] > most[f][i & 1];
+      for (int i = 0; i < 4; ++i) raise |= s[f][i] > (base[f][i & 1] == m[f][i & 1] ? m[f][i & 1] + lag : kNegInf);
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
       for (int f = 0; f < NQ; ++f)
@@ -339,17 +338,20 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_few_ke
           float top = fmaxf(s[f][i], s[f][i + 2]);
 #pragma unroll
           for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-          top *= p.scale_log2;
           if (top > m[f][i]) {
-            const float e = exp2_fast(m[f][i] - top);   // m = -inf: 0
+            const float e = exp2_fast((m[f][i] - top) * p.scale_log2);   // m = -inf: 0
             m[f][i] = top;
-            most[f][i] = (top + kRaise) / p.scale_log2;
+            base[f][i] = row_base(top, p.scale_log2);
             l[f][i] *= e;
 #pragma unroll
             for (int d = 0; d < DP / 16; ++d) {
               o[d][f][i] *= e;
               o[d][f][i + 2] *= e;
             }
+          }
+          if (base[f][i] != m[f][i]) {
+            s[f][i] -= m[f][i];
+            s[f][i + 2] -= m[f][i];
           }
         }
     }
@@ -361,11 +363,10 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_few_ke
     uint32_t b[NQ * kParts][2];
 #pragma unroll
     for (int f = 0; f < NQ; ++f) {
-      const float less[2] = {m[f][0] == kNegInf ? 0.f : Num<T>::kBias - m[f][0],
-                             m[f][1] == kNegInf ? 0.f : Num<T>::kBias - m[f][1]};
+      const float plus[2] = {base_offset<T>(base[f][0], p.scale_log2), base_offset<T>(base[f][1], p.scale_log2)};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        s[f][i] = exp2_fast(fmaf(s[f][i], p.scale_log2, less[i & 1]));
+        s[f][i] = exp2_fast(fmaf(s[f][i], p.scale_log2, plus[i & 1]));
         l[f][i & 1] += s[f][i];
       }
 #pragma unroll
@@ -434,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_few_ke
 #pragma unroll
         for (int ww = 0; ww < kWarps; ++ww) {
           const float mw = merge_m[ww][f0 * 8 + r];
-          e[ww] = mw == kNegInf ? 0.f : exp2_fast(mw - top);
+          e[ww] = mw == kNegInf ? 0.f : exp2_fast((mw - top) * p.scale_log2);
           sum = fmaf(merge_l[ww][f0 * 8 + r], e[ww], sum);
           const float4* src = reinterpret_cast<const float4*>(left + (r >> 3) * (S::kTileBytes / 4) + ww * 8 * DP +
                                                               (r & 7) * DP + ((d8 * 8) ^ (((r & 7) >> 1) * 8)));
@@ -507,7 +508,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_mid_ke
 
   const int g = lane >> 2, t4 = lane & 3;
   float o[DP / 8][4];
-  float m[2], l[2];
+  float m[2], base[2], l[2];
   int lim[2], lim_all = 0;
   int tile_kb0 = w.kb;
   auto open_tile = [&]() {
@@ -517,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_mid_ke
     for (int i = 0; i < 2; ++i) {
       const int row = w.rt * TR + warp * 16 + g + 8 * i;
       lim[i] = row < w.r.rows ? min(w.r.kv, attn_limit(p, w.r, row)) : 0;
-      m[i] = kNegInf;
+      m[i] = base[i] = kNegInf;
       l[i] = 0.f;
     }
 #pragma unroll
@@ -575,27 +576,33 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_mid_ke
     for (int i = 0; i < 2; ++i) {
       mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
       mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-      mx[i] = fmaxf(m[i], mx[i] * p.scale_log2);
     }
-    if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
+    if (__any_sync(0xffffffffu, mx[0] > (base[0] == m[0] ? m[0] : kNegInf) || mx[1] > (base[1] == m[1] ? m[1] : kNegInf))) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float e = mx[i] > m[i] ? exp2_fast(m[i] - mx[i]) : 1.f;   // m = -inf: 0
-        m[i] = mx[i];
+        const float e = mx[i] > m[i] ? exp2_fast((m[i] - mx[i]) * p.scale_log2) : 1.f;   // m = -inf: 0
+        m[i] = fmaxf(m[i], mx[i]);
+        base[i] = m[i] == kNegInf ? m[i] : row_base(m[i], p.scale_log2);
         l[i] *= e;
 #pragma unroll
         for (int d = 0; d < DP / 8; ++d) {
           o[d][2 * i] *= e;
           o[d][2 * i + 1] *= e;
         }
+        const float less = base[i] == m[i] ? 0.f : m[i];
+#pragma unroll
+        for (int n = 0; n < kKeys / 8; ++n) {
+          s[n][2 * i] -= less;
+          s[n][2 * i + 1] -= less;
+        }
       }
     }
-    const float sub[2] = {m[0] == kNegInf ? 0.f : Num<T>::kBias - m[0], m[1] == kNegInf ? 0.f : Num<T>::kBias - m[1]};
+    const float plus[2] = {base_offset<T>(base[0], p.scale_log2), base_offset<T>(base[1], p.scale_log2)};
 #pragma unroll
     for (int n = 0; n < kKeys / 8; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        s[n][i] = exp2_fast(fmaf(s[n][i], p.scale_log2, sub[i >> 1]));
+        s[n][i] = exp2_fast(fmaf(s[n][i], p.scale_log2, plus[i >> 1]));
         l[i >> 1] += s[n][i];
       }
 #pragma unroll
@@ -660,9 +667,11 @@ constexpr int kJoinWarps = 32;
 // a row when there are fewer rows, each taking every w-th piece with a running
 // maximum of its own; a row's warps meet in shared memory in warp order.  The
 // pieces were just written, so they come from L2; bound by the latency of
-// three dependent reads (7 to 8 us alone, 11 for 8 rows of 74 pieces).
+// three dependent reads (7 to 8 us alone, 11 for 8 rows of 74 pieces).  Two CTAs
+// an SM: all of the few-row kernel's CTAs are joined at once (a second round
+// cost a prompt beside decoding requests 7 of 99 us).
 template <typename T, int TR, int DP>
-__global__ void __launch_bounds__(32 * kJoinWarps) paged_attn_join_kernel(const AttnParams p, int ctas) {
+__global__ void __launch_bounds__(32 * kJoinWarps, DP <= 128 ? 2 : 1) paged_attn_join_kernel(const AttnParams p, int ctas) {
   constexpr int kRows = TR < kJoinWarps ? TR : kJoinWarps;    // rows a CTA joins
   constexpr int kCols = DP >= 128 ? 4 : 2;                    // consecutive columns a lane
   constexpr int kN = DP / 32;                                 // columns a lane
@@ -713,9 +722,10 @@ __global__ void __launch_bounds__(32 * kJoinWarps) paged_attn_join_kernel(const 
         else *reinterpret_cast<float2*>(v + 2 * s) = *reinterpret_cast<const float2*>(src + s * 64);
       }
       const bool some = ml.y != 0.f;    // or it saw no key, and its context may not have been written
-      const float top = some ? fmaxf(m, ml.x) : m;
-      const float f = m == top ? 1.f : exp2_fast(m - top), e = some ? exp2_fast(ml.x - top) : 0.f;
-      m = top;
+      const bool up = some && ml.x > m;
+      const float t = exp2_fast(-fabsf((m - ml.x) * p.scale_log2));   // of the lower maximum
+      const float f = up ? t : 1.f, e = up ? 1.f : some ? t : 0.f;
+      if (up) m = ml.x;
       l = fmaf(ml.y, e, l * f);
 #pragma unroll
       for (int k = 0; k < kN; ++k) a[k] = fmaf(some ? v[k] : 0.f, e, a[k] * f);
@@ -729,14 +739,14 @@ __global__ void __launch_bounds__(32 * kJoinWarps) paged_attn_join_kernel(const 
     if (part || row_t >= rows) return;
     float top = m;
     for (int w = 1; w < share; ++w) top = fmaxf(top, wml[warp + w].x);
-    const float f = m == kNegInf ? 0.f : exp2_fast(m - top);
+    const float f = m == kNegInf ? 0.f : exp2_fast((m - top) * p.scale_log2);
     l *= f;
 #pragma unroll
     for (int k = 0; k < kN; ++k) a[k] *= f;
     for (int w = 1; w < share; ++w) {
       const float2 ml = wml[warp + w];
       if (ml.y == 0.f) continue;
-      const float e = exp2_fast(ml.x - top);
+      const float e = exp2_fast((ml.x - top) * p.scale_log2);
       l = fmaf(ml.y, e, l);
 #pragma unroll
       for (int k = 0; k < kN; ++k)

@@ -49,7 +49,7 @@ struct AttnParams {
   int causal;
   int rows_lo, rows_hi;   // requests with rows_lo < rows <= rows_hi are this launch's
   float* part_o;          // [2 * CTAs][TR][DP]
-  float2* part_ml;        // [2 * CTAs][TR] running maximum (log2 units), sum
+  float2* part_ml;        // [2 * CTAs][TR] running maximum (before the scale), sum
   int4* head;             // [CTAs] tile left unfinished at the end {first row of its request or -1, the
                           // request's packed rows, row tile, key head}
   int* state;             // [CTAs] state of slot 0
@@ -310,6 +310,22 @@ struct Num<__nv_bfloat16> {
 // What a row's context is multiplied by in the end: nothing seen gives zeros,
 // NaN stays.
 __device__ __forceinline__ float row_scale(float sum) { return sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum); }
+
+// A row's weights are 2^(kBias + c (s - m)), c = scale * log2(e): one fused
+// multiply-add a score, c s + (kBias - c m), as exact as the second part.  Once
+// c m passes 2^22, where fp32 has steps of half and more, the scores are
+// subtracted first, which is exact near the maximum.  `base` is what the
+// multiply-add subtracts: m, or 0 for such a far row.  A far row's maximum may
+// not lag, and any score of it opens the branch in which maxima are raised:
+// the subtraction is there and costs other rows nothing.
+constexpr float kRaise = 8.f;          // growth of the maximum (log2) that rescales what was gathered
+constexpr float kFar = 4194304.f;
+__device__ __forceinline__ float row_base(float m, float c) { return fabsf(m) * c < kFar ? m : 0.f; }
+__device__ __forceinline__ float raise_lag(float c) { return fminf(kRaise / c, 1e38f); }   // -inf plus it is -inf
+template <typename T>
+__device__ __forceinline__ float base_offset(float base, float c) {
+  return base == -INFINITY ? 0.f : fmaf(-base, c, Num<T>::kBias);
+}
 
 // 2^x, the hardware's approximation (2 ulp; 2^-inf = 0).
 __device__ __forceinline__ float exp2_fast(float x) {

@@ -5,7 +5,7 @@
 // The mathematics is that of paged_attn.cu, on tiles of 256 packed rows (two
 // halves of 128, the MMA's M) and blocks of 128 keys:
 //   S_t = Q_t K^T      tcgen05.mma, both operands in shared memory, fp32 in TMEM
-//   P_t = 2^(c S_t - m) in registers: a thread owns a row, so its maximum and
+//   P_t = 2^(c (S_t - m)) in registers: a thread owns a row, so its maximum and
 //                      sum need no exchange; P replaces S in TMEM as 16-bit pairs
 //   O_t += P_t V       tcgen05.mma with P read from TMEM, O fp32 in TMEM
 // The running maximum is only raised when it grows by more than 2^8 (P then
@@ -62,7 +62,6 @@ constexpr int kTmaMinPage = 8;       // tokens
 // 384 threads x 168 registers at launch = 256 x 208 + 128 x 88
 constexpr int kAtom = 128 * 128;     // 128 rows x 128 bytes
 constexpr int kTmemCols = 512;       // S0 S1 (128 columns each), O0 O1 (up to 128 each)
-constexpr float kRaise = 8.f;        // growth of the maximum (log2) that rescales O
 constexpr float kNegInf = -INFINITY;
 
 template <int DP>
@@ -587,7 +586,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
       const int lim = live ? min(w.r.kv, attn_limit(p, w.r, row)) : 0;
       const int lim_all = min(w.r.kv, attn_limit(p, w.r, row - r));
       const bool dead = row - lane >= w.r.rows;
-      float mx = kNegInf, l = 0.f;
+      // plus: what the multiply-add adds; of a far row, or before the first maximum, so large that any score is above
+      constexpr float kOpens = 3.4e38f;
+      float mx = kNegInf, plus = kOpens, l = 0.f;
       const int cnt = s.cnt[t];
       for (int b = 0; b < cnt; ++b) {
         if (!(ok = wait_warp(m, &m.s_full[t], sc & 1, p.err, limit_ns))) break;
@@ -619,11 +620,24 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
 #pragma unroll
         for (int k = 0; k < 8; ++k) top[k] = fmaxf(top[k], v[120 + k]);
         const float mn = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])),
-                               fmaxf(fmaxf(top[4], top[5]), fmaxf(top[6], top[7]))) * p.scale_log2;
-        const bool raise = mn > mx + kRaise || (mx == kNegInf && mn > mx);
-        if (__any_sync(0xffffffffu, raise)) {
-          const float f = raise ? exp2_fast(mx - mn) : 1.f;
-          if (raise) mx = mn;
+                               fmaxf(fmaxf(top[4], top[5]), fmaxf(top[6], top[7])));
+        const bool open = fmaf(mn, p.scale_log2, plus) > Num<T>::kBias + kRaise;
+        float add = plus;
+        if (__any_sync(0xffffffffu, open)) {
+          const bool raise = open && mn > mx;
+          const float f = raise ? exp2_fast((mx - mn) * p.scale_log2) : 1.f;   // mx = -inf: 0
+          if (raise) {
+            mx = mn;
+            plus = row_base(mn, p.scale_log2) == mn ? base_offset<T>(mn, p.scale_log2) : kOpens;
+          }
+          add = plus;
+          if (__any_sync(0xffffffffu, plus == kOpens)) {
+            const bool far = plus == kOpens && mx > kNegInf;
+            const float less = far ? mx : 0.f;
+            if (far) add = Num<T>::kBias;
+#pragma unroll
+            for (int i = 0; i < 128; ++i) v[i] -= less;
+          }
           l *= f;
           if (b > 0) {
 #pragma unroll 1
@@ -638,15 +652,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
             }
           }
         }
-        const float sub = mx == kNegInf ? 0.f : Num<T>::kBias - mx;
-        const uint64_t c2 = pack_f32x2(p.scale_log2, p.scale_log2), sub2 = pack_f32x2(sub, sub);
+        const uint64_t c2 = pack_f32x2(p.scale_log2, p.scale_log2), add2 = pack_f32x2(add, add);
         uint64_t sum2[2] = {0ull, 0ull};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           uint32_t w16[16];
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
-            const uint64_t x = fma_f32x2(pack_f32x2(v[i * 32 + 2 * k], v[i * 32 + 2 * k + 1]), c2, sub2);
+            const uint64_t x = fma_f32x2(pack_f32x2(v[i * 32 + 2 * k], v[i * 32 + 2 * k + 1]), c2, add2);
             const float e0 = exp2_fast(__uint_as_float((uint32_t)x)), e1 = exp2_fast(__uint_as_float((uint32_t)(x >> 32)));
             sum2[k & 1] = add_f32x2(sum2[k & 1], pack_f32x2(e0, e1));
             w16[k] = Num<T>::pack(e0, e1);
@@ -692,8 +705,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
         ++xc;
         const float2 ml = dead ? make_float2(kNegInf, 0.f) : m.x_ml[r];
         const float top = fmaxf(mx, ml.x);
-        f0 = mx == kNegInf ? 0.f : exp2_fast(mx - top);
-        f1 = ml.x == kNegInf ? 0.f : exp2_fast(ml.x - top);
+        f0 = mx == kNegInf ? 0.f : exp2_fast((mx - top) * p.scale_log2);
+        f1 = ml.x == kNegInf ? 0.f : exp2_fast((ml.x - top) * p.scale_log2);
         l = fmaf(ml.y, f1, l * f0);
         mx = top;
       }

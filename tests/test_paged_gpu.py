@@ -376,6 +376,29 @@ def test_attention_large_scores_and_scale(cuda):
         assert ((out[lo:hi].double() - ref).abs() <= 1.01 * (half * ref.abs() + (half + 8e-4) * size) + 2.0 ** -25).all()
 
 
+@pytest.mark.parametrize("scale", [2.0 ** -7, 2.0 ** -4])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("H,K,D,lens", [(4, 1, 128, [(1, 900), (1, 20000), (1, 70)]), (4, 1, 64, [(4, 900), (3, 5000)]),
+                                        (4, 2, 128, [(12, 900), (10, 6000)]), (2, 1, 256, [(40, 900), (9, 5000)]),
+                                        (4, 2, 128, [(200, 900), (300, 5000), (20, 3000), (1, 600)])])
+def test_attention_far_scores(cuda, dtype, scale, H, K, D, lens):
+    """Scores of +-2^30 + 128 j, j of 0 to 11, which fp32 holds exactly (2^30 has
+    steps of 128): times the scale they are +-2^23 + j and +-2^26 + 8 j, where
+    fp32 has steps of one to eight.  The weights are e^j and e^8j all the same."""
+    p = Problem(cuda, lens, H, K, D, 16, dtype, seed=21)
+    g = torch.Generator(device=cuda).manual_seed(22)
+    p.q.zero_()
+    p.q[..., 0], p.q[..., 1] = 2.0 ** 15, 8.0
+    for i, ((_, m), (kr, _)) in enumerate(zip(p.lens, p.rows)):
+        kr[..., 0] = 2.0 ** 15 if i % 2 else -2.0 ** 15
+        kr[..., 1] = 16 * torch.randint(0, 12, kr.shape[:2], generator=g, device=cuda).to(dtype)
+        at = torch.arange(m, device=cuda)
+        p.k[p.table[i, at // 16].long(), :, at % 16] = kr
+    out = p.run(scale=scale)
+    # the scale is rounded twice on its way: 17 * 8 octaves * 2^-23 = 2e-5 of a weight, inside check()'s 1e-4
+    p.check(out, scale=scale)
+
+
 def test_attention_infinities_stay_in_their_request(cuda):
     p = Problem(cuda, [(1, 100), (3, 80), (1, 70)], 4, 2, 64, 16, F16, seed=8)
     clean = p.run().clone()
