@@ -97,7 +97,7 @@ int smeai_paged_append(const smeai_kv_cache *cache, const float *k, int64_t ld_k
  * head_dim values of the cache's type a row, row strides ld_q and ld_out
  * elements (multiples of 8), 16-byte aligned; n_tokens rows; out and q do not
  * overlap; rows of out outside q_start[0] .. q_start[n_req] are left as they
- * were.  Scores, softmax
+ * were.  scale is positive, up to 2e38.  Scores, softmax
  * and the running sums are fp32; the softmax weights are rounded to the
  * cache's type for the tensor cores.  Slots past kv_len are never read, so
  * they may hold anything; a NaN or infinity within reaches the rows of its own

@@ -28,6 +28,7 @@ int log2_of(int64_t n) {   // -1: not a power of two
   return l;
 }
 
+constexpr float kLog2e = 1.4426950408889634f;
 constexpr int64_t kMaxStride = (int64_t)1 << 40;   // elements; keeps every byte offset inside 64 bits
 
 int view(const char* what, const smeai_kv_cache* c, KvView* v) {
@@ -168,7 +169,7 @@ int smeai_paged_attention(const smeai_kv_cache* cache, const void* q, int64_t ld
     return bad(what, "a row stride of q or out is smaller than n_heads * head_dim");
   if (!aligned16(q) || !aligned16(out) || ld_q % 8 || ld_out % 8) return bad(what, "rows of q and out are 16-byte aligned");
   if (ld_table < max_blocks) return bad(what, "ld_table is at least max_blocks");
-  if (!(scale > 0.f) || isinf(scale)) return bad(what, "scale is positive and finite");
+  if (!(scale > 0.f) || isinf(scale * kLog2e)) return bad(what, "scale is positive and at most 2e38");
   st = ready(what);
   if (st) return st;
   const size_t need = paged_attention_workspace(a);

@@ -905,7 +905,7 @@ int paged_attention(const PagedAttention& a, cudaStream_t stream) {
   p.max_kv = a.max_kv;
   p.n_tokens = (int)a.n_tokens;
   p.group = a.n_heads / a.kv.n_kv;
-  p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.scale_log2 = a.scale * 1.4426950408889634f;   // finite: the entry point checks it
   p.causal = a.causal ? 1 : 0;
   p.rows_lo = 0;
   p.rows_hi = 0x7fffffff;

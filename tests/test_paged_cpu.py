@@ -75,6 +75,12 @@ def test_attention_refuses(kw):
     assert attention(**kw) == BAD and S.last_error().startswith("smeai_paged_attention")
 
 
+@pytest.mark.parametrize("scale", [2.4e38, 3.4e38])
+def test_attention_refuses_scales_that_overflow(scale):
+    """Finite, but times log2(e), as the kernels use it, they are not."""
+    assert attention(scale=scale) == BAD and "scale" in S.last_error()
+
+
 def test_empty_calls_do_nothing():
     assert append(T=0, k=None) == 0 and attention(T=0, q=None) == 0
 
