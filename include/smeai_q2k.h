@@ -114,7 +114,8 @@ int smeai_rms_q8k_quantize_w(const float *x_dev, int64_t ld_x, int64_t n_cols, i
  * the quants equal smeai_rms_q8k_quantize_w's on that sum bit for bit.  For
  * linears without a residual epilogue (Q3_K, Q6_K) and for the norm that
  * follows one.  sum may be x or resid themselves (same pointer and stride);
- * otherwise it must not overlap them.  k is a multiple of 256 up to 65536. */
+ * otherwise it must not overlap them.  y_q8k_dev is 4-byte aligned; k is a
+ * multiple of 256 up to 65536. */
 int smeai_add_rms_q8k_quantize(const float *x_dev, int64_t ld_x, const float *resid_dev, int64_t ld_resid,
                                int64_t n_cols, int64_t k, const float *weight_dev, float eps, float *sum_dev,
                                int64_t ld_sum, void *y_q8k_dev, void *stream);

@@ -258,6 +258,10 @@ int smeai_add_rms_q8k_quantize(const float* x_dev, int64_t ld_x, const float* re
     set_last_error("smeai_add_rms_q8k_quantize: NULL pointer");
     return kBadArgument;
   }
+  if (reinterpret_cast<uintptr_t>(y_q8k_dev) & 3) {
+    set_last_error("smeai_add_rms_q8k_quantize: the blocks are 4-byte aligned");
+    return kBadArgument;
+  }
   if ((sum_dev == x_dev && ld_sum != ld_x) || (sum_dev == resid_dev && ld_sum != ld_resid)) {
     set_last_error("smeai_add_rms_q8k_quantize: a sum in place of an input has that input's row stride");
     return kBadArgument;

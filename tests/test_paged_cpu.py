@@ -97,6 +97,12 @@ def test_add_rms_refuses(kw):
     assert add_rms(**kw) == BAD and "add_rms_q8k_quantize" in S.last_error()
 
 
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_add_rms_refuses_blocks_off_their_words(off):
+    """A byte view of any offset is a legal tensor; the blocks are written in words."""
+    assert add_rms(y=P + off) == BAD and "aligned" in S.last_error()
+
+
 @pytest.mark.skipif(__import__("torch").cuda.is_available(), reason="only meaningful on a host without a GPU")
 def test_without_a_device():
     assert plan() == NONE and append() == NONE and attention() == NONE
