@@ -42,8 +42,9 @@
 // known changed nothing.
 //
 // Every wait is bounded by wall time; on expiry the kernel records
-// kDevErrTimeout, all roles stop, copies and MMAs in flight are drained, TMEM
-// is freed and the kernel returns.  No multicast.
+// kDevErrTimeout, all roles stop, copies and MMAs in flight are drained (they
+// always end, so that wait has a bound of its own, whatever the limit that ran
+// out), TMEM is freed and the kernel returns.  No multicast.
 #include <cuda.h>
 #include <string.h>
 
@@ -59,6 +60,7 @@ constexpr int kKB = 128;             // keys a block
 constexpr int kThreads = 384;
 constexpr int kLoadWarp0 = 8, kLoadWarps = 2, kMmaWarp = 10;
 constexpr int kTmaMinPage = 8;       // tokens
+constexpr uint64_t kDrainNs = 1000000000ull;
 // 384 threads x 168 registers at launch = 256 x 208 + 128 x 88
 constexpr int kAtom = 128 * 128;     // 128 rows x 128 bytes
 constexpr int kTmemCols = 512;       // S0 S1 (128 columns each), O0 O1 (up to 128 each)
@@ -80,6 +82,7 @@ struct TcSmem {
   uint64_t* q_empty;                 // commit: the tile's last QK has read the queries
   uint64_t *s_full, *p_full, *o_full;  // per half: commit; 4 warps; commit
   uint64_t *x_full, *x_done;         // one half's rows on both: 4 warps have left half 1's results; 4 have taken them
+  int64_t* items;                    // per load warp: ring items it has announced
   float2* x_ml;                      // [128] half 1's maximum and sum; its context lies where the queries were
   uint64_t* drain;
   uint32_t* tmem;
@@ -104,6 +107,7 @@ __device__ __forceinline__ TcSmem carve(uint8_t* base) {
   m.abort = reinterpret_cast<int*>(b + 25);
   m.x_full = b + 26;
   m.x_done = b + 27;
+  m.items = reinterpret_cast<int64_t*>(b + 28);
   m.x_ml = reinterpret_cast<float2*>(b + 32);
   return m;
 }
@@ -301,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
     int64_t left = units;
     int slot = 0;                  // of the next item
     unsigned round = 1;            // parity of the wait for its being free
-    int64_t items = 0;             // announced
+    int64_t items = 0;             // announced: arrived on `full`
     bool ok = true;
     unsigned q_round = 1;          // parity of the wait for the queries' place
     // cp.async: 4 rows at a time, 8 lanes take 128 contiguous bytes of a row.
@@ -432,13 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
     }
     cp_async_commit();
     cp_async_wait<0>();
-    if (kTma && !ok) {
-      // gave up: TMA loads in flight still write this CTA's shared memory; their
-      // bytes complete the phases they were announced on (a phase that the
-      // other load warp never joined costs the whole millisecond)
-      for (int64_t i = items > C::kSlots ? items - C::kSlots : 0; i < items; ++i)
-        mbar_wait_bounded(&m.full[i % C::kSlots], (unsigned)((i / C::kSlots) & 1), 1000000);
-    }
+    if (lane == 0) m.items[lw] = items;
   } else if (warp >= kMmaWarp) {
     // ---------------- issue the MMAs
     // The whole warp walks and waits, so that descriptors stay in uniform
@@ -564,7 +562,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
       }
       // everything issued has finished before TMEM is freed
       commit(m.drain);
-      mbar_wait_bounded(m.drain, 0, limit_ns);
+      mbar_wait_bounded(m.drain, 0, kDrainNs);
     }
     __syncwarp();
   } else {
@@ -768,6 +766,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (kTma && *reinterpret_cast<volatile int*>(m.abort)) {
+    // A wait ran out: TMA loads that nobody waited for still write this CTA's
+    // shared memory.  Their bytes complete the phases they were announced on
+    // once both load warps have arrived there; the warp that left earlier is at
+    // most a ring behind.
+    if (threadIdx.x == 0) {
+      const int64_t some = min(m.items[0], m.items[1]), all = max(m.items[0], m.items[1]);
+      for (int64_t i = some; i < all; ++i) mbar_arrive(&m.full[i % C::kSlots]);
+      for (int64_t i = max(all - C::kSlots, (int64_t)0); i < all; ++i)
+        mbar_wait_bounded(&m.full[i % C::kSlots], (unsigned)((i / C::kSlots) & 1), kDrainNs);
+    }
+    __syncthreads();
+  }
   pdl_trigger();
   if (warp == kMmaWarp)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");

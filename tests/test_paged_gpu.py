@@ -529,3 +529,25 @@ def test_refused_tensors(cuda):
     with pytest.raises(S.SmeaiError, match="overlap"):
         paged.append(paged.PagedKV(one, one), torch.zeros((1, 1, 64), device=cuda), torch.zeros((1, 1, 64), device=cuda),
                      torch.zeros(1, dtype=torch.int64, device=cuda))
+
+
+@pytest.mark.parametrize("H,K,D,page,lens", [(8, 2, 128, 16, [(300, 3000), (40, 5000), (1, 900)]), (8, 8, 64, 32, [(64, 4000)] * 30),
+                                             (4, 2, 128, 4, [(300, 3000), (40, 5000)])])
+def test_attention_gives_up_when_a_wait_runs_out(cuda, H, K, D, page, lens):
+    """With a limit of a nanosecond the first wait of the tensor-core kernel that
+    is not over at once runs out.  The call ends, says so, and the next one is
+    right: nothing of the first was left in flight, and tensor memory was freed."""
+    p = Problem(cuda, lens, H, K, D, page, F16, seed=23)
+    want = p.run().clone()
+    assert S.take_device_error() == 0
+    try:
+        S.lib().smeai_set_wait_timeouts(1, 0)
+        for _ in range(5):
+            p.run()
+    finally:
+        S.lib().smeai_set_wait_timeouts(0, 0)
+    torch.cuda.synchronize()
+    assert S.take_device_error() == 1
+    for _ in range(3):
+        assert torch.equal(p.run(), want)
+    p.check(want)
