@@ -295,154 +295,154 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
 
   if (units <= 0) {
     // nothing to do
-  } else if (warp >= kLoadWarp0 && warp < kLoadWarp0 + kLoadWarps) {
-    // ---------------- load: this warp's 64 rows of every item
+  } else if (warp >= kLoadWarp0) {
+    // one instruction for the whole warpgroup: load, MMA and idle warp
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    const int lw = warp - kLoadWarp0;
-    AttnPos w;
-    attn_open<kTR, kKB>(p, share, w);
-    const int page_mask = (1 << p.kv.page_log2) - 1;
-    int64_t left = units;
-    int slot = 0;                  // of the next item
-    unsigned round = 1;            // parity of the wait for its being free
-    int64_t items = 0;             // announced: arrived on `full`
-    bool ok = true;
-    unsigned q_round = 1;          // parity of the wait for the queries' place
-    // cp.async: 4 rows at a time, 8 lanes take 128 contiguous bytes of a row.
-    // Row i * 4 + sub of 32 lands in atom row row0 + that row, its 16-byte
-    // chunks XORed with the row mod 8 -- which is sub, or sub + 4 for odd i.
-    const int sub = lane >> 3, col = lane & 7;
-    const uint32_t even = (uint32_t)(sub * 128 + ((col ^ sub) << 4)), odd = (uint32_t)(sub * 128 + ((col ^ (sub + 4)) << 4));
-    int bytes[C::kCb];                             // 0 past the head's elements
+    if (warp < kLoadWarp0 + kLoadWarps) {
+      // ---------------- load: this warp's 64 rows of every item
+      const int lw = warp - kLoadWarp0;
+      AttnPos w;
+      attn_open<kTR, kKB>(p, share, w);
+      const int page_mask = (1 << p.kv.page_log2) - 1;
+      int64_t left = units;
+      int slot = 0;                  // of the next item
+      unsigned round = 1;            // parity of the wait for its being free
+      int64_t items = 0;             // announced: arrived on `full`
+      bool ok = true;
+      unsigned q_round = 1;          // parity of the wait for the queries' place
+      // cp.async: 4 rows at a time, 8 lanes take 128 contiguous bytes of a row.
+      // Row i * 4 + sub of 32 lands in atom row row0 + that row, its 16-byte
+      // chunks XORed with the row mod 8 -- which is sub, or sub + 4 for odd i.
+      const int sub = lane >> 3, col = lane & 7;
+      const uint32_t even = (uint32_t)(sub * 128 + ((col ^ sub) << 4)), odd = (uint32_t)(sub * 128 + ((col ^ (sub + 4)) << 4));
+      int bytes[C::kCb];                             // 0 past the head's elements
 #pragma unroll
-    for (int cb = 0; cb < C::kCb; ++cb) bytes[cb] = cb * 64 + col * 8 < p.kv.dim ? 16 : 0;
-    // off: byte offset of row row0 + lane, -1: zeros
-    auto copy_rows = [&](uint8_t* dst, const char* src, int64_t off, int row0) {
-      const uint32_t d = smem_addr(dst) + row0 * 128;
-      const char* from = src + col * 16;
+      for (int cb = 0; cb < C::kCb; ++cb) bytes[cb] = cb * 64 + col * 8 < p.kv.dim ? 16 : 0;
+      // off: byte offset of row row0 + lane, -1: zeros
+      auto copy_rows = [&](uint8_t* dst, const char* src, int64_t off, int row0) {
+        const uint32_t d = smem_addr(dst) + row0 * 128;
+        const char* from = src + col * 16;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int64_t o = __shfl_sync(0xffffffffu, off, i * 4 + sub);
+        for (int i = 0; i < 8; ++i) {
+          const int64_t o = __shfl_sync(0xffffffffu, off, i * 4 + sub);
 #pragma unroll
-        for (int cb = 0; cb < C::kCb; ++cb) {
-          const int n = o >= 0 ? bytes[cb] : 0;
-          cp_async16(d + i * 512 + cb * kAtom + (i & 1 ? odd : even), n ? from + o + cb * 128 : src, n);
+          for (int cb = 0; cb < C::kCb; ++cb) {
+            const int n = o >= 0 ? bytes[cb] : 0;
+            cp_async16(d + i * 512 + cb * kAtom + (i & 1 ? odd : even), n ? from + o + cb * 128 : src, n);
+          }
         }
+      };
+      auto acquire = [&]() {   // the first round over the ring finds it free
+        return wait_warp(m, &m.empty[slot], round, p.err, limit_ns);
+      };
+      auto next_slot = [&]() {
+        ++items;
+        if (++slot == C::kSlots) {
+          slot = 0;
+          round ^= 1;
+        }
+      };
+      // copies of this warp so far have landed: announce them
+      auto landed = [&]() {
+        cp_async_commit();
+        cp_async_wait<0>();
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&m.full[slot]);
+      };
+      const int box_rows = 1 << maps.box_log2, boxes = 64 >> maps.box_log2;
+      const int my_box = lane / C::kCb, my_cb = lane % C::kCb;
+      while (left > 0 && ok) {
+        const Stretch s = stretch(p, w, left);
+        const int32_t* table = p.table + (int64_t)w.b * p.ld_table;
+        auto page_of = [&](int key) {   // -1: no such key, or a bad page
+          if (key >= w.r.kv) return -1;
+          const int page = table[key >> p.kv.page_log2];
+          if (page >= 0 && page < p.kv.n_pages) return page;
+          raise_device_error(p.err, kDevErrBadIndex);
+          return -1;
+        };
+        auto row_off = [&](int key) {
+          const int page = page_of(key);
+          return page < 0 ? (int64_t)-1
+                          : page * p.kv.page_bytes + (key & page_mask) * p.kv.token_bytes + w.h * p.kv.head_bytes;
+        };
+        auto copy_item = [&](const char* src, int key0) {
+          uint8_t* dst = m.ring + (size_t)slot * C::kItem;
+          copy_rows(dst, src, row_off(key0 + lane), lw * 64);
+          copy_rows(dst, src, row_off(key0 + 32 + lane), lw * 64 + 32);
+        };
+        // this lane's box of a TMA item: its first key's page, -1 when it has none
+        const bool has_box = kTma && my_box < boxes;
+        int page = has_box ? page_of(s.kb0 * kKB + lw * 64 + my_box * box_rows) : -1;
+        auto load_item = [&](const CUtensorMap* map, int key0) {
+          const unsigned n = __popc(__ballot_sync(0xffffffffu, page >= 0));
+          if (lane == 0) mbar_expect_tx(&m.full[slot], n * box_rows * 128);
+          __syncwarp();
+          if (page >= 0) {
+            const int row = my_box * box_rows;
+            tma_load_box(smem_addr(m.ring) + slot * C::kItem + my_cb * kAtom + (lw * 64 + row) * 128, map, my_cb * 64,
+                         (key0 + row) & page_mask, w.h, page, &m.full[slot]);
+          }
+        };
+        for (int b = 0; b < s.n && ok; ++b) {
+          const int key0 = (s.kb0 + b) * kKB + lw * 64;
+          // the next block's pages are looked up before this block's waits
+          const int next_page = has_box && b + 1 < s.n ? page_of(key0 + kKB + my_box * box_rows) : -1;
+          if (!(ok = acquire())) break;
+          if (kTma) load_item(&maps.k, key0);
+          if (b == 0) {
+            // the tile's queries land with its first keys, once the last tile's are read
+            if (!(ok = wait_warp(m, m.q_empty, q_round, p.err, limit_ns))) {
+              if (lane == 0) mbar_arrive(&m.full[slot]);
+              ++items;
+              break;
+            }
+            q_round ^= 1;
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+              const int row = w.rt * kTR + (s.dual ? 0 : lw * 128) + q4 * 32 + lane;
+              int64_t off = -1;
+              if (row < w.r.rows) {
+                const int tok = row / p.group, hd = w.h * p.group + row % p.group;
+                off = (int64_t)(w.r.q0 + tok) * p.ld_q + (int64_t)hd * p.kv.dim * 2;
+              }
+              copy_rows(m.q + lw * C::kItem, p.q, off, q4 * 32);
+            }
+          }
+          if (!kTma) {
+            copy_item(p.kv.k, key0);
+            cp_async_arrive(&m.full[slot]);
+          } else if (b == 0) {
+            landed();
+          } else if (lane == 0) {
+            mbar_arrive(&m.full[slot]);
+          }
+          next_slot();
+          if (!(ok = acquire())) break;
+          if (!kTma) {
+            copy_item(p.kv.v, key0);
+            cp_async_arrive(&m.full[slot]);
+          } else if ((s.kb0 + b + 1) * kKB > w.r.kv) {
+            copy_item(p.kv.v, key0);
+            landed();
+          } else {
+            load_item(&maps.v, key0);
+            if (lane == 0) mbar_arrive(&m.full[slot]);
+          }
+          next_slot();
+          page = next_page;
+        }
+        left -= s.n;
+        if (left > 0) attn_next_tile<kTR, kKB>(p, w);
       }
-    };
-    auto acquire = [&]() {   // the first round over the ring finds it free
-      return wait_warp(m, &m.empty[slot], round, p.err, limit_ns);
-    };
-    auto next_slot = [&]() {
-      ++items;
-      if (++slot == C::kSlots) {
-        slot = 0;
-        round ^= 1;
-      }
-    };
-    // copies of this warp so far have landed: announce them
-    auto landed = [&]() {
       cp_async_commit();
       cp_async_wait<0>();
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&m.full[slot]);
-    };
-    const int box_rows = 1 << maps.box_log2, boxes = 64 >> maps.box_log2;
-    const int my_box = lane / C::kCb, my_cb = lane % C::kCb;
-    while (left > 0 && ok) {
-      const Stretch s = stretch(p, w, left);
-      const int32_t* table = p.table + (int64_t)w.b * p.ld_table;
-      auto page_of = [&](int key) {   // -1: no such key, or a bad page
-        if (key >= w.r.kv) return -1;
-        const int page = table[key >> p.kv.page_log2];
-        if (page >= 0 && page < p.kv.n_pages) return page;
-        raise_device_error(p.err, kDevErrBadIndex);
-        return -1;
-      };
-      auto row_off = [&](int key) {
-        const int page = page_of(key);
-        return page < 0 ? (int64_t)-1
-                        : page * p.kv.page_bytes + (key & page_mask) * p.kv.token_bytes + w.h * p.kv.head_bytes;
-      };
-      auto copy_item = [&](const char* src, int key0) {
-        uint8_t* dst = m.ring + (size_t)slot * C::kItem;
-        copy_rows(dst, src, row_off(key0 + lane), lw * 64);
-        copy_rows(dst, src, row_off(key0 + 32 + lane), lw * 64 + 32);
-      };
-      // this lane's box of a TMA item: its first key's page, -1 when it has none
-      const bool has_box = kTma && my_box < boxes;
-      int page = has_box ? page_of(s.kb0 * kKB + lw * 64 + my_box * box_rows) : -1;
-      auto load_item = [&](const CUtensorMap* map, int key0) {
-        const unsigned n = __popc(__ballot_sync(0xffffffffu, page >= 0));
-        if (lane == 0) mbar_expect_tx(&m.full[slot], n * box_rows * 128);
-        __syncwarp();
-        if (page >= 0) {
-          const int row = my_box * box_rows;
-          tma_load_box(smem_addr(m.ring) + slot * C::kItem + my_cb * kAtom + (lw * 64 + row) * 128, map, my_cb * 64,
-                       (key0 + row) & page_mask, w.h, page, &m.full[slot]);
-        }
-      };
-      for (int b = 0; b < s.n && ok; ++b) {
-        const int key0 = (s.kb0 + b) * kKB + lw * 64;
-        // the next block's pages are looked up before this block's waits
-        const int next_page = has_box && b + 1 < s.n ? page_of(key0 + kKB + my_box * box_rows) : -1;
-        if (!(ok = acquire())) break;
-        if (kTma) load_item(&maps.k, key0);
-        if (b == 0) {
-          // the tile's queries land with its first keys, once the last tile's are read
-          if (!(ok = wait_warp(m, m.q_empty, q_round, p.err, limit_ns))) {
-            if (lane == 0) mbar_arrive(&m.full[slot]);
-            ++items;
-            break;
-          }
-          q_round ^= 1;
-#pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4) {
-            const int row = w.rt * kTR + (s.dual ? 0 : lw * 128) + q4 * 32 + lane;
-            int64_t off = -1;
-            if (row < w.r.rows) {
-              const int tok = row / p.group, hd = w.h * p.group + row % p.group;
-              off = (int64_t)(w.r.q0 + tok) * p.ld_q + (int64_t)hd * p.kv.dim * 2;
-            }
-            copy_rows(m.q + lw * C::kItem, p.q, off, q4 * 32);
-          }
-        }
-        if (!kTma) {
-          copy_item(p.kv.k, key0);
-          cp_async_arrive(&m.full[slot]);
-        } else if (b == 0) {
-          landed();
-        } else if (lane == 0) {
-          mbar_arrive(&m.full[slot]);
-        }
-        next_slot();
-        if (!(ok = acquire())) break;
-        if (!kTma) {
-          copy_item(p.kv.v, key0);
-          cp_async_arrive(&m.full[slot]);
-        } else if ((s.kb0 + b + 1) * kKB > w.r.kv) {
-          copy_item(p.kv.v, key0);
-          landed();
-        } else {
-          load_item(&maps.v, key0);
-          if (lane == 0) mbar_arrive(&m.full[slot]);
-        }
-        next_slot();
-        page = next_page;
-      }
-      left -= s.n;
-      if (left > 0) attn_next_tile<kTR, kKB>(p, w);
-    }
-    cp_async_commit();
-    cp_async_wait<0>();
-    if (lane == 0) m.items[lw] = items;
-  } else if (warp >= kMmaWarp) {
-    // ---------------- issue the MMAs
-    // The whole warp walks and waits, so that descriptors stay in uniform
-    // registers; one elected lane issues.
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (warp == kMmaWarp) {
+      if (lane == 0) m.items[lw] = items;
+    } else if (warp == kMmaWarp) {
+      // ---------------- issue the MMAs
+      // The whole warp walks and waits, so that descriptors stay in uniform
+      // registers; one elected lane issues.
       constexpr uint32_t kQk = idesc(Num<T>::kIsBf16, kKB, false), kPv = idesc(Num<T>::kIsBf16, DP, true);
       AttnPos w;
       attn_open<kTR, kKB>(p, share, w);

@@ -103,6 +103,16 @@ def test_add_rms_refuses_blocks_off_their_words(off):
     assert add_rms(y=P + off) == BAD and "aligned" in S.last_error()
 
 
+def test_register_hand_over_is_one_instruction_a_warpgroup():
+    """All warps of a warpgroup have to meet at the same setmaxnreg; the roles
+    of the tensor-core kernel's last four warps differ, so it stands before them."""
+    import os
+    source = os.path.join(os.path.dirname(__file__), "..", "sme-ai-ops_b200", "csrc", "paged_attn_tc.cu")
+    with open(source) as f:
+        text = f.read()
+    assert text.count("setmaxnreg.dec") == 1 and text.count("setmaxnreg.inc") == 1
+
+
 @pytest.mark.skipif(__import__("torch").cuda.is_available(), reason="only meaningful on a host without a GPU")
 def test_without_a_device():
     assert plan() == NONE and append() == NONE and attention() == NONE
