@@ -325,7 +325,7 @@ class Q2KDecodeStack:
         """One step of a serving loop: x [T, hidden] fp32 holds the new tokens
         of all requests behind one another (one each while decoding, a chunk of
         a prompt, both), `plan` their PagedPlan, built, `caches` one PagedKV a
-        layer (hidden / head_dim key heads), rope a paged.rope_table.  Every
+        layer (hidden / head_dim key heads, the plan's page size), rope a paged.rope_table.  Every
         layer's attention is taken over the request's cached tokens; returns
         logits [T, vocab].  Rows behind the last request's hold anything.  One
         GPU; queued on the current stream without waiting."""
@@ -333,7 +333,10 @@ class Q2KDecodeStack:
         assert self.world == 1 and len(caches) == self.L and x.shape == (plan.n_tokens, self.H)
         T, H, e = x.shape[0], self.H, self.eps
         heads, D = caches[0].n_kv_heads, caches[0].head_dim
-        assert heads * D == H
+        assert heads * D == H, "hidden / head_dim key heads"
+        # slots name pages of the plan's size, which each cache takes for its own
+        assert all(c.page_size == plan.page_size for c in caches), "the caches' pages are of the plan's page size"
+        assert all(c.n_kv_heads == heads and c.head_dim == D for c in caches), "the caches' heads are alike"
 
         def linear(m, xq, epilogue=EPI_STORE):
             return (m.mul_mat_tc if T >= 16 else m.mul_mat)(xq, T, epilogue=epilogue)

@@ -116,3 +116,23 @@ def test_register_hand_over_is_one_instruction_a_warpgroup():
 @pytest.mark.skipif(__import__("torch").cuda.is_available(), reason="only meaningful on a host without a GPU")
 def test_without_a_device():
     assert plan() == NONE and append() == NONE and attention() == NONE
+
+
+def step_cached(caches, **plan):
+    """Q2KDecodeStack.step_cached on a host without tensors on a GPU: its checks come first."""
+    import types
+    import torch
+    from smeai_b200.stack import Q2KDecodeStack
+    stack = types.SimpleNamespace(world=1, L=len(caches), H=256, eps=1e-5, V=32)
+    plan = types.SimpleNamespace(**{**dict(n_tokens=3, page_size=16), **plan})
+    return Q2KDecodeStack.step_cached(stack, torch.zeros((plan.n_tokens, 256)), plan, caches, 1)
+
+
+@pytest.mark.parametrize("second,match", [(dict(page_size=32), "page size"), (dict(n_kv_heads=4), "alike"), (dict(head_dim=64), "alike")])
+def test_step_refuses_caches_that_do_not_fit_the_plan(second, match):
+    import types
+    kv = lambda **kw: types.SimpleNamespace(**{**dict(page_size=16, n_kv_heads=2, head_dim=128), **kw})  # noqa: E731
+    with pytest.raises(AssertionError, match=match):
+        step_cached([kv(), kv(**second)])
+    with pytest.raises(AssertionError, match="page size"):
+        step_cached([kv(), kv()], page_size=8)
