@@ -337,6 +337,8 @@ class Q2KDecodeStack:
         # slots name pages of the plan's size, which each cache takes for its own
         assert all(c.page_size == plan.page_size for c in caches), "the caches' pages are of the plan's page size"
         assert all(c.n_kv_heads == heads and c.head_dim == D for c in caches), "the caches' heads are alike"
+        if T == 0:
+            return x.new_empty((0, self.V))
 
         def linear(m, xq, epilogue=EPI_STORE):
             return (m.mul_mat_tc if T >= 16 else m.mul_mat)(xq, T, epilogue=epilogue)

@@ -136,3 +136,9 @@ def test_step_refuses_caches_that_do_not_fit_the_plan(second, match):
         step_cached([kv(), kv(**second)])
     with pytest.raises(AssertionError, match="page size"):
         step_cached([kv(), kv()], page_size=8)
+
+
+def test_step_without_tokens_does_nothing():
+    import types
+    kv = types.SimpleNamespace(page_size=16, n_kv_heads=2, head_dim=128)
+    assert step_cached([kv, kv], n_tokens=0).shape == (0, 32)
