@@ -47,7 +47,7 @@ class PagedKV:
         self.struct = KVCache(k.data_ptr(), v.data_ptr(), _TYPES[k.dtype], self.page_size, self.n_kv_heads, self.head_dim,
                               self.n_pages, strides[0], strides[1], strides[2])
         self.ref = ctypes.byref(self.struct)
-        self._workspace = {}         # bytes of attention()'s workspace, by sizes
+        self._workspace = {}         # bytes of attention()'s workspace, by sizes; few of them, a server's sizes never end
 
     @classmethod
     def empty(cls, n_pages: int, n_kv_heads: int, page_size: int, head_dim: int, dtype=torch.float16, device=None) -> "PagedKV":
@@ -183,6 +183,8 @@ def attention_workspace(kv: PagedKV, n_heads: int, n_tokens: int, n_req: int, ma
     key = (n_heads, n_tokens, n_req, max_blocks, max_new)
     n = kv._workspace.get(key)
     if n is None:
+        if len(kv._workspace) >= 64:
+            kv._workspace.clear()
         with torch.cuda.device(kv.device):
             n = kv._workspace[key] = lib().smeai_paged_attention_workspace(kv.ref, *key)
     return n

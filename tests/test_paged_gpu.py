@@ -551,3 +551,11 @@ def test_attention_gives_up_when_a_wait_runs_out(cuda, H, K, D, page, lens):
     for _ in range(3):
         assert torch.equal(p.run(), want)
     p.check(want)
+
+
+def test_workspace_sizes_are_not_collected(cuda):
+    """A server's steps differ in their sizes for ever; a cache keeps a bounded number of answers."""
+    kv = paged.PagedKV.empty(4, 2, 16, 64, device=cuda)
+    sizes = [paged.attention_workspace(kv, 8, t, 3, 100, t) for t in range(1, 1000)]
+    assert len(kv._workspace) <= 64
+    assert sizes == [paged.attention_workspace(kv, 8, t, 3, 100, t) for t in range(1, 1000)] and min(sizes) > 0
