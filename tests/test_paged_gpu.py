@@ -559,3 +559,88 @@ def test_workspace_sizes_are_not_collected(cuda):
     sizes = [paged.attention_workspace(kv, 8, t, 3, 100, t) for t in range(1, 1000)]
     assert len(kv._workspace) <= 64
     assert sizes == [paged.attention_workspace(kv, 8, t, 3, 100, t) for t in range(1, 1000)] and min(sizes) > 0
+
+
+# ---- every head_dim and tile that the documentation allows ---------------------------
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("H,K,D,page", [(4, 2, 24, 16), (3, 1, 40, 4), (8, 1, 104, 8), (4, 2, 136, 16), (9, 1, 192, 1), (2, 2, 248, 64)])
+def test_attention_one_token_odd_head_dims(cuda, dtype, H, K, D, page):
+    p = Problem(cuda, DECODE + [(1, 9000)], H, K, D, page, dtype, seed=24)
+    p.check(p.run())
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("H,K,D,page", [(4, 2, 136, 16), (3, 1, 192, 4), (2, 2, 216, 32)])
+def test_attention_chunks_odd_head_dims(cuda, causal, H, K, D, page):
+    """64-row tiles over padded columns, some of them split over CTAs."""
+    p = Problem(cuda, CHUNK + [(40, 6000)], H, K, D, page, BF16, seed=25)
+    p.check(p.run(causal=causal), causal=causal)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype,H,K,D,page", [(F16, 2, 1, 8, 16), (BF16, 2, 1, 8, 4), (F16, 1, 1, 24, 4), (BF16, 1, 1, 24, 64), (F16, 3, 1, 40, 8),
+                                              (F16, 2, 2, 72, 16), (BF16, 1, 1, 88, 128), (F16, 2, 1, 104, 2), (BF16, 2, 1, 120, 32)])
+def test_attention_many_rows_odd_head_dims(cuda, causal, dtype, H, K, D, page):
+    """The tensor-core kernel's boxes and tiles are wider than the head."""
+    p = Problem(cuda, MANY, H, K, D, page, dtype, seed=26)
+    p.check(p.run(causal=causal), causal=causal)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("H,K,D", [(4, 1, 128), (6, 2, 64), (8, 1, 96), (1, 1, 128)])
+def test_attention_drafts(cuda, dtype, causal, H, K, D):
+    """Tiles of 24 rows: several tokens a request, so several limits in a tile;
+    rows that the tile has too many; long requests split and joined."""
+    most = 24 * K // H
+    lens = [(1 + i % most, m) for i, m in enumerate((1, 30, 64, 65, 190, 383, 384, 385, 700, 1000, 2500, 3001))]
+    lens += [(most, 20000), (most, most), (most, 0), (0, 70), (most - 1, 9000)]
+    p = Problem(cuda, lens, H, K, D, 16, dtype, seed=27)
+    assert 16 < most * (H // K) <= 24
+    out = p.run(causal=causal)
+    p.check(out, causal=causal)
+    assert torch.equal(out, p.run(causal=causal))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("H,K,D,n", [(8, 2, 128, 1), (4, 1, 64, 4), (2, 1, 128, 8), (16, 1, 80, 1), (4, 2, 256, 3)])
+def test_attention_of_up_to_16_rows_keeps_its_weights(cuda, dtype, H, K, D, n):
+    """Up to 16 rows a request the weights keep what their rounding leaves, so
+    the result is off by its own rounding and that of fp32 alone."""
+    p = Problem(cuda, [(n, m) for m in (n, 40, 100, 500, 3000, 20000)], H, K, D, 16, dtype, seed=28)
+    out = p.run()
+    half = torch.finfo(dtype).eps / 2
+    for i, (n, m) in enumerate(p.lens):
+        lo, hi = p.starts[i], p.starts[i + 1]
+        k, v = (x.double().repeat_interleave(H // K, 1) for x in p.rows[i])
+        s = torch.einsum("nhd,mhd->hnm", p.q[lo:hi].double(), k) * D ** -0.5
+        s = s.masked_fill(torch.arange(m, device=cuda)[None] > m - n + torch.arange(n, device=cuda)[:, None], -math.inf)
+        w = torch.softmax(s, -1)
+        ref, size = torch.einsum("hnm,mhd->nhd", w, v), torch.einsum("hnm,mhd->nhd", w, v.abs())
+        # as check(), with the square of half a step for the weights: what one rounding leaves, rounded again
+        assert ((out[lo:hi].double() - ref).abs() <= 1.01 * (half * ref.abs() + (half * half + 1e-4) * size) + 2.0 ** -25).all(), (n, m)
+
+
+@pytest.mark.parametrize("D", [8, 24, 40, 72, 136, 248])
+@pytest.mark.parametrize("rope", ["pairs", "halves"])
+def test_append_odd_head_dims(cuda, rope, D):
+    """Against the same values appended by hand."""
+    T, H, K, page = 37, 3, 2, 8
+    g = torch.Generator(device=cuda).manual_seed(D)
+    q, k, v = (torch.randn((T, n, D), generator=g, device=cuda) for n in (H, K, K))
+    kv = paged.PagedKV(*(torch.zeros((8, K, page, D), dtype=F16, device=cuda) for _ in range(2)))
+    slots, pos = torch.randperm(8 * page, generator=g, device=cuda)[:T].contiguous(), torch.arange(T, dtype=torch.int32, device=cuda) + 100
+    table = paged.rope_table(200, D, device=cuda)
+    got = paged.append(kv, k, v, slots, q=q, positions=pos, rope=table, halves=rope == "halves")
+    cs = table.double()[pos.long()][:, None]
+    c, s = cs[..., :D // 2], cs[..., D // 2:]
+    for out, x in ((got, q), (kv.k[slots // page, :, slots % page], k)):
+        y = x.double()
+        a, b = (y[..., :D // 2], y[..., D // 2:]) if rope == "halves" else (y[..., 0::2], y[..., 1::2])
+        ref = [a * c - b * s, a * s + b * c]
+        ref = torch.cat(ref, -1) if rope == "halves" else torch.stack(ref, -1).flatten(-2)
+        # fp32 products and sum of values below 6 (3 * 6 * 2^-24 < 2^-19), then one rounding
+        assert ((out.double() - ref).abs() <= 2.0 ** -11 * ref.abs() + 2.0 ** -19 + 2.0 ** -25).all()
+    assert torch.equal(kv.v[slots // page, :, slots % page], v.half())
+    assert S.take_device_error() == 0
