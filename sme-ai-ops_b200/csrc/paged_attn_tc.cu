@@ -112,13 +112,15 @@ __device__ __forceinline__ TcSmem carve(uint8_t* base) {
   return m;
 }
 
-// Bounded wait that also gives up once another role has.
+// Bounded wait that also gives up once another role has.  With a limit below
+// the clock's step a wait that is not over at once has run out.
 __device__ __forceinline__ bool wait_or_abort(const TcSmem& m, uint64_t* bar, unsigned parity, unsigned* err,
                                               uint64_t limit_ns) {
-  if (mbar_try_wait(bar, parity)) return true;
+  if (mbar_test_wait(bar, parity)) return true;
   const uint64_t t0 = global_timer_ns();
+  const int tries = limit_ns < 1024 ? 0 : 32;
   for (;;) {
-    for (int i = 0; i < 32; ++i)
+    for (int i = 0; i < tries; ++i)
       if (mbar_try_wait(bar, parity)) return true;
     if (*reinterpret_cast<volatile int*>(m.abort)) return false;
     if (global_timer_ns() - t0 > limit_ns) {
