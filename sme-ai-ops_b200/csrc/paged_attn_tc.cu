@@ -631,13 +631,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
             plus = row_base(mn, p.scale_log2) == mn ? base_offset<T>(mn, p.scale_log2) : kOpens;
           }
           add = plus;
-          if (__any_sync(0xffffffffu, plus == kOpens)) {
-            const bool far = plus == kOpens && mx > kNegInf;
-            const float less = far ? mx : 0.f;
-            if (far) add = Num<T>::kBias;
-#pragma unroll
-            for (int i = 0; i < 128; ++i) v[i] -= less;
-          }
           l *= f;
           if (b > 0) {
 #pragma unroll 1
@@ -650,6 +643,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
               for (int k = 0; k < 32; ++k) o[k] *= f;
               tmem_st32(o_col + i * 32, o);
             }
+          }
+          const bool far = plus == kOpens && mx > kNegInf;
+          if (__any_sync(0xffffffffu, far)) {
+            const float less = far ? mx : 0.f;
+            if (far) add = Num<T>::kBias;
+#pragma unroll
+            for (int i = 0; i < 128; ++i) v[i] -= less;
           }
         }
         const uint64_t c2 = pack_f32x2(p.scale_log2, p.scale_log2), add2 = pack_f32x2(add, add);
