@@ -454,8 +454,8 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_few_ke
           const int2 to = out_offset(w, w.rt * TR + f0 * 8 + r);
           if (d8 * 8 < p.kv.dim)
             *reinterpret_cast<uint4*>(p.out + (int64_t)to.x * p.ld_out + ((int64_t)to.y * p.kv.dim + d8 * 8) * 2) =
-                make_uint4(Num<T>::pack(v[0] * inv, v[1] * inv), Num<T>::pack(v[2] * inv, v[3] * inv),
-                           Num<T>::pack(v[4] * inv, v[5] * inv), Num<T>::pack(v[6] * inv, v[7] * inv));
+                make_uint4(pack_mean<T>(v[0] * inv, v[1] * inv), pack_mean<T>(v[2] * inv, v[3] * inv),
+                           pack_mean<T>(v[4] * inv, v[5] * inv), pack_mean<T>(v[6] * inv, v[7] * inv));
         } else {
           float4* dst = reinterpret_cast<float4*>(p.part_o + (slot * TR + f0 * 8 + r) * DP + d8 * 8);
           dst[0] = make_float4(v[0], v[1], v[2], v[3]);
@@ -639,7 +639,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_mid_ke
 #pragma unroll
         for (int d = 0; d < DP / 8; ++d)
           if (d * 8 < p.kv.dim)
-            *reinterpret_cast<uint32_t*>(dst + (d * 8 + 2 * t4) * 2) = Num<T>::pack(o[d][2 * i] * inv, o[d][2 * i + 1] * inv);
+            *reinterpret_cast<uint32_t*>(dst + (d * 8 + 2 * t4) * 2) = pack_mean<T>(o[d][2 * i] * inv, o[d][2 * i + 1] * inv);
       } else if (row < w.r.rows) {
         float* dst = p.part_o + (slot * TR + r) * DP;
 #pragma unroll
@@ -760,7 +760,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps, DP <= 128 ? 2 : 1) paged_attn
 #pragma unroll
   for (int k = 0; k < kN; k += 2) {
     const int d = (k / kCols) * 32 * kCols + lane * kCols + k % kCols;
-    if (d < p.kv.dim) *reinterpret_cast<uint32_t*>(dst + d * 2) = Num<T>::pack(a[k] * inv, a[k + 1] * inv);
+    if (d < p.kv.dim) *reinterpret_cast<uint32_t*>(dst + d * 2) = pack_mean<T>(a[k] * inv, a[k + 1] * inv);
   }
 }
 

@@ -307,6 +307,18 @@ struct Num<__nv_bfloat16> {
   }
 };
 
+// Context values rounded to the output's type.  A mean of finite halves is at
+// most 65504; the rounding of the weights may have carried it past that, where
+// it would round to infinity.  True infinities and NaN stay.
+template <typename T>
+__device__ __forceinline__ uint32_t pack_mean(float lo, float hi) {
+  if constexpr (!Num<T>::kIsBf16) {
+    if (fabsf(lo) < INFINITY) lo = fminf(fmaxf(lo, -65504.f), 65504.f);
+    if (fabsf(hi) < INFINITY) hi = fminf(fmaxf(hi, -65504.f), 65504.f);
+  }
+  return Num<T>::pack(lo, hi);
+}
+
 // What a row's context is multiplied by in the end: nothing seen gives zeros,
 // NaN stays.
 __device__ __forceinline__ float row_scale(float sum) { return sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum); }

@@ -739,10 +739,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_tc_kernel(const AttnPa
             for (int k = 0; k < 4; ++k)
               if (i * 32 + k * 8 < p.kv.dim)
                 *reinterpret_cast<uint4*>(dst + (i * 32 + k * 8) * 2) =
-                    make_uint4(Num<T>::pack(o[8 * k] * inv, o[8 * k + 1] * inv),
-                               Num<T>::pack(o[8 * k + 2] * inv, o[8 * k + 3] * inv),
-                               Num<T>::pack(o[8 * k + 4] * inv, o[8 * k + 5] * inv),
-                               Num<T>::pack(o[8 * k + 6] * inv, o[8 * k + 7] * inv));
+                    make_uint4(pack_mean<T>(o[8 * k] * inv, o[8 * k + 1] * inv),
+                               pack_mean<T>(o[8 * k + 2] * inv, o[8 * k + 3] * inv),
+                               pack_mean<T>(o[8 * k + 4] * inv, o[8 * k + 5] * inv),
+                               pack_mean<T>(o[8 * k + 6] * inv, o[8 * k + 7] * inv));
           } else if (mine) {
 #pragma unroll
             for (int k = 0; k < 8; ++k)

@@ -644,3 +644,23 @@ def test_append_odd_head_dims(cuda, rope, D):
         assert ((out.double() - ref).abs() <= 2.0 ** -11 * ref.abs() + 2.0 ** -19 + 2.0 ** -25).all()
     assert torch.equal(kv.v[slots // page, :, slots % page], v.half())
     assert S.take_device_error() == 0
+
+
+@pytest.mark.parametrize("H,K,D,lens", [(4, 1, 128, [(1, 900), (1, 20000)]), (4, 2, 128, [(12, 900), (10, 6000)]),
+                                        (2, 1, 256, [(40, 900), (9, 5000)]), (4, 2, 128, [(200, 900), (300, 5000), (20, 3000)])])
+def test_attention_of_the_largest_values(cuda, H, K, D, lens):
+    """A mean of values is no larger than they are: with values of +-65504 the
+    rounding of the weights must not carry a row past fp16's range.  An infinite
+    value still gives infinities."""
+    p = Problem(cuda, lens, H, K, D, 16, F16, seed=29, spread=3.0)
+    for i, ((_, m), (_, vr)) in enumerate(zip(p.lens, p.rows)):
+        vr.copy_(torch.where(torch.arange(D, device=cuda) % 3 > 0, 65504.0, -65504.0).half().expand_as(vr))
+        at = torch.arange(m, device=cuda)
+        p.v[p.table[i, at // 16].long(), :, at % 16] = vr
+    out = p.run()
+    p.check(out)
+    p.v[p.table[0, 0].item(), :, 0, :8] = math.inf
+    out = p.run()
+    n = p.lens[0][0]
+    assert not out[:n, :, :8].isfinite().any() and out[:n, :, 8:].isfinite().all() and out[n:].isfinite().all()
+    S.take_device_error()
