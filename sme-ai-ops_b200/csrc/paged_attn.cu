@@ -166,8 +166,8 @@ struct Loader {
 // latency (44 GB/s x ~1 us = 44 KB an SM) through the ends of tiles; bound by
 // the cache's bytes.  Measured: 64 requests of 17 to 8192 keys, 32 query and 8
 // key heads of 128: 166 us = 6.3 TB/s; one request of 131001 keys, 4 key heads
-// of 64: 38 us (28 of them here, 5 until the first block is computed, the rest
-// the joining); 24 requests with 2 to 6 drafted tokens (24-row tiles): 54 us =
+// of 64: 38 us (28 of them here, 5 until the first block is computed, 10 the
+// joining); 24 requests with 2 to 6 drafted tokens (24-row tiles): 54 us =
 // 4.3 TB/s, where opening and ending a tile costs 2 to 3 us of a CTA's time.
 
 // 8x8 16-bit transpose across the warp.
@@ -475,7 +475,10 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kPerSm) paged_attn_few_ke
 // ---- more rows, head_dim above 128 ----------------------------------------------
 // Tiles of 64 rows, 16 a warp, every warp through all keys of a block; the
 // query tile stays in shared memory (its fragments would take the registers
-// that the context needs).
+// that the context needs).  Weights are rounded once to the cache's type: the
+// products bound it, and the remainder would add half as many again.  Measured:
+// 2 x 1024 new tokens over 4096 keys, 16 query and 4 key heads of 256: 664 us =
+// 181 TFLOP/s.
 template <int DP>
 constexpr size_t mid_smem() {
   using S = Shape<DP>;
@@ -667,7 +670,7 @@ constexpr int kJoinWarps = 32;
 // a row when there are fewer rows, each taking every w-th piece with a running
 // maximum of its own; a row's warps meet in shared memory in warp order.  The
 // pieces were just written, so they come from L2; bound by the latency of
-// three dependent reads (7 to 8 us alone, 11 for 8 rows of 74 pieces).  Two CTAs
+// three dependent reads (7 to 8 us alone, 10 for 8 rows of 74 pieces).  Two CTAs
 // an SM: all of the few-row kernel's CTAs are joined at once (a second round
 // cost a prompt beside decoding requests 7 of 99 us).
 template <typename T, int TR, int DP>
@@ -799,7 +802,10 @@ int run_join(const AttnParams& p, int sms, cudaStream_t stream) {
 //                         decoding) unless the total says that there are none:
 //                         one row costs the tensor-core kernel's tile as much
 //                         as 128, and 8 requests, one of 860 rows, took 148 us
-//                         without the second kernel and 104 us with it
+//                         without the second kernel and 104 us with it.  Rows
+//                         behind the last request count into the total: padded
+//                         up to n_req * max_new, a step's few rows take the
+//                         tensor-core kernel
 // head_dim above 128: up to 16 rows as above, more the 64-row tiles for all.
 struct Classes {
   int few;      // rows a tile of the few-row kernel; 0: not needed

@@ -10,7 +10,11 @@
 //   O_t += P_t V       tcgen05.mma with P read from TMEM, O fp32 in TMEM
 // The running maximum is only raised when it grows by more than 2^8 (P then
 // stays below 2^8, or 2^15 with half's bias), so O, which has to be rescaled
-// when it is, is touched rarely; the thread that owns the row does it.
+// when it is, is touched rarely; the thread that owns the row does it.  P is
+// rounded once to the cache's type, the only type that an MMA takes beside its
+// values: the result is off by 1.4 times the rounding of the exact one (2.3e-3
+// against 1.7e-3 in bf16).  The remainder as a second P would be half as many
+// MMAs again in a kernel that they bound.
 //
 // Warp roles (12 warps, one CTA an SM):
 //   warps 0-3, 4-7   softmax of half 0 and half 1 (208 registers a thread)
@@ -24,15 +28,15 @@
 // A tile with rows for one half only gives both halves the same rows and deals
 // them the blocks in turn; half 1's maximum, sum and context go through shared
 // memory to half 0 at the end (24 requests of 64 rows over 300 to 4096 keys,
-// 8 key heads of 128: 81.5 -> 77 us).
+// 8 key heads of 128: 81.5 -> 77 us; 69 now, with a tile's cost on the line).
 // While one half's softmax runs, the tensor core works for the other: in issue
 // order PV_0(j), QK_0(j+1), PV_1(j), QK_1(j+1).  At 128 elements a block
 // takes 4 x 128^3 multiply-adds for the tensor core (2048 cycles at its rate)
 // and 2 x 128 x 128 exponentials (2048 cycles at 16 a cycle): the two are
 // nearly in balance, and both halves' softmax has to hide behind the MMAs.
 // Measured: 2 x 2048 new tokens over 8k keys, 32 query and 8 key heads of 128,
-// 428 us = 1071 TFLOP/s, 3500 cycles a block; back to back for seconds 498 us
-// (the board's power limit lowers the clock).  What bounds it: QK reads shared
+// 428 us = 1071 TFLOP/s, 3500 cycles a block; back to back for seconds 482 to
+// 498 us (the board's power limit lowers the clock).  What bounds it: QK reads shared
 // memory at its full 128 bytes a cycle, and the copies of keys and values have
 // to fit beside that.  Slower when tried: two threads a row (16 softmax warps,
 // 523 us), a part of the exponentials as polynomials on the FMA pipe (434 to

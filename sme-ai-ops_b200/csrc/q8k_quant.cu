@@ -92,10 +92,9 @@ __device__ __forceinline__ void norm_quantize_store(float (&t)[8], const float (
 // resid, one write of h and one of the blocks: 13.1 bytes a value.  All loads
 // of a warp (the weight's too) go out together before anything waits; blocks
 // past kKeep a warp are read back from h by the lanes that wrote it.  Measured:
-// 2048 x 4096 25.6 us = 4.3 TB/s, one row 3.0 us; the quantization's
+// 2048 x 4096 27 us = 4.1 TB/s, one row 3.2 us; the quantization's
 // instructions (issue slots 53% busy, mostly waiting between the two barriers)
-// bound it, not the bytes.  No
-// __restrict__ on h: it may be x or resid.
+// bound it, not the bytes.  No __restrict__ on h: it may be x or resid.
 template <int kKeep, bool kWeight, bool kAligned>
 __global__ void __launch_bounds__(512) add_rms_q8k_quantize_kernel(const float* x, int64_t ld_x, const float* resid,
                                                                    int64_t ld_r, int nb, float eps,
@@ -204,9 +203,10 @@ int add_rms_q8k_quantize(const float* x, int64_t ld_x, const float* resid, int64
   uint8_t* out = static_cast<uint8_t*>(y);
   auto wide = [](const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 4 == 0; };
   const bool aligned = wide(x, ld_x) && wide(resid, ld_r) && wide(h, ld_h) && wide(norm_w, 0);
-  // One block a warp up to 16 warps: 2048 rows of 4096 take 25.6 us, with two
+  // One block a warp up to 16 warps: 2048 rows of 4096 take 27 us, with two
   // blocks a warp they took 32.5 us (84 registers a thread leave room for half
-  // the rows).
+  // the rows).  Wider rows have no choice: 2048 rows of 5120, 8192, 11008 take
+  // 53, 67 and 92 us (2.6 to 3.3 TB/s).
   const int warps = nb < 16 ? nb : 16;
   auto run = [&](auto kernel) {
     return launch(kernel, dim3((unsigned)n_rows), dim3(32 * warps), smem, stream, x, ld_x, resid, ld_r, nb, eps, norm_w,
