@@ -663,4 +663,4 @@ def test_attention_of_the_largest_values(cuda, H, K, D, lens):
     out = p.run()
     n = p.lens[0][0]
     assert not out[:n, :, :8].isfinite().any() and out[:n, :, 8:].isfinite().all() and out[n:].isfinite().all()
-    S.take_device_error()
+    assert S.take_device_error() == 0
